@@ -58,7 +58,13 @@ enum lq_status {
  *   MXFP4 : packed [rows,K/32,16] + e8m0 scales [rows,K/32] (crates/larql-models/src/quant/mxfp4.rs:1-9)
  *   NVFP4 : packed [rows,K/16,8] + e4m3 scales [rows,K/16] + f32 tensor scale
  *           (crates/larql-models/src/quant/nvfp4.rs:24-36)                              */
-enum lq_format { LQ_FMT_Q4_K = 0, LQ_FMT_Q8_0 = 1, LQ_FMT_MXFP4 = 2, LQ_FMT_NVFP4 = 3, LQ_FMT_Q6_K = 4 };
+enum lq_format { LQ_FMT_Q4_K = 0, LQ_FMT_Q8_0 = 1, LQ_FMT_MXFP4 = 2, LQ_FMT_NVFP4 = 3, LQ_FMT_Q6_K = 4,
+                 LQ_FMT_FP8_B128 = 5 };
+/*   FP8_B128 : e4m3 codes [rows,K] + one f32 scale per 128 x 128 block, [ceil(rows/128), ceil(K/128)]
+ *           (scales_len in bytes; no counterpart in the reference).  Taken by the layer operators below,
+ *           refused by every other entry point. */
+/* Element types of the layer operators' activations, weights and outputs. */
+enum lq_type { LQ_T_F32 = 0, LQ_T_BF16 = 1, LQ_T_F16 = 2, LQ_T_E4M3 = 3 };
 /* OR-ed into lq_matrix.fmt: data/scales are DEVICE pointers already (resident weights handed to
  * a host-pointer entry point; activations and outputs stay host memory). */
 #define LQ_MAT_DEVICE 0x100
@@ -369,6 +375,63 @@ LQ_API int lq_moe_walk_ffn(lq_ctx* ctx, const lq_matrix* gates, const lq_matrix*
                            size_t n_experts, const float* logits, const float* x, size_t batch, size_t top_e,
                            int renormalise, size_t top_k, uint32_t flags, float* out, uint32_t* expert_idx_out,
                            float* expert_w_out);
+
+/* ---- layer operators beside the walk (no counterpart in the reference) -------------------
+ * Norms around a block, the FP8 product, the whole mixture-of-experts layer.  Sums and statistics are held in 32 bits
+ * or more whatever the element type; a result is rounded once, when it is stored.  The lq_dev_* forms take DEVICE
+ * pointers and enqueue on the context's stream: work on another stream that makes their inputs or takes their
+ * outputs is ordered against lq_stream(ctx) by the caller.  They may be captured into a graph on that stream; what a
+ * call needs of the context's workspace has to be there already then (run the same call once before the capture:
+ * "workspace growth during capture" otherwise), and graphs of one context share that workspace, so they are
+ * replayed one after another.  Workspace a graph may hold stays allocated until lq_destroy.
+ *
+ * lq_dev_block_norm: the norms before and after a block, its gate and residual scale, in one pass over the rows:
+ *     z  = y / rms(y) * (w_offset + post_w)           z = y when post_norm is 0; post_w NULL: unit weight
+ *     h' = h_scale * h + y_scale * gate * z           gate NULL: 1; y NULL: h' = h_scale * h
+ *     n  = h' / rms(h') * (w_offset + pre_w)          rms(v) = sqrt(mean(v^2) + eps); pre_w NULL: unit weight
+ * (run_ffn's norm and residual add, crates/larql-compute/src/forward/layer.rs:61-127, with learned weights, the norm
+ * behind the block, gate and scale).  n is taken from the unrounded h'.  h_out or n_out may be NULL (not written), and
+ * each may be the very rows of h or y (same pointer and stride; else nothing may overlap).  gate is [gate rows,
+ * gate_cols], gate_cols 1 (a scalar per row) or cols; row r uses gate row r / gate_group.  Strides count elements
+ * between rows; the padding behind a row is left as it is.  eps >= 2^-126, cols <= 16384. */
+typedef struct lq_block_norm_args {
+    int32_t type;    /* LQ_T_F32 / BF16 / F16: h, y, gate, h_out, n_out */
+    int32_t w_type;  /* LQ_T_F32 / BF16 / F16: post_w, pre_w */
+    int32_t post_norm;
+    float w_offset, h_scale, y_scale;
+    double eps;
+    size_t rows, cols;
+    const void* h;
+    size_t h_stride;
+    const void* y;
+    size_t y_stride;
+    const void *post_w, *pre_w;
+    const void* gate;
+    size_t gate_cols, gate_stride, gate_group;
+    void* h_out;
+    size_t h_out_stride;
+    void* n_out;
+    size_t n_out_stride;
+} lq_block_norm_args;
+LQ_API int lq_dev_block_norm(lq_ctx* ctx, const lq_block_norm_args* args);
+
+/* FP8 activations: per token and 128 columns, scale = max(amax / 448, 2^-126) and code = e4m3(x / scale), both
+ * divisions rounded to f32, the code to nearest even.  x [tokens, cols] of LQ_T_F32 / BF16 / F16, x_stride
+ * elements between tokens; codes [tokens, cols], scales [tokens, ceil(cols / 128)].  A NaN or infinity makes its
+ * block's products NaN. */
+LQ_API int lq_dev_fp8_quantize(lq_ctx* ctx, const void* x, int x_type, size_t tokens, size_t cols, size_t x_stride,
+                               uint8_t* codes, float* scales);
+
+/* out[t, r] = sum_b sx[t,b] sw[r/128,b] sum_{k in block b} qx[t,k] qw[r,k] for an LQ_FMT_FP8_B128 matrix (device
+ * resident, LQ_MAT_DEVICE).  x is quantised on the way as lq_dev_fp8_quantize does (x_scales NULL), or holds codes
+ * already: x_type LQ_T_E4M3 with x_scales [tokens, ceil(cols / 128)] (16-byte aligned, x_stride a multiple of 16).
+ * cols is a multiple of 16, the matrix's codes 16-byte aligned.  out [tokens, rows] of LQ_T_F32 / BF16 / F16,
+ * out_stride elements between tokens; it may not overlap an input. */
+LQ_API int lq_dev_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const void* x, int x_type, const float* x_scales,
+                             size_t tokens, size_t x_stride, void* out, int out_type, size_t out_stride);
+/* The same with host pointers, f32 in and out (as lq_q4k_matmul): x [tokens, cols] -> out [tokens, rows]. */
+LQ_API int lq_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const float* x, size_t x_len, size_t tokens, float* out,
+                         size_t out_len);
 
 /* ---- allocation-free entry point ---------------------------------------------------- */
 /* Has no counterpart in the reference.  A Q4_K matvec (same arithmetic and kernels as

@@ -22,7 +22,8 @@ import numpy as np
 _HERE = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("LARQL_B200_LIB") or (_HERE / "liblarql_b200.so"))  # override: a tuning build
 
-FMT_Q4_K, FMT_Q8_0, FMT_MXFP4, FMT_NVFP4, FMT_Q6_K = 0, 1, 2, 3, 4
+FMT_Q4_K, FMT_Q8_0, FMT_MXFP4, FMT_NVFP4, FMT_Q6_K, FMT_FP8_B128 = 0, 1, 2, 3, 4, 5
+T_F32, T_BF16, T_F16, T_E4M3 = 0, 1, 2, 3  # element types of the layer operators
 MAT_DEVICE = 0x100  # OR-ed into a matrix format: data/scales are device pointers
 WALK_RMSNORM, WALK_RESIDUAL, WALK_FORCE_SPARSE = 1, 2, 4
 
@@ -44,7 +45,7 @@ EXPORTS = [
     "lq_gemv16_topk", "lq_f16_gemv_topk", "lq_comm_unique_id", "lq_comm_init", "lq_comm_destroy",
     "lq_stack_create_sharded", "lq_stack_path", "lq_q6k_matvec", "lq_dequantize_q6k", "lq_q4k_dual_matvec",
     "lq_k_quant_padded_cols", "lq_vindex_open", "lq_vindex_num_layers", "lq_vindex_layer", "lq_vindex_close",
-    "lq_nvfp4_pack_split",
+    "lq_nvfp4_pack_split", "lq_dev_block_norm", "lq_dev_fp8_quantize", "lq_dev_fp8_matmul", "lq_fp8_matmul",
 ]
 
 
@@ -60,6 +61,17 @@ class LqMatrix(C.Structure):
 class WalkStats(C.Structure):
     _fields_ = [("n_certain", C.c_int32), ("n_band", C.c_int32), ("n_hits", C.c_int32), ("need", C.c_int32),
                 ("tau", C.c_float), ("bound", C.c_float)]
+
+
+class BlockNormArgs(C.Structure):
+    """Operands of dev_block_norm (pointers are device addresses; a field left out is 0 / NULL):
+    z = post norm of y, h' = h_scale h + y_scale gate z, n = norm of h'.  Keep one per layer and call with it."""
+    _fields_ = [("type", C.c_int32), ("w_type", C.c_int32), ("post_norm", C.c_int32), ("w_offset", C.c_float),
+                ("h_scale", C.c_float), ("y_scale", C.c_float), ("eps", C.c_double), ("rows", C.c_size_t),
+                ("cols", C.c_size_t), ("h", C.c_void_p), ("h_stride", C.c_size_t), ("y", C.c_void_p),
+                ("y_stride", C.c_size_t), ("post_w", C.c_void_p), ("pre_w", C.c_void_p), ("gate", C.c_void_p),
+                ("gate_cols", C.c_size_t), ("gate_stride", C.c_size_t), ("gate_group", C.c_size_t),
+                ("h_out", C.c_void_p), ("h_out_stride", C.c_size_t), ("n_out", C.c_void_p), ("n_out_stride", C.c_size_t)]
 
 
 _lib = None
@@ -140,6 +152,10 @@ def load_library() -> C.CDLL:
         "lq_bf16_gemv": (C.c_int, [vp, vp, sz, f32p, sz, sz, sz, f32p]),
         "lq_q4k_matvec_topk": (C.c_int, [vp, vp, sz, f32p, sz, sz, sz, sz, u32p, f32p, C.POINTER(sz)]),
         "lq_gemv16_topk": (C.c_int, [vp, C.c_int, vp, sz, f32p, sz, sz, sz, sz, u32p, f32p, C.POINTER(sz)]),
+        "lq_dev_block_norm": (C.c_int, [vp, C.POINTER(BlockNormArgs)]),
+        "lq_dev_fp8_quantize": (C.c_int, [vp, vp, C.c_int, sz, sz, sz, vp, vp]),
+        "lq_dev_fp8_matmul": (C.c_int, [vp, mp, vp, C.c_int, vp, sz, sz, vp, C.c_int, sz]),
+        "lq_fp8_matmul": (C.c_int, [vp, mp, f32p, sz, sz, f32p, sz]),
         "lq_f16_gemv_topk": (C.c_int, [vp, vp, sz, f32p, sz, sz, sz, sz, u32p, f32p, C.POINTER(sz)]),
     }
     for name, (res, args) in sig.items():
@@ -168,6 +184,8 @@ class HostMatrix:
     def __init__(self, fmt: int, rows: int, cols: int, data, scales=None, tensor_scale: float = 1.0):
         self.fmt, self.rows, self.cols = int(fmt), int(rows), int(cols)
         self.data = _u8(data)
+        if self.fmt == FMT_FP8_B128 and scales is not None:  # f32 scales, held as their bytes
+            scales = np.ascontiguousarray(scales, np.float32).view(np.uint8).reshape(-1)
         self.scales = _u8(scales) if scales is not None else None
         self.tensor_scale = float(tensor_scale)
 
@@ -576,6 +594,35 @@ class CudaBackend:
         ok = self._status(self._lib.lq_profile_walk(self._h, C.byref(g), C.byref(u), C.byref(d), x_ptr, int(top_k),
                                                     flags, out_ptr, ms))
         return list(ms) if ok else None
+
+    # -- layer operators (device pointers, enqueued on the context's stream) -----------
+    def dev_block_norm(self, args: "BlockNormArgs"):
+        """Norm behind a block, gate, residual and the next norm in one pass (lq_dev_block_norm)."""
+        return self._status(self._lib.lq_dev_block_norm(self._h, args))
+
+    def dev_fp8_quantize(self, x_ptr: int, x_type: int, tokens: int, cols: int, x_stride: int, codes_ptr: int,
+                         scales_ptr: int):
+        """e4m3 codes [tokens, cols] and one f32 scale per token and 128 columns."""
+        return self._status(self._lib.lq_dev_fp8_quantize(self._h, x_ptr, x_type, tokens, cols, x_stride, codes_ptr,
+                                                          scales_ptr))
+
+    def dev_fp8_matmul(self, w: DeviceMatrix, x_ptr: int, x_type: int, tokens: int, x_stride: int, out_ptr: int,
+                       out_type: int, out_stride: int, x_scales_ptr: int = 0):
+        """out [tokens, w.rows] = x . w^T for an FMT_FP8_B128 matrix; x is quantised on the way, or holds e4m3 codes
+        (x_type T_E4M3) with their scales."""
+        return self._status(self._lib.lq_dev_fp8_matmul(self._h, w.c(), x_ptr, x_type, x_scales_ptr or None, tokens,
+                                                        x_stride, out_ptr, out_type, out_stride))
+
+    def fp8_matmul(self, w: HostMatrix, x):
+        """x [tokens, cols] (host, f32) . w^T for an FMT_FP8_B128 matrix; None on a refusal."""
+        x = _f32(x)
+        x2 = x.reshape(-1, x.shape[-1])
+        out = np.empty((x2.shape[0], w.rows), np.float32)
+        if x2.shape[1] != w.cols:
+            return None
+        m = w.c()
+        ok = self._status(self._lib.lq_fp8_matmul(self._h, C.byref(m), _ptr(x2), x2.size, x2.shape[0], _ptr(out), out.size))
+        return out.reshape(*x.shape[:-1], w.rows) if ok else None
 
     # -- feature-sharded walk: the steps between the collectives --------------------
     def dev_shard_scan(self, gate, x_ptr: int, flags: int, rank: int, world: int, hist_ptr: int):

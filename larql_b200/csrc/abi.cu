@@ -114,6 +114,14 @@ struct lq_ctx {
     // multi-GPU: one NCCL communicator per context (lq_comm_init)
     ncclComm_t comm = nullptr;
     int rank = 0, world = 1;
+    // layer operators: FP8 activations (codes, scales), partial tiles and their counters.  Captured graphs hold
+    // these addresses, so a buffer that is outgrown is kept until the context goes.
+    struct OpBuf {
+        uint8_t* p = nullptr;
+        size_t cap = 0;
+    };
+    OpBuf op_codes, op_part, op_done;
+    std::vector<void*> retired;
     const lq_stack* last_xstack = nullptr;  // sharded fused stack that ran last (its selection: lq_dev_shard_hits)
 };
 
@@ -345,6 +353,28 @@ int ensure_sort(lq_ctx* ctx, size_t n) {
     return LQ_OK;
 }
 
+// Workspace of the layer operators: at least `bytes` in b, zeroed when it is new.
+int ensure_op(lq_ctx* ctx, lq_ctx::OpBuf& b, size_t bytes) {
+    if (bytes <= b.cap) return LQ_OK;
+    cudaStreamCaptureStatus cs;
+    CK(cudaStreamIsCapturing(ctx->stream, &cs));
+    if (cs != cudaStreamCaptureStatusNone) return fail(ctx, LQ_ERR_ARGUMENT, "workspace growth during capture");
+    ctx->retired.reserve(ctx->retired.size() + 1);
+    const size_t cap = a256(std::max(bytes, 2 * b.cap));
+    uint8_t* p = nullptr;
+    cudaError_t e = cudaMalloc(&p, cap);
+    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, cap, ctx->stream);
+    if (e != cudaSuccess) {
+        cudaGetLastError();  // (not a launch's error)
+        if (p) cudaFree(p);
+        return cuda_fail(ctx, e, "layer operator workspace");
+    }
+    if (b.p) ctx->retired.push_back(b.p);
+    b.p = p;
+    b.cap = cap;
+    return LQ_OK;
+}
+
 // Device copy of a host weight range: inside a registered region, else cached on first use
 // by (address, length) — the reference GPU backend's buffer-cache rule.
 int resolve(lq_ctx* ctx, const void* host, size_t len, const uint8_t** dev) {
@@ -409,9 +439,27 @@ int check_device_err(lq_ctx* ctx) {
     CK(cudaMemsetAsync(ctx->d_err, 0, sizeof(int), ctx->stream));
     // a failed fused launch may leave its histogram / counters dirty
     if (ctx->fws) CK(cudaMemsetAsync(ctx->fws, 0, fused_q4k_ws_dirty_bytes(), ctx->stream));
+    if (ctx->op_done.p) CK(cudaMemsetAsync(ctx->op_done.p, 0, ctx->op_done.cap, ctx->stream));
     if (h == DEV_ERR_NAN_SCORE) return fail(ctx, LQ_ERR_NAN_SCORE, "NaN gate score or non-finite activation");
     if (h == DEV_ERR_TMA_TIMEOUT) return fail(ctx, LQ_ERR_TIMEOUT, "a bounded device-side wait ran out");
     return fail(ctx, LQ_ERR_CUDA, "device-side internal error");
+}
+
+bool float_type(int t) { return t == LQ_T_F32 || t == LQ_T_BF16 || t == LQ_T_F16; }
+size_t type_bytes(int t) { return t == LQ_T_F32 ? 4 : (t == LQ_T_E4M3 ? 1 : 2); }
+
+// An FP8_B128 matrix, host or device resident: [rows, cols] codes and the blocks' f32 scales.
+int check_fp8(lq_ctx* ctx, const lq_matrix* m, const char* name) {
+    if ((m->fmt & 0xff) != LQ_FMT_FP8_B128) return fail(ctx, LQ_REFUSED_UNSUPPORTED, std::string(name) + ": not an FP8_B128 matrix");
+    if (m->rows < 0 || m->cols < 0 || m->cols % 16 != 0 || m->rows > 0x40000000 || m->cols > 0x40000000)
+        return fail(ctx, LQ_REFUSED_SHAPE, std::string(name) + ": FP8_B128 geometry");
+    const size_t r = (size_t)m->rows, k = (size_t)m->cols;
+    if (m->data_len < r * k || m->scales_len < (r + 127) / 128 * ((k + 127) / 128) * 4)
+        return fail(ctx, LQ_REFUSED_SHAPE, std::string(name) + ": FP8_B128 lengths");
+    if (r && k && (!m->data || !m->scales)) return fail(ctx, LQ_ERR_ARGUMENT, std::string(name) + ": null data");
+    if ((m->fmt & LQ_MAT_DEVICE) && (((uintptr_t)m->data & 15) || ((uintptr_t)m->scales & 3)))
+        return fail(ctx, LQ_ERR_ARGUMENT, std::string(name) + ": FP8_B128 codes not 16-byte aligned");
+    return LQ_OK;
 }
 
 XPrep xprep_of(const TokenWs& w) { return XPrep{w.xn, w.xa, w.xb, w.bscale, w.bsum, w.babs}; }
@@ -768,6 +816,8 @@ void lq_destroy(lq_ctx* ctx) {
     cudaFree(ctx->fws);
     cudaFree(ctx->stats_dev);
     cudaFree(ctx->tc_scratch);
+    for (lq_ctx::OpBuf* b : {&ctx->op_codes, &ctx->op_part, &ctx->op_done}) cudaFree(b->p);
+    for (void* p : ctx->retired) cudaFree(p);
     cudaFree(ctx->stage);
     cudaFree(ctx->sort_buf);
     cudaFree(ctx->d_err);
@@ -2223,6 +2273,143 @@ void lq_stack_destroy(lq_ctx* ctx, lq_stack* s) {
     if (s->xarea) cudaFree(s->xarea);
     if (s->xhits) cudaFree(s->xhits);
     delete s;
+}
+
+// ------------------------------------------------------------ layer operators ----
+int lq_dev_block_norm(lq_ctx* ctx, const lq_block_norm_args* q) {
+    DevGuard dev_guard(ctx);
+    if (!ctx || !q) return LQ_ERR_ARGUMENT;
+    if (!float_type(q->type) || !float_type(q->w_type)) return fail(ctx, LQ_REFUSED_UNSUPPORTED, "block_norm: element type");
+    if (q->rows == 0 || q->cols == 0) return LQ_OK;
+    if (q->cols > 16384) return fail(ctx, LQ_REFUSED_UNSUPPORTED, "block_norm: cols > 16384");
+    if (q->rows > 0x7fffffffu) return fail(ctx, LQ_REFUSED_UNSUPPORTED, "block_norm: too many rows");
+    if (!(q->eps >= 0x1p-126) || !std::isfinite(q->eps)) return fail(ctx, LQ_ERR_ARGUMENT, "block_norm: eps below 2^-126 or not finite");
+    if (!q->h || (!q->h_out && !q->n_out)) return fail(ctx, LQ_ERR_ARGUMENT, "block_norm: null h or no output");
+    if (!q->y && (q->post_norm || q->gate)) return fail(ctx, LQ_ERR_ARGUMENT, "block_norm: post norm or gate without a block output");
+    const size_t z = type_bytes(q->type), wz = type_bytes(q->w_type);
+    auto odd = [](const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) != 0; };
+    if (odd(q->h, z) || odd(q->y, z) || odd(q->gate, z) || odd(q->h_out, z) || odd(q->n_out, z) || odd(q->post_w, wz) ||
+        odd(q->pre_w, wz))
+        return fail(ctx, LQ_ERR_ARGUMENT, "block_norm: pointer not aligned to its elements");
+    const bool many = q->rows > 1;
+    if (many && (q->h_stride < q->cols || (q->y && q->y_stride < q->cols) || (q->h_out && q->h_out_stride < q->cols) ||
+                 (q->n_out && q->n_out_stride < q->cols)))
+        return fail(ctx, LQ_REFUSED_SHAPE, "block_norm: row stride below cols");
+    if (q->gate && ((q->gate_cols != 1 && q->gate_cols != q->cols) || q->gate_group == 0))
+        return fail(ctx, LQ_REFUSED_SHAPE, "block_norm: gate_cols is 1 or cols, gate_group at least 1");
+    if (q->gate && q->gate_group < q->rows && q->gate_stride < q->gate_cols)
+        return fail(ctx, LQ_REFUSED_SHAPE, "block_norm: gate stride below gate_cols");
+    BlockNorm a;
+    a.h = q->h, a.y = q->y, a.post_w = q->post_w, a.pre_w = q->pre_w, a.gate = q->gate;
+    a.h_out = q->h_out, a.n_out = q->n_out;
+    a.h_stride = (long long)q->h_stride, a.y_stride = (long long)q->y_stride, a.gate_stride = (long long)q->gate_stride;
+    a.h_out_stride = (long long)q->h_out_stride, a.n_out_stride = (long long)q->n_out_stride;
+    a.gate_group = (long long)std::min<size_t>(std::max<size_t>(q->gate_group, 1), 0x7fffffffu);
+    a.rows = (int)q->rows, a.cols = (int)q->cols, a.gate_cols = (int)q->gate_cols;
+    a.w_type = q->w_type, a.post_norm = q->post_norm != 0;
+    a.w_offset = q->w_offset, a.h_scale = q->h_scale, a.y_scale = q->y_scale, a.eps = q->eps;
+    CK(launch_block_norm(a, q->type, ctx->sm_count, ctx->stream));
+    ctx->launches += 1;
+    return LQ_OK;
+}
+
+int lq_dev_fp8_quantize(lq_ctx* ctx, const void* x, int x_type, size_t tokens, size_t cols, size_t x_stride, uint8_t* codes,
+                        float* scales) {
+    DevGuard dev_guard(ctx);
+    if (!ctx) return LQ_ERR_ARGUMENT;
+    if (!float_type(x_type)) return fail(ctx, LQ_REFUSED_UNSUPPORTED, "fp8_quantize: element type");
+    if (tokens == 0 || cols == 0) return LQ_OK;
+    if (!x || !codes || !scales) return fail(ctx, LQ_ERR_ARGUMENT, "fp8_quantize: null pointer");
+    if (((uintptr_t)x & (type_bytes(x_type) - 1)) || ((uintptr_t)scales & 3))
+        return fail(ctx, LQ_ERR_ARGUMENT, "fp8_quantize: pointer not aligned to its elements");
+    if (tokens > 0x7fffffffu || cols > 0x7fffff00u) return fail(ctx, LQ_REFUSED_UNSUPPORTED, "fp8_quantize: size");
+    if (tokens > 1 && x_stride < cols) return fail(ctx, LQ_REFUSED_SHAPE, "fp8_quantize: row stride below cols");
+    CK(launch_fp8_quantize(x, x_type, tokens, cols, x_stride, codes, cols, scales, ctx->sm_count, ctx->stream));
+    ctx->launches += 1;
+    return LQ_OK;
+}
+
+int lq_dev_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const void* x, int x_type, const float* x_scales, size_t tokens,
+                      size_t x_stride, void* out, int out_type, size_t out_stride) {
+    DevGuard dev_guard(ctx);
+    if (!ctx || !w) return LQ_ERR_ARGUMENT;
+    int rc = check_fp8(ctx, w, "fp8_matmul");
+    if (rc) return rc;
+    if (!(w->fmt & LQ_MAT_DEVICE)) return fail(ctx, LQ_ERR_ARGUMENT, "fp8_matmul: the matrix is not device resident");
+    const bool coded = x_type == LQ_T_E4M3;
+    if ((!coded && !float_type(x_type)) || !float_type(out_type))
+        return fail(ctx, LQ_REFUSED_UNSUPPORTED, "fp8_matmul: element type");
+    if (coded != (x_scales != nullptr))
+        return fail(ctx, LQ_ERR_ARGUMENT, "fp8_matmul: x_scales go with e4m3 activations and with nothing else");
+    const size_t rows = (size_t)w->rows, cols = (size_t)w->cols;
+    if (tokens == 0 || rows == 0) return LQ_OK;
+    if (!out || (!x && cols)) return fail(ctx, LQ_ERR_ARGUMENT, "fp8_matmul: null pointer");
+    if (tokens > 0x7fffffffu) return fail(ctx, LQ_REFUSED_UNSUPPORTED, "fp8_matmul: too many tokens");
+    if (tokens > 1 && (x_stride < cols || out_stride < rows))
+        return fail(ctx, LQ_REFUSED_SHAPE, "fp8_matmul: row stride below the row");
+    const size_t oz = type_bytes(out_type);
+    if (((uintptr_t)out & (oz - 1)) || (!coded && ((uintptr_t)x & (type_bytes(x_type) - 1))) || ((uintptr_t)x_scales & 3))
+        return fail(ctx, LQ_ERR_ARGUMENT, "fp8_matmul: pointer not aligned to its elements");
+    if (coded && (((uintptr_t)x & 15) || (tokens > 1 && (x_stride & 15))))
+        return fail(ctx, LQ_ERR_ARGUMENT, "fp8_matmul: e4m3 activations need 16-byte aligned rows");
+    if (cols == 0) {
+        CK(cudaMemset2DAsync(out, out_stride * oz, 0, rows * oz, tokens, ctx->stream));
+        return LQ_OK;
+    }
+    const size_t kb = (cols + 127) / 128, chunk = 32768;  // (bounds the codes' workspace)
+    for (size_t t0 = 0; t0 < tokens; t0 += chunk) {
+        const size_t n = std::min(chunk, tokens - t0);
+        Fp8Product p;
+        p.w = (const uint8_t*)w->data;
+        p.w_scales = (const float*)w->scales;
+        p.rows = rows, p.cols = cols, p.tokens = n;
+        p.out = (uint8_t*)out + t0 * out_stride * oz;
+        p.out_stride = out_stride, p.out_type = out_type;
+        if (coded) {
+            p.codes = (const uint8_t*)x + t0 * x_stride;
+            p.code_pitch = n > 1 ? x_stride : (cols + 15) / 16 * 16;
+            p.scales = x_scales + t0 * kb;
+        } else {
+            const size_t pitch = cols;  // a multiple of 16
+            if ((rc = ensure_op(ctx, ctx->op_codes, a256(n * pitch) + n * kb * 4))) return rc;
+            p.codes = ctx->op_codes.p;
+            p.code_pitch = pitch;
+            p.scales = (const float*)(ctx->op_codes.p + a256(n * pitch));
+        }
+        if ((rc = ensure_op(ctx, ctx->op_part, fp8_part_bytes(n, ctx->sm_count)))) return rc;
+        if ((rc = ensure_op(ctx, ctx->op_done, fp8_tile_count(n, rows) * sizeof(unsigned)))) return rc;
+        p.part = (float*)ctx->op_part.p;
+        p.done = (unsigned*)ctx->op_done.p;
+        if (!coded) {
+            CK(launch_fp8_quantize((const uint8_t*)x + t0 * x_stride * type_bytes(x_type), x_type, n, cols, x_stride,
+                                   const_cast<uint8_t*>(p.codes), p.code_pitch, const_cast<float*>(p.scales), ctx->sm_count,
+                                   ctx->stream));
+            ctx->launches += 1;
+        }
+        CK(launch_fp8_matmul(p, !coded, ctx->sm_count, ctx->d_err, ctx->stream));
+        ctx->launches += 1;
+    }
+    return LQ_OK;
+}
+
+int lq_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const float* x, size_t x_len, size_t tokens, float* out, size_t out_len) {
+    DevGuard dev_guard(ctx);
+    if (!ctx || !w) return LQ_ERR_ARGUMENT;
+    int rc = check_fp8(ctx, w, "fp8_matmul");
+    if (rc) return rc;
+    const size_t rows = (size_t)w->rows, cols = (size_t)w->cols;
+    if (x_len != tokens * cols || out_len != tokens * rows) return fail(ctx, LQ_REFUSED_SHAPE, "fp8_matmul: lengths");
+    if (out_len == 0) return LQ_OK;
+    if (!out || (!x && x_len)) return fail(ctx, LQ_ERR_ARGUMENT, "fp8_matmul: null pointer");
+    lq_matrix dm;
+    if ((rc = resolve_matrix(ctx, w, &dm))) return rc;
+    dm.fmt |= LQ_MAT_DEVICE;
+    if ((rc = ensure_stage(ctx, a256(x_len * 4) + out_len * 4))) return rc;
+    float *dx = (float*)ctx->stage, *dout = (float*)(ctx->stage + a256(x_len * 4));
+    if (x_len) CK(cudaMemcpyAsync(dx, x, x_len * 4, cudaMemcpyHostToDevice, ctx->stream));
+    if ((rc = lq_dev_fp8_matmul(ctx, &dm, dx, LQ_T_F32, nullptr, tokens, cols, dout, LQ_T_F32, rows))) return rc;
+    CK(cudaMemcpyAsync(out, dout, out_len * 4, cudaMemcpyDeviceToHost, ctx->stream));
+    return lq_synchronize(ctx);
 }
 
 }  // extern "C"

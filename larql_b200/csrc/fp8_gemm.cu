@@ -1,0 +1,682 @@
+// Matrix product in 8-bit floating point with one scale per block of 128 (lq_dev_fp8_matmul), and the quantisation
+// of its activations (lq_dev_fp8_quantize):
+//
+//   out[t, r] = sum_b sx[t, b] * sw[r / 128, b] * sum_{k in block b} qx[t, k] * qw[r, k]
+//
+// with qx, qw in e4m3, sx one f32 per token and 128 columns, sw one f32 per 128 x 128 block of the weight.  The
+// scales change along the contraction, so a block's 128-long partial product (four K = 32 steps of tcgen05.mma
+// kind::f8f6f4, f32 accumulators in tensor memory) is read back, multiplied by its scale and added to an f32
+// accumulator in registers, while the tensor core works on the next block in another accumulator buffer.  The
+// partial products are exact sums of 8-bit products in f32; every other operation is one f32 fused multiply-add.
+//
+// Two kernels, chosen by the number of tokens (launch_fp8_matmul has the rule and what both measured):
+//   fp8_few_kernel    rows of the weight are the 128 lanes of an accumulator, tokens its 16..128 columns.  What
+//                     bounds it is reading the weight, so the (row tile, k block) units are dealt out evenly over
+//                     the SMs in one contiguous run each, and tiles that end inside a run are joined through a
+//                     workspace by the last CTA to finish its piece, always in the order of k: results do not
+//                     depend on timing.
+//   fp8_many_kernel   tokens are the lanes, 256 rows of the weight the columns: the scale of a lane and block is one
+//                     number per thread, one fused multiply-add per value.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "../../include/larql_cuda.h"
+#include "kernels.h"
+#include "tc5.cuh"
+
+namespace lq {
+
+namespace {
+
+constexpr float F8_MAX = 448.0f;
+constexpr float F8_MIN_SCALE = 1.17549435e-38f;  // 2^-126: a zero block gets a scale too
+
+__device__ __forceinline__ float ld_f32(const float* p) { return *p; }
+__device__ __forceinline__ float ld_f32(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float ld_f32(const __half* p) { return __half2float(*p); }
+
+__device__ __forceinline__ void ld8(const float* p, float (&v)[8]) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void ld8(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void ld8(const __half* p, float (&v)[8]) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN wins: it must reach the scale
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+    unsigned short r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// 16 threads per (token, block of 128), 8 consecutive elements each.  The quotient is the correctly rounded one
+// (and not x times 1 / s): the codes are defined by it, and the tests hold them to the definition bit for bit.
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__ x, long long x_stride, long long units,
+                                                           int kb_n, int cols, uint8_t* __restrict__ codes,
+                                                           long long code_pitch, float* __restrict__ scales, int wide_store) {
+    pdl_launch_next();
+    const int sub = threadIdx.x & 15;
+    for (long long u0 = (long long)blockIdx.x * 16; u0 < units; u0 += (long long)gridDim.x * 16) {
+        const long long u = u0 + (threadIdx.x >> 4);
+        const bool on = u < units;
+        const long long t = on ? u / kb_n : 0;
+        const int kb = on ? (int)(u - t * kb_n) : 0, k0 = kb * 128 + sub * 8;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        if (on) {
+            const T* p = x + t * x_stride + k0;
+            if (VEC) {
+                if (k0 < cols) ld8(p, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (k0 + i < cols) v[i] = ld_f32(p + i);
+            }
+        }
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(v[i]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float s = max_nan(__fdiv_rn(m, F8_MAX), F8_MIN_SCALE);
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = e4m3x2(__fdiv_rn(v[2 * i], s), __fdiv_rn(v[2 * i + 1], s));
+        if (on) {
+            if (sub == 0) scales[t * kb_n + kb] = s;
+            uint8_t* q = codes + t * code_pitch + k0;
+            if (wide_store) {  // cols (and the pitch) are multiples of 8
+                if (k0 < cols) *reinterpret_cast<uint2*>(q) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (k0 + i < cols) q[i] = (uint8_t)(w[i >> 1] >> (8 * (i & 1)));
+            }
+        }
+    }
+}
+
+template <class T>
+__device__ __forceinline__ T narrow(float v);
+template <>
+__device__ __forceinline__ float narrow<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ void store_as(void* out, int type, size_t at, float v) {
+    if (type == LQ_T_F32) static_cast<float*>(out)[at] = v;
+    else if (type == LQ_T_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(out)[at] = __float2half_rn(v);
+}
+
+// What both kernels are told.
+struct F8Args {
+    const float* sx;   // [tokens][kb_n]
+    const float* sw;   // [ceil(rows / 128)][kb_n]
+    void* out;
+    long long out_stride;
+    int out_type;
+    int tokens, rows, kb_n;
+    float* part;       // few-token kernel: [grid][2][NT][128] partial tiles
+    unsigned* done;    // few-token kernel: k blocks finished per tile (zero between launches)
+    int* err;
+};
+
+// ------------------------------------------------------------ few tokens ----
+constexpr int FEW_BUFS = 4;  // accumulator buffers in tensor memory
+
+constexpr int few_stage_bytes(int nt) { return 128 * 128 + nt * 128; }
+constexpr int few_stages(int nt) { return nt <= 16 ? 11 : (nt <= 32 ? 10 : (nt <= 64 ? 8 : 6)); }
+constexpr int few_promo_warps(int nt) { return nt <= 64 ? 4 : 8; }
+constexpr int few_threads(int nt) { return 64 + 32 * few_promo_warps(nt); }
+
+template <int NT>
+struct FewSmem {
+    uint64_t full[few_stages(NT)], empty[few_stages(NT)];
+    uint64_t acc_full[FEW_BUFS], acc_empty[FEW_BUFS];
+    float sx[few_promo_warps(NT)][2][NT];  // the scales of a k block's tokens, per warp
+    uint32_t tmem;
+    int failed;
+    int last;
+};
+
+template <int NT>
+__global__ void __launch_bounds__(few_threads(NT), 1)
+fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const F8Args a) {
+    constexpr int STAGES = few_stages(NT), STAGE = few_stage_bytes(NT), PW = few_promo_warps(NT);
+    constexpr int COLS = NT * 4 / PW;  // columns (tokens) per promoting warp: all of them with one warpgroup
+    constexpr uint32_t TMEM_COLS = NT * FEW_BUFS < 32 ? 32 : NT * FEW_BUFS;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    FewSmem<NT>& sh = *reinterpret_cast<FewSmem<NT>*>(ring + STAGES * STAGE);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tok_tiles = (a.tokens + NT - 1) / NT, row_tiles = (a.rows + 127) / 128;
+    const long long units = (long long)row_tiles * tok_tiles * a.kb_n;
+    const long long u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+
+    if (tid == 0) {
+        for (int i = 0; i < STAGES; ++i) {
+            mbar_init(&sh.full[i], 1);
+            mbar_init(&sh.empty[i], 1);
+        }
+        for (int i = 0; i < FEW_BUFS; ++i) {
+            mbar_init(&sh.acc_full[i], 1);
+            mbar_init(&sh.acc_empty[i], PW * 32);
+        }
+        sh.failed = 0;
+        fence_mbar_init();
+        tma_prefetch_map(&map_w);
+        tma_prefetch_map(&map_x);
+    }
+    if (warp == 1) tmem_alloc(&sh.tmem, TMEM_COLS);
+    tc5_fence_before();
+    __syncthreads();
+    tc5_fence_after();
+    const uint32_t tmem = sh.tmem;
+
+    if (warp == 0) {
+        // ---- producer: weight and token tiles of the run's units ----
+        if (lane == 0) {
+            auto coords = [&](long long u, int& row, int& tok, int& k) {
+                const long long tile = u / a.kb_n;
+                k = (int)(u - tile * a.kb_n) * 128;
+                row = (int)(tile / tok_tiles) * 128;
+                tok = (int)(tile % tok_tiles) * NT;
+            };
+            // the weight does not depend on the kernel before this one (the quantisation of the tokens)
+            const long long head = min(u1, u0 + STAGES);
+            int row, tok, k;
+            for (long long u = u0; u < head; ++u) {
+                const int st = (int)(u - u0);
+                coords(u, row, tok, k);
+                mbar_expect_tx(&sh.full[st], STAGE);
+                tma_load_2d(ring + st * STAGE, &map_w, k, row, &sh.full[st]);
+            }
+            pdl_wait();
+            for (long long u = u0; u < head; ++u) {
+                const int st = (int)(u - u0);
+                coords(u, row, tok, k);
+                tma_load_2d(ring + st * STAGE + 128 * 128, &map_x, k, tok, &sh.full[st]);
+            }
+            bool ok = true;
+            long long u = head;
+            for (; u < u1; ++u) {
+                const int n = (int)(u - u0), st = n % STAGES;
+                if (!mbar_wait(&sh.empty[st], (uint32_t)(n / STAGES - 1) & 1u)) {
+                    ok = false;
+                    break;
+                }
+                coords(u, row, tok, k);
+                mbar_expect_tx(&sh.full[st], STAGE);
+                tma_load_2d(ring + st * STAGE, &map_w, k, row, &sh.full[st]);
+                tma_load_2d(ring + st * STAGE + 128 * 128, &map_x, k, tok, &sh.full[st]);
+            }
+            if (!ok) {  // the copies in flight have to land before the block's shared memory goes away
+                for (long long v = max(u0, u - STAGES); v < u; ++v) {
+                    const int n = (int)(v - u0);
+                    mbar_wait(&sh.full[n % STAGES], (uint32_t)(n / STAGES) & 1u);
+                }
+                sh.failed = 1;
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---- tensor core: one accumulator buffer per k block ----
+        bool ok = true;
+        for (long long u = u0; u < u1; ++u) {
+            const int n = (int)(u - u0), st = n % STAGES, buf = n % FEW_BUFS;
+            ok = mbar_wait(&sh.full[st], (uint32_t)(n / STAGES) & 1u);
+            if (ok && n >= FEW_BUFS) ok = mbar_wait(&sh.acc_empty[buf], (uint32_t)(n / FEW_BUFS - 1) & 1u);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc5_fence_after();
+            if (elect_one()) {
+                const uint32_t sa = smem_u32(ring + st * STAGE), sb = sa + 128 * 128;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    umma_f8(tmem + buf * NT, sw128_desc(sa + 32 * j), sw128_desc(sb + 32 * j), f8_idesc(128, NT), j > 0);
+                umma_commit1(&sh.empty[st]);
+                umma_commit1(&sh.acc_full[buf]);
+            }
+            __syncwarp();
+        }
+        if (!__all_sync(0xffffffffu, ok) && lane == 0) sh.failed = 1;
+    } else {
+        // ---- promotion: thread = row of the weight (TMEM lane); COLS tokens ----
+        pdl_wait();  // the tokens' scales
+        const int pw = warp - 2, quarter = warp & 3, col0 = (pw >> 2) * COLS;
+        const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)col0;
+        float acc[COLS];
+        bool ok = true;
+        long long u = u0;
+        int n = 0;
+        // (a wait that ran out is not waited for again, but the run is walked to its end: the other warps of the
+        // block count on this one at the named barriers, and the tiles' counters have to come out even)
+        while (u < u1) {
+            const long long tile = u / a.kb_n;
+            const int kb_a = (int)(u - tile * a.kb_n);
+            const int kb_b = (int)min((long long)a.kb_n, kb_a + (u1 - u));
+            const int row0 = (int)(tile / tok_tiles) * 128, tok0 = (int)(tile % tok_tiles) * NT;
+            const float* swp = a.sw + (size_t)(row0 >> 7) * a.kb_n;
+            float nx[(COLS + 31) / 32], nw = swp[kb_a];
+            auto fetch = [&](int kb) {
+#pragma unroll
+                for (int i = 0; i < (COLS + 31) / 32; ++i) {
+                    const int c = col0 + i * 32 + lane;
+                    nx[i] = (i * 32 + lane < COLS && tok0 + c < a.tokens) ? a.sx[(size_t)(tok0 + c) * a.kb_n + kb] : 0.0f;
+                }
+            };
+            fetch(kb_a);
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
+            for (int kb = kb_a; kb < kb_b; ++kb, ++n) {
+                const int buf = n % FEW_BUFS;
+                float* sxs = sh.sx[pw][n & 1];
+#pragma unroll
+                for (int i = 0; i < (COLS + 31) / 32; ++i)
+                    if (i * 32 + lane < COLS) sxs[i * 32 + lane] = nx[i] * nw;
+                __syncwarp();
+                if (kb + 1 < kb_b) {
+                    nw = swp[kb + 1];
+                    fetch(kb + 1);
+                }
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[buf], (uint32_t)(n / FEW_BUFS) & 1u));
+                tc5_fence_after();
+#pragma unroll
+                for (int c = 0; c < COLS; c += 16) {
+                    uint32_t v[16];
+                    tmem_load16(tbase + buf * NT + c, v);
+                    tmem_wait16(v);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(__uint_as_float(v[i]), sxs[c + i], acc[c + i]);
+                }
+                tc5_fence_before();
+                mbar_arrive_one(&sh.acc_empty[buf]);
+            }
+            u += kb_b - kb_a;
+            const int row = row0 + quarter * 32 + lane;
+            if (kb_a == 0 && kb_b == a.kb_n) {
+                if (row < a.rows)
+#pragma unroll
+                    for (int i = 0; i < COLS; ++i)
+                        if (tok0 + col0 + i < a.tokens)
+                            store_as(a.out, a.out_type, (size_t)(tok0 + col0 + i) * a.out_stride + row, acc[i]);
+                continue;
+            }
+            // A piece of a tile: into the workspace; the CTA whose piece is the last to arrive adds them all up.
+            auto slot = [&](int cta, long long first) {  // slot 0: the piece the CTA's run begins with
+                return a.part + (((size_t)cta * 2 + (first / a.kb_n == tile ? 0 : 1)) * NT) * 128;
+            };
+            float* mine = slot(blockIdx.x, u0);
+#pragma unroll
+            for (int i = 0; i < COLS; ++i)
+                if (tok0 + col0 + i < a.tokens) __stcg(mine + (size_t)(col0 + i) * 128 + quarter * 32 + lane, acc[i]);
+            __threadfence();
+            asm volatile("bar.sync 1, %0;" ::"n"(PW * 32) : "memory");
+            if (tid == 64) {
+                const unsigned before = atomicAdd(&a.done[tile], (unsigned)(kb_b - kb_a));
+                sh.last = before + (unsigned)(kb_b - kb_a) == (unsigned)a.kb_n;
+                if (sh.last) a.done[tile] = 0;  // ready for the next launch
+                __threadfence();
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(PW * 32) : "memory");
+            const int is_last = sh.last;
+            if (is_last) {
+                const long long t0 = tile * a.kb_n, t1 = t0 + a.kb_n;
+                // the run of CTA c is [units * c / grid, units * (c + 1) / grid)
+                int c = (int)(t0 * gridDim.x / units);
+                while (units * (c + 1) / gridDim.x <= t0) ++c;
+                while (c > 0 && units * c / gridDim.x > t0) --c;
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
+                for (; units * c / gridDim.x < t1; ++c) {
+                    const float* p = slot(c, units * c / gridDim.x);
+#pragma unroll
+                    for (int i = 0; i < COLS; ++i)
+                        if (tok0 + col0 + i < a.tokens) acc[i] += __ldcg(p + (size_t)(col0 + i) * 128 + quarter * 32 + lane);
+                    if (c + 1 >= (int)gridDim.x) break;
+                }
+                if (row < a.rows)
+#pragma unroll
+                    for (int i = 0; i < COLS; ++i)
+                        if (tok0 + col0 + i < a.tokens)
+                            store_as(a.out, a.out_type, (size_t)(tok0 + col0 + i) * a.out_stride + row, acc[i]);
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(PW * 32) : "memory");  // sh.last may be written again
+        }
+        if (!ok && lane == 0) sh.failed = 1;
+    }
+    tc5_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc5_fence_after();
+        tmem_free(tmem, TMEM_COLS);
+    }
+    if (tid == 0 && sh.failed) set_err(a.err, DEV_ERR_TMA_TIMEOUT);
+}
+
+// ----------------------------------------------------------- many tokens ----
+constexpr int MANY_M = 128, MANY_N = 256, MANY_STAGES = 4;
+constexpr int MANY_STAGE = (MANY_M + MANY_N) * 128;
+constexpr int MANY_THREADS = 64 + 256;
+
+struct ManySmem {
+    uint64_t full[MANY_STAGES], empty[MANY_STAGES];
+    uint64_t acc_full[2], acc_empty[2];
+    uint32_t tmem;
+    int failed;
+};
+
+template <class T>
+__global__ void __launch_bounds__(MANY_THREADS, 1)
+fp8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const F8Args a) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    ManySmem& sh = *reinterpret_cast<ManySmem*>(ring + MANY_STAGES * MANY_STAGE);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int m_tiles = (a.tokens + MANY_M - 1) / MANY_M, n_tiles = (a.rows + MANY_N - 1) / MANY_N;
+    const int tiles = m_tiles * n_tiles;
+    // tiles in bands of up to 16 token tiles: the CTAs at work share few row and token tiles of both operands in L2
+    auto tile_at = [&](int t, int& m, int& n) {
+        constexpr int BAND = 16;
+        const int band = t / (BAND * n_tiles), in = t - band * BAND * n_tiles;
+        const int h = min(BAND, m_tiles - band * BAND);
+        m = band * BAND + in % h;
+        n = in / h;
+    };
+
+    if (tid == 0) {
+        for (int i = 0; i < MANY_STAGES; ++i) {
+            mbar_init(&sh.full[i], 1);
+            mbar_init(&sh.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.acc_full[i], 1);
+            mbar_init(&sh.acc_empty[i], 256);
+        }
+        sh.failed = 0;
+        fence_mbar_init();
+        tma_prefetch_map(&map_w);
+        tma_prefetch_map(&map_x);
+    }
+    if (warp == 1) tmem_alloc(&sh.tmem, 512);
+    tc5_fence_before();
+    __syncthreads();
+    tc5_fence_after();
+    const uint32_t tmem = sh.tmem;
+    pdl_wait();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            bool ok = true;
+            int n = 0;
+            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                int mt, nt;
+                tile_at(t, mt, nt);
+                for (int kb = 0; kb < a.kb_n; ++kb, ++n) {
+                    const int st = n % MANY_STAGES;
+                    if (n >= MANY_STAGES && !mbar_wait(&sh.empty[st], (uint32_t)(n / MANY_STAGES - 1) & 1u)) {
+                        ok = false;
+                        break;
+                    }
+                    mbar_expect_tx(&sh.full[st], MANY_STAGE);
+                    tma_load_2d(ring + st * MANY_STAGE, &map_x, kb * 128, mt * MANY_M, &sh.full[st]);
+                    tma_load_2d(ring + st * MANY_STAGE + MANY_M * 128, &map_w, kb * 128, nt * MANY_N, &sh.full[st]);
+                }
+            }
+            if (!ok) {
+                for (int v = max(0, n - MANY_STAGES); v < n; ++v)
+                    mbar_wait(&sh.full[v % MANY_STAGES], (uint32_t)(v / MANY_STAGES) & 1u);
+                sh.failed = 1;
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        bool ok = true;
+        int n = 0;
+        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+            for (int kb = 0; kb < a.kb_n; ++kb, ++n) {
+                const int st = n % MANY_STAGES, buf = n & 1;
+                ok = mbar_wait(&sh.full[st], (uint32_t)(n / MANY_STAGES) & 1u);
+                if (ok && n >= 2) ok = mbar_wait(&sh.acc_empty[buf], (uint32_t)(n / 2 - 1) & 1u);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc5_fence_after();
+                if (elect_one()) {
+                    const uint32_t sa = smem_u32(ring + st * MANY_STAGE), sb = sa + MANY_M * 128;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        umma_f8(tmem + buf * MANY_N, sw128_desc(sa + 32 * j), sw128_desc(sb + 32 * j),
+                                f8_idesc(MANY_M, MANY_N), j > 0);
+                    umma_commit1(&sh.empty[st]);
+                    umma_commit1(&sh.acc_full[buf]);
+                }
+                __syncwarp();
+            }
+        if (!ok && lane == 0) sh.failed = 1;
+    } else {
+        // thread = token (TMEM lane), 128 rows of the weight (one row of scale blocks)
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+        const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | (size_t)a.out_stride * sizeof(T)) & 15) == 0;
+        bool ok = true;
+        int n = 0;
+        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            int mt, nt;
+            tile_at(t, mt, nt);
+            const int tok = mt * MANY_M + quarter * 32 + lane, row0 = nt * MANY_N + half * 128;
+            const float* sxp = a.sx + (size_t)min(tok, a.tokens - 1) * a.kb_n;
+            const float* swp = a.sw + (size_t)(min(row0, a.rows - 1) >> 7) * a.kb_n;
+            float acc[128];
+#pragma unroll
+            for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
+            float nx = sxp[0], nw = swp[0];
+            for (int kb = 0; kb < a.kb_n; ++kb, ++n) {
+                const int buf = n & 1;
+                const float f = nx * nw;
+                if (kb + 1 < a.kb_n) {
+                    nx = sxp[kb + 1];
+                    nw = swp[kb + 1];
+                }
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[buf], (uint32_t)(n >> 1) & 1u));
+                if (!ok) break;
+                tc5_fence_after();
+#pragma unroll
+                for (int c = 0; c < 128; c += 32) {
+                    uint32_t v[16], w[16];
+                    tmem_load16(tbase + buf * MANY_N + c, v);
+                    tmem_load16(tbase + buf * MANY_N + c + 16, w);
+                    tmem_wait16(v);
+                    tmem_wait16(w);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(__uint_as_float(v[i]), f, acc[c + i]);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[c + 16 + i] = fmaf(__uint_as_float(w[i]), f, acc[c + 16 + i]);
+                }
+                tc5_fence_before();
+                mbar_arrive_one(&sh.acc_empty[buf]);
+            }
+            if (!ok) break;
+            if (tok < a.tokens) {
+                T* o = static_cast<T*>(a.out) + (size_t)tok * a.out_stride + row0;
+                constexpr int V = 16 / (int)sizeof(T);
+                if (wide && row0 + 128 <= a.rows) {
+#pragma unroll
+                    for (int i = 0; i < 128; i += V) {
+                        alignas(16) T p[V];
+#pragma unroll
+                        for (int j = 0; j < V; ++j) p[j] = narrow<T>(acc[i + j]);
+                        *reinterpret_cast<uint4*>(o + i) = *reinterpret_cast<const uint4*>(p);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 128; ++i)
+                        if (row0 + i < a.rows) o[i] = narrow<T>(acc[i]);
+                }
+            }
+        }
+        if (!ok && lane == 0) sh.failed = 1;
+    }
+    tc5_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc5_fence_after();
+        tmem_free(tmem, 512);
+    }
+    if (tid == 0 && sh.failed) set_err(a.err, DEV_ERR_TMA_TIMEOUT);
+}
+
+// ------------------------------------------------------------------ host ----
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+    static EncodeFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+// [rows][cols] bytes, box of 128 columns; what lies past the ends reads as zero (an e4m3 zero).
+cudaError_t encode_bytes(CUtensorMap* map, const void* base, size_t rows, size_t cols, size_t pitch, int box_rows) {
+    EncodeFn fn = encode_fn();
+    if (!fn) return cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
+    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, step[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, step,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+template <class K>
+cudaError_t launch_after(K kernel, int grid, int threads, size_t smem, cudaStream_t st, bool overlap, const CUtensorMap& w,
+                         const CUtensorMap& x, const F8Args& a) {
+    cudaError_t e = set_max_dyn_smem((const void*)kernel, 227 * 1024);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = overlap ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, w, x, a);
+}
+
+template <int NT>
+cudaError_t launch_few(const Fp8Product& p, const F8Args& a, int grid, bool overlap, cudaStream_t st) {
+    CUtensorMap mw, mx;
+    cudaError_t e = encode_bytes(&mw, p.w, p.rows, p.cols, p.cols, 128);
+    if (e == cudaSuccess) e = encode_bytes(&mx, p.codes, p.tokens, p.cols, p.code_pitch, NT);
+    if (e != cudaSuccess) return e;
+    const size_t smem = 1024 + (size_t)few_stages(NT) * few_stage_bytes(NT) + sizeof(FewSmem<NT>);
+    static_assert(1024 + few_stages(NT) * few_stage_bytes(NT) + sizeof(FewSmem<NT>) <= 227 * 1024, "shared memory");
+    return launch_after(fp8_few_kernel<NT>, grid, few_threads(NT), smem, st, overlap, mw, mx, a);
+}
+
+template <class T>
+cudaError_t launch_many(const Fp8Product& p, const F8Args& a, int grid, bool overlap, cudaStream_t st) {
+    CUtensorMap mw, mx;
+    cudaError_t e = encode_bytes(&mw, p.w, p.rows, p.cols, p.cols, MANY_N);
+    if (e == cudaSuccess) e = encode_bytes(&mx, p.codes, p.tokens, p.cols, p.code_pitch, MANY_M);
+    if (e != cudaSuccess) return e;
+    constexpr size_t smem = 1024 + (size_t)MANY_STAGES * MANY_STAGE + sizeof(ManySmem);
+    static_assert(smem <= 227 * 1024, "shared memory");
+    return launch_after(fp8_many_kernel<T>, grid, MANY_THREADS, smem, st, overlap, mw, mx, a);
+}
+
+// Columns of an accumulator of the few-token kernel.
+int few_columns(size_t tokens) { return tokens <= 16 ? 16 : (tokens <= 32 ? 32 : (tokens <= 64 ? 64 : 128)); }
+bool takes_few(size_t tokens) { return tokens <= 128; }
+
+}  // namespace
+
+cudaError_t launch_fp8_quantize(const void* x, int type, size_t tokens, size_t cols, size_t x_stride, uint8_t* codes,
+                                size_t code_pitch, float* scales, int sm_count, cudaStream_t st) {
+    if (tokens == 0 || cols == 0) return cudaSuccess;
+    const int kb_n = (int)((cols + 127) / 128);
+    const long long units = (long long)tokens * kb_n;
+    const int grid = (int)std::min<long long>((units + 15) / 16, (long long)sm_count * 64);
+    const size_t z = type == LQ_T_F32 ? 4 : 2;
+    const bool vec = cols % 8 == 0 && (((uintptr_t)x | x_stride * z) & 15) == 0;
+    const int wide = cols % 8 == 0 && (((uintptr_t)codes | code_pitch) & 7) == 0;
+    auto go = [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        if (vec)
+            fp8_quantize_kernel<T, true><<<grid, 256, 0, st>>>((const T*)x, (long long)x_stride, units, kb_n, (int)cols, codes,
+                                                               (long long)code_pitch, scales, wide);
+        else
+            fp8_quantize_kernel<T, false><<<grid, 256, 0, st>>>((const T*)x, (long long)x_stride, units, kb_n, (int)cols, codes,
+                                                                (long long)code_pitch, scales, wide);
+    };
+    if (type == LQ_T_F32) go((float*)nullptr);
+    else if (type == LQ_T_BF16) go((__nv_bfloat16*)nullptr);
+    else go((__half*)nullptr);
+    return cudaGetLastError();
+}
+
+// Partial tiles and counters of the few-token kernel.
+size_t fp8_part_bytes(size_t tokens, int sm_count) {
+    return takes_few(tokens) ? (size_t)sm_count * 2 * few_columns(tokens) * 128 * 4 : 0;
+}
+size_t fp8_tile_count(size_t tokens, size_t rows) {
+    const size_t nt = (size_t)few_columns(tokens);
+    return takes_few(tokens) ? ((rows + 127) / 128) * ((tokens + nt - 1) / nt) : 0;
+}
+
+cudaError_t launch_fp8_matmul(const Fp8Product& p, bool overlap, int sm_count, int* err, cudaStream_t st) {
+    const int kb_n = (int)((p.cols + 127) / 128);
+    const F8Args a{p.scales, p.w_scales, p.out, (long long)p.out_stride, p.out_type, (int)p.tokens, (int)p.rows, kb_n, p.part,
+                   p.done, err};
+    if (takes_few(p.tokens)) {
+        const int nt = few_columns(p.tokens);
+        const long long units = (long long)fp8_tile_count(p.tokens, p.rows) * kb_n;
+        const int grid = (int)std::min<long long>(units, sm_count);
+        switch (nt) {
+            case 16: return launch_few<16>(p, a, grid, overlap, st);
+            case 32: return launch_few<32>(p, a, grid, overlap, st);
+            case 64: return launch_few<64>(p, a, grid, overlap, st);
+        }
+        return launch_few<128>(p, a, grid, overlap, st);
+    }
+    const long long tiles = (long long)((p.tokens + MANY_M - 1) / MANY_M) * ((p.rows + MANY_N - 1) / MANY_N);
+    const int grid = (int)std::min<long long>(tiles, sm_count);
+    if (p.out_type == LQ_T_F32) return launch_many<float>(p, a, grid, overlap, st);
+    if (p.out_type == LQ_T_BF16) return launch_many<__nv_bfloat16>(p, a, grid, overlap, st);
+    return launch_many<__half>(p, a, grid, overlap, st);
+}
+
+}  // namespace lq

@@ -4,6 +4,9 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace lq {
@@ -182,6 +185,37 @@ cudaError_t launch_finish(const float* partials, int n_partials, int hidden, con
 // walk_fused_q4k.cu — the fused persistent walk (one token, all layers, one cooperative launch)
 bool fused_q4k_supported(int hidden, int n_rows, int top_k, int sm_count);
 size_t fused_q4k_ws_bytes(int hidden, int n_rows, int sm_count);
+// block_norm.cu
+struct BlockNorm {
+    const void *h, *y, *post_w, *pre_w, *gate;  // y, gate, weights may be null (no block output / no gate / unit weight)
+    void *h_out, *n_out;                        // either may be null
+    long long h_stride, y_stride, gate_stride, h_out_stride, n_out_stride;  // elements between rows
+    long long gate_group;                       // rows that share a gate row
+    int rows, cols, gate_cols, w_type, post_norm;
+    float w_offset, h_scale, y_scale;
+    double eps;
+};
+cudaError_t launch_block_norm(const BlockNorm& a, int type, int sm_count, cudaStream_t st);
+
+// fp8_gemm.cu
+cudaError_t launch_fp8_quantize(const void* x, int type, size_t tokens, size_t cols, size_t x_stride, uint8_t* codes,
+                                size_t code_pitch, float* scales, int sm_count, cudaStream_t st);
+struct Fp8Product {
+    const uint8_t* w;        // [rows][cols] e4m3
+    const float* w_scales;   // [ceil(rows / 128)][ceil(cols / 128)]
+    const uint8_t* codes;    // [tokens][code_pitch] e4m3
+    const float* scales;     // [tokens][ceil(cols / 128)]
+    void* out;
+    size_t rows, cols, tokens, code_pitch, out_stride;
+    int out_type;
+    float* part;             // fp8_part_bytes of workspace
+    unsigned* done;          // fp8_tile_count counters, zero between launches
+};
+size_t fp8_part_bytes(size_t tokens, int sm_count);
+size_t fp8_tile_count(size_t tokens, size_t rows);
+// overlap: the kernel before this one on the stream is this product's own quantisation (it may start while that ends)
+cudaError_t launch_fp8_matmul(const Fp8Product& p, bool overlap, int sm_count, int* err, cudaStream_t st);
+
 int fused_q4k_stamp_count();
 size_t fused_q4k_ws_dirty_bytes();
 }  // namespace lq
