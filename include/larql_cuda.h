@@ -433,6 +433,30 @@ LQ_API int lq_dev_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const void* x, int
 LQ_API int lq_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const float* x, size_t x_len, size_t tokens, float* out,
                          size_t out_len);
 
+/* A whole mixture-of-experts layer for a few tokens, one launch per 64 tokens (cpu_moe_forward,
+ * crates/larql-compute/src/cpu/ops/moe/forward.rs:24-140, over dense experts and with the router's product):
+ *     logits = x . router^T + bias; the top_e experts by logit (ties to the lower index), softmax weights over all
+ *     experts, renormalised over the selected when renormalise != 0;
+ *     out_t = sum_j w_tj down_j (silu(gate_j x_t) * (up_j x_t)), j in selection order.
+ * lq_moe_create  gates, ups [inter, hidden] and downs [hidden, inter] (NOT feature-major), n_experts of each, all of
+ *                one format (MXFP4, NVFP4, FP8_B128) and device resident (LQ_MAT_DEVICE), codes and FP4 scales 16-byte
+ *                aligned; hidden and inter multiples of 32, at most 8192; 1..256 experts, top_e <= 32.  router
+ *                [n_experts, hidden] and router_bias [n_experts] (may be NULL) are device pointers of router_type.
+ *                The handle keeps the pointers, not the data, and a workspace for 64 tokens.
+ * lq_dev_moe_ffn x, out [tokens, hidden] of type (LQ_T_F32 / BF16 / F16; out may be x); idx_out, w_out [tokens,
+ *                min(top_e, n_experts)] may be NULL.  Calls on one handle run one after another on the stream.
+ * lq_moe_ffn     the same with host pointers, f32 (the handle's matrices stay on the device).
+ * A token with a NaN or infinity gets NaN outputs and weights; the other tokens are not touched by it. */
+typedef struct lq_moe lq_moe;
+LQ_API int lq_moe_create(lq_ctx* ctx, const lq_matrix* gates, const lq_matrix* ups, const lq_matrix* downs, size_t n_experts,
+                         const void* router, int router_type, const void* router_bias, size_t top_e, int renormalise,
+                         lq_moe** out);
+LQ_API int lq_dev_moe_ffn(lq_ctx* ctx, lq_moe* moe, const void* x, int type, size_t tokens, void* out, uint32_t* idx_out,
+                          float* w_out);
+LQ_API int lq_moe_ffn(lq_ctx* ctx, lq_moe* moe, const float* x, size_t x_len, size_t tokens, float* out, uint32_t* idx_out,
+                      float* w_out);
+LQ_API void lq_moe_destroy(lq_ctx* ctx, lq_moe* moe);
+
 /* ---- allocation-free entry point ---------------------------------------------------- */
 /* Has no counterpart in the reference.  A Q4_K matvec (same arithmetic and kernels as
  * lq_dev_q4k_matvec) for hosts that must not allocate device memory while running: processes

@@ -46,6 +46,7 @@ EXPORTS = [
     "lq_stack_create_sharded", "lq_stack_path", "lq_q6k_matvec", "lq_dequantize_q6k", "lq_q4k_dual_matvec",
     "lq_k_quant_padded_cols", "lq_vindex_open", "lq_vindex_num_layers", "lq_vindex_layer", "lq_vindex_close",
     "lq_nvfp4_pack_split", "lq_dev_block_norm", "lq_dev_fp8_quantize", "lq_dev_fp8_matmul", "lq_fp8_matmul",
+    "lq_moe_create", "lq_dev_moe_ffn", "lq_moe_ffn", "lq_moe_destroy",
 ]
 
 
@@ -156,6 +157,10 @@ def load_library() -> C.CDLL:
         "lq_dev_fp8_quantize": (C.c_int, [vp, vp, C.c_int, sz, sz, sz, vp, vp]),
         "lq_dev_fp8_matmul": (C.c_int, [vp, mp, vp, C.c_int, vp, sz, sz, vp, C.c_int, sz]),
         "lq_fp8_matmul": (C.c_int, [vp, mp, f32p, sz, sz, f32p, sz]),
+        "lq_moe_create": (C.c_int, [vp, mp, mp, mp, sz, vp, C.c_int, vp, sz, C.c_int, C.POINTER(vp)]),
+        "lq_dev_moe_ffn": (C.c_int, [vp, vp, vp, C.c_int, sz, vp, vp, vp]),
+        "lq_moe_ffn": (C.c_int, [vp, vp, f32p, sz, sz, f32p, u32p, f32p]),
+        "lq_moe_destroy": (None, [vp, vp]),
         "lq_f16_gemv_topk": (C.c_int, [vp, vp, sz, f32p, sz, sz, sz, sz, u32p, f32p, C.POINTER(sz)]),
     }
     for name, (res, args) in sig.items():
@@ -272,6 +277,25 @@ class DeviceMatrix:
     def c(self) -> LqMatrix:
         return LqMatrix(self.fmt | MAT_DEVICE, self.data_ptr, self.data_len, self.scales_ptr or None,
                         self.scales_len, self.tensor_scale, self.rows, self.cols)
+
+
+class MoeLayer:
+    """A mixture-of-experts layer on one backend (CudaBackend.moe_create): the experts' table, the router and the
+    workspace.  ``keepalive`` holds what owns the device memory the layer points into."""
+
+    def __init__(self, backend, handle, hidden, top_e, keepalive):
+        self._backend, self.handle, self.hidden, self.top_e, self.keepalive = backend, handle, hidden, top_e, keepalive
+
+    def close(self):
+        if self.handle:
+            self._backend._lib.lq_moe_destroy(self._backend._h, self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 def q4k_matvec_static(w_ptr: int, w_len: int, x_ptr: int, num_rows: int, hidden: int, out_ptr: int, stream: int = 0):
@@ -623,6 +647,38 @@ class CudaBackend:
         m = w.c()
         ok = self._status(self._lib.lq_fp8_matmul(self._h, C.byref(m), _ptr(x2), x2.size, x2.shape[0], _ptr(out), out.size))
         return out.reshape(*x.shape[:-1], w.rows) if ok else None
+
+    def moe_create(self, gates, ups, downs, router_ptr: int, router_type: int, bias_ptr: int, top_e: int,
+                   renormalise: bool = True, keepalive=None):
+        """A whole MoE layer: gates, ups [inter, hidden] and downs [hidden, inter] (DeviceMatrix each), the router's
+        weight [experts, hidden] and bias (0: none) on the device.  A MoeLayer, or None on a refusal."""
+        n = len(gates)
+        if n == 0 or len(ups) != n or len(downs) != n:
+            return None
+        arr = lambda ms: (LqMatrix * n)(*[m.c() for m in ms])
+        ga, ua, da = arr(gates), arr(ups), arr(downs)
+        h = C.c_void_p()
+        ok = self._status(self._lib.lq_moe_create(self._h, ga, ua, da, n, router_ptr or None, router_type, bias_ptr or None,
+                                                  int(top_e), int(renormalise), C.byref(h)))
+        return MoeLayer(self, h, gates[0].cols, min(int(top_e), n), (gates, ups, downs, keepalive)) if ok else None
+
+    def dev_moe_ffn(self, layer: MoeLayer, x_ptr: int, x_type: int, tokens: int, out_ptr: int, idx_ptr: int = 0, w_ptr: int = 0):
+        """out [tokens, hidden] of the layer for x [tokens, hidden], one launch per 64 tokens."""
+        return self._status(self._lib.lq_dev_moe_ffn(self._h, layer.handle, x_ptr, x_type, tokens, out_ptr, idx_ptr or None,
+                                                     w_ptr or None))
+
+    def moe_ffn(self, layer: MoeLayer, x):
+        """x [tokens, hidden] (host, f32) -> (out, expert indexes, weights); None on a refusal."""
+        x = _f32(x)
+        x2 = x.reshape(-1, x.shape[-1])
+        t, k = x2.shape[0], layer.top_e
+        out = np.empty_like(x2)
+        idx, w = np.zeros((t, max(k, 1)), np.uint32), np.zeros((t, max(k, 1)), np.float32)
+        if x2.shape[1] != layer.hidden:
+            return None
+        ok = self._status(self._lib.lq_moe_ffn(self._h, layer.handle, _ptr(x2), x2.size, t, _ptr(out), idx.ctypes.data,
+                                               w.ctypes.data))
+        return (out.reshape(x.shape), idx[:, :k], w[:, :k]) if ok else None
 
     # -- feature-sharded walk: the steps between the collectives --------------------
     def dev_shard_scan(self, gate, x_ptr: int, flags: int, rank: int, world: int, hist_ptr: int):

@@ -71,6 +71,14 @@ struct lq_stack {
     uint32_t* sync_word = nullptr;        // one word for the launch rendezvous
 };
 
+struct lq_moe {
+    lq_ctx* ctx = nullptr;
+    int device = 0, fmt = 0;
+    MoeLayer layer = {};       // everything but the call's operands
+    size_t max_tokens = 0;     // per launch
+    uint8_t* raw = nullptr;    // table and workspace, one allocation
+};
+
 struct lq_ctx {
     int device = 0;
     cudaStream_t stream = nullptr;
@@ -122,6 +130,7 @@ struct lq_ctx {
     };
     OpBuf op_codes, op_part, op_done;
     std::vector<void*> retired;
+    std::vector<lq_moe*> moes;  // live handles: their barriers are cleared after a device error
     const lq_stack* last_xstack = nullptr;  // sharded fused stack that ran last (its selection: lq_dev_shard_hits)
 };
 
@@ -440,6 +449,7 @@ int check_device_err(lq_ctx* ctx) {
     // a failed fused launch may leave its histogram / counters dirty
     if (ctx->fws) CK(cudaMemsetAsync(ctx->fws, 0, fused_q4k_ws_dirty_bytes(), ctx->stream));
     if (ctx->op_done.p) CK(cudaMemsetAsync(ctx->op_done.p, 0, ctx->op_done.cap, ctx->stream));
+    for (lq_moe* m : ctx->moes) CK(cudaMemsetAsync(m->layer.barrier, 0, 8, ctx->stream));
     if (h == DEV_ERR_NAN_SCORE) return fail(ctx, LQ_ERR_NAN_SCORE, "NaN gate score or non-finite activation");
     if (h == DEV_ERR_TMA_TIMEOUT) return fail(ctx, LQ_ERR_TIMEOUT, "a bounded device-side wait ran out");
     return fail(ctx, LQ_ERR_CUDA, "device-side internal error");
@@ -818,6 +828,7 @@ void lq_destroy(lq_ctx* ctx) {
     cudaFree(ctx->tc_scratch);
     for (lq_ctx::OpBuf* b : {&ctx->op_codes, &ctx->op_part, &ctx->op_done}) cudaFree(b->p);
     for (void* p : ctx->retired) cudaFree(p);
+    for (lq_moe* m : ctx->moes) m->ctx = nullptr;  // (a handle that outlives its context frees its own memory)
     cudaFree(ctx->stage);
     cudaFree(ctx->sort_buf);
     cudaFree(ctx->d_err);
@@ -2410,6 +2421,136 @@ int lq_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const float* x, size_t x_len,
     if ((rc = lq_dev_fp8_matmul(ctx, &dm, dx, LQ_T_F32, nullptr, tokens, cols, dout, LQ_T_F32, rows))) return rc;
     CK(cudaMemcpyAsync(out, dout, out_len * 4, cudaMemcpyDeviceToHost, ctx->stream));
     return lq_synchronize(ctx);
+}
+
+int lq_moe_create(lq_ctx* ctx, const lq_matrix* gates, const lq_matrix* ups, const lq_matrix* downs, size_t n_experts,
+                  const void* router, int router_type, const void* router_bias, size_t top_e, int renormalise, lq_moe** out) {
+    DevGuard dev_guard(ctx);
+    if (out) *out = nullptr;
+    if (!ctx || !gates || !ups || !downs || !router || !out) return LQ_ERR_ARGUMENT;
+    if (n_experts == 0 || n_experts > MOE_LAYER_MAX_EXPERTS) return fail(ctx, LQ_REFUSED_UNSUPPORTED, "moe: 1..256 experts");
+    if (!float_type(router_type)) return fail(ctx, LQ_REFUSED_UNSUPPORTED, "moe: router element type");
+    const size_t k = std::min(top_e, n_experts);
+    if (k > MOE_LAYER_MAX_TOP) return fail(ctx, LQ_REFUSED_UNSUPPORTED, "moe: more than 32 experts a token");
+    if (((uintptr_t)router | (uintptr_t)router_bias) & (type_bytes(router_type) - 1))
+        return fail(ctx, LQ_ERR_ARGUMENT, "moe: router not aligned to its elements");
+    const int fmt = gates[0].fmt & 0xff;
+    if (fmt != LQ_FMT_MXFP4 && fmt != LQ_FMT_NVFP4 && fmt != LQ_FMT_FP8_B128)
+        return fail(ctx, LQ_REFUSED_UNSUPPORTED, "moe: experts are MXFP4, NVFP4 or FP8_B128");
+    const int64_t inter = gates[0].rows, hidden = gates[0].cols;
+    std::vector<MoeExpert> table(n_experts);
+    for (size_t e = 0; e < n_experts; ++e) {
+        const lq_matrix* m[3] = {gates + e, ups + e, downs + e};
+        for (int i = 0; i < 3; ++i) {
+            if ((m[i]->fmt & 0xff) != fmt) return fail(ctx, LQ_REFUSED_UNSUPPORTED, "moe: experts of different formats");
+            int rc = fmt == LQ_FMT_FP8_B128 ? check_fp8(ctx, m[i], "moe") : check_matrix(ctx, m[i], "moe");
+            if (rc) return rc;
+            if (!(m[i]->fmt & LQ_MAT_DEVICE)) return fail(ctx, LQ_ERR_ARGUMENT, "moe: a matrix is not device resident");
+            if (m[i]->rows != (i == 2 ? hidden : inter) || m[i]->cols != (i == 2 ? inter : hidden))
+                return fail(ctx, LQ_REFUSED_SHAPE, "moe: gate, up [inter, hidden], down [hidden, inter]");
+            if ((uintptr_t)m[i]->data & 15 || (fmt != LQ_FMT_FP8_B128 && (uintptr_t)m[i]->scales & 15))
+                return fail(ctx, LQ_ERR_ARGUMENT, "moe: codes or scales not 16-byte aligned");
+            table[e].codes[i] = (const uint8_t*)m[i]->data;
+            table[e].scales[i] = (const uint8_t*)m[i]->scales;
+            table[e].ts[i] = fmt == LQ_FMT_NVFP4 ? m[i]->tensor_scale : 1.0f;
+        }
+    }
+    if (hidden > 0x40000000 || inter > 0x40000000 || !moe_layer_supported(fmt, (int)hidden, (int)inter))
+        return fail(ctx, LQ_REFUSED_UNSUPPORTED, "moe: hidden and inter are multiples of 32, at most 8192");
+    lq_moe* h = new lq_moe();
+    h->device = ctx->device;
+    h->fmt = fmt;
+    h->max_tokens = std::min<size_t>(MOE_LAYER_MAX_TOKENS, MOE_LAYER_MAX_PAIRS / std::max<size_t>(k, 1));
+    const size_t pairs = h->max_tokens * std::max<size_t>(k, 1);
+    const size_t tb = a256(n_experts * sizeof(MoeExpert)), lb = a256(h->max_tokens * n_experts * 4),
+                 ab = a256(pairs * (size_t)inter * 4), pb = a256(pairs * (size_t)hidden * 4);
+    cudaError_t e = cudaMalloc(&h->raw, tb + lb + ab + pb + 256);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(h->raw, table.data(), n_experts * sizeof(MoeExpert), cudaMemcpyHostToDevice, ctx->stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(h->raw + tb + lb + ab + pb, 0, 256, ctx->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        cudaFree(h->raw);
+        delete h;
+        return cuda_fail(ctx, e, "moe workspace");
+    }
+    MoeLayer& L = h->layer;
+    L.table = (const MoeExpert*)h->raw;
+    L.logits = (float*)(h->raw + tb);
+    L.act = (float*)(h->raw + tb + lb);
+    L.pair_out = (float*)(h->raw + tb + lb + ab);
+    L.barrier = (unsigned*)(h->raw + tb + lb + ab + pb);
+    L.router = router, L.bias = router_bias, L.router_type = router_type;
+    L.hidden = (int)hidden, L.inter = (int)inter, L.experts = (int)n_experts, L.top_e = (int)k;
+    L.renormalise = renormalise != 0;
+    L.err = ctx->d_err;
+    h->ctx = ctx;
+    ctx->moes.push_back(h);
+    *out = h;
+    return LQ_OK;
+}
+
+int lq_dev_moe_ffn(lq_ctx* ctx, lq_moe* moe, const void* x, int type, size_t tokens, void* out, uint32_t* idx_out, float* w_out) {
+    DevGuard dev_guard(ctx);
+    if (!ctx || !moe) return LQ_ERR_ARGUMENT;
+    if (moe->ctx != ctx) return fail(ctx, LQ_ERR_ARGUMENT, "moe: the handle belongs to another context");
+    if (!float_type(type)) return fail(ctx, LQ_REFUSED_UNSUPPORTED, "moe: element type");
+    if (tokens == 0) return LQ_OK;
+    if (!x || !out) return fail(ctx, LQ_ERR_ARGUMENT, "moe: null pointer");
+    const size_t z = type_bytes(type);
+    if (((uintptr_t)x | (uintptr_t)out) & (z - 1) || ((uintptr_t)idx_out | (uintptr_t)w_out) & 3)
+        return fail(ctx, LQ_ERR_ARGUMENT, "moe: pointer not aligned to its elements");
+    const size_t H = (size_t)moe->layer.hidden, k = (size_t)moe->layer.top_e;
+    if (tokens > 0x7fffffffu) return fail(ctx, LQ_REFUSED_UNSUPPORTED, "moe: too many tokens");
+    if (k == 0) {
+        CK(cudaMemsetAsync(out, 0, tokens * H * z, ctx->stream));
+        return LQ_OK;
+    }
+    for (size_t t0 = 0; t0 < tokens; t0 += moe->max_tokens) {
+        MoeLayer L = moe->layer;
+        L.tokens = (int)std::min(moe->max_tokens, tokens - t0);
+        L.type = type;
+        L.x = (const uint8_t*)x + t0 * H * z;
+        L.out = (uint8_t*)out + t0 * H * z;
+        L.idx_out = idx_out ? idx_out + t0 * k : nullptr;
+        L.w_out = w_out ? w_out + t0 * k : nullptr;
+        CK(launch_moe_layer(moe->fmt, L, ctx->sm_count, ctx->stream));
+        ctx->launches += 1;
+    }
+    return LQ_OK;
+}
+
+int lq_moe_ffn(lq_ctx* ctx, lq_moe* moe, const float* x, size_t x_len, size_t tokens, float* out, uint32_t* idx_out, float* w_out) {
+    DevGuard dev_guard(ctx);
+    if (!ctx || !moe) return LQ_ERR_ARGUMENT;
+    const size_t H = (size_t)moe->layer.hidden, k = (size_t)moe->layer.top_e;
+    if (x_len != tokens * H) return fail(ctx, LQ_REFUSED_SHAPE, "moe: x_len != tokens * hidden");
+    if (tokens == 0) return LQ_OK;
+    if (!x || !out) return fail(ctx, LQ_ERR_ARGUMENT, "moe: null pointer");
+    const size_t xb = a256(x_len * 4), rb = a256(tokens * std::max<size_t>(k, 1) * 4);
+    int rc = ensure_stage(ctx, xb + 2 * rb);
+    if (rc) return rc;
+    float *dx = (float*)ctx->stage, *dw = (float*)(ctx->stage + xb + rb);
+    uint32_t* di = (uint32_t*)(ctx->stage + xb);
+    CK(cudaMemcpyAsync(dx, x, x_len * 4, cudaMemcpyHostToDevice, ctx->stream));
+    if ((rc = lq_dev_moe_ffn(ctx, moe, dx, LQ_T_F32, tokens, dx, di, dw))) return rc;
+    CK(cudaMemcpyAsync(out, dx, x_len * 4, cudaMemcpyDeviceToHost, ctx->stream));
+    if (idx_out && k) CK(cudaMemcpyAsync(idx_out, di, tokens * k * 4, cudaMemcpyDeviceToHost, ctx->stream));
+    if (w_out && k) CK(cudaMemcpyAsync(w_out, dw, tokens * k * 4, cudaMemcpyDeviceToHost, ctx->stream));
+    return lq_synchronize(ctx);
+}
+
+void lq_moe_destroy(lq_ctx* ctx, lq_moe* moe) {
+    if (!moe) return;
+    DevGuard dev_guard(moe->ctx);
+    if (moe->ctx) {
+        cudaStreamSynchronize(moe->ctx->stream);
+        auto& v = moe->ctx->moes;
+        v.erase(std::remove(v.begin(), v.end(), moe), v.end());
+    }
+    (void)ctx;
+    cudaFree(moe->raw);
+    delete moe;
 }
 
 }  // extern "C"

@@ -216,6 +216,33 @@ size_t fp8_tile_count(size_t tokens, size_t rows);
 // overlap: the kernel before this one on the stream is this product's own quantisation (it may start while that ends)
 cudaError_t launch_fp8_matmul(const Fp8Product& p, bool overlap, int sm_count, int* err, cudaStream_t st);
 
+// moe_layer.cu: the whole mixture-of-experts layer for up to MOE_LAYER_MAX_TOKENS tokens, one cooperative launch
+#define MOE_LAYER_MAX_EXPERTS 256
+#define MOE_LAYER_MAX_TOKENS 64
+#define MOE_LAYER_MAX_TOP 32
+#define MOE_LAYER_MAX_PAIRS 1024  // tokens x top_e of a launch
+struct MoeExpert {
+    const uint8_t* codes[3];   // gate, up [inter][hidden]; down [hidden][inter]
+    const uint8_t* scales[3];
+    float ts[3];
+};
+struct MoeLayer {
+    const MoeExpert* table;
+    const void *router, *bias;  // [experts][hidden], [experts] or null
+    int router_type, hidden, inter, experts, top_e, renormalise;
+    const void* x;              // [tokens][hidden]
+    int type, tokens;
+    void* out;                  // [tokens][hidden]
+    uint32_t* idx_out;          // [tokens][top_e] or null
+    float* w_out;
+    float *logits, *act, *pair_out;  // workspace: [tokens][experts], [pairs][inter], [pairs][hidden]
+    unsigned* barrier;               // two words, zero between launches but for the generation
+    int n_stages, stage_bytes;       // filled in by the launch
+    int* err;
+};
+bool moe_layer_supported(int fmt, int hidden, int inter);
+cudaError_t launch_moe_layer(int fmt, const MoeLayer& L, int sm_count, cudaStream_t st);
+
 int fused_q4k_stamp_count();
 size_t fused_q4k_ws_dirty_bytes();
 }  // namespace lq
