@@ -77,6 +77,7 @@ struct lq_moe {
     MoeLayer layer = {};       // everything but the call's operands
     size_t max_tokens = 0;     // per launch
     uint8_t* raw = nullptr;    // table and workspace, one allocation
+    size_t sync_bytes = 0;     // the counters: from layer.exits on
 };
 
 struct lq_ctx {
@@ -449,7 +450,7 @@ int check_device_err(lq_ctx* ctx) {
     // a failed fused launch may leave its histogram / counters dirty
     if (ctx->fws) CK(cudaMemsetAsync(ctx->fws, 0, fused_q4k_ws_dirty_bytes(), ctx->stream));
     if (ctx->op_done.p) CK(cudaMemsetAsync(ctx->op_done.p, 0, ctx->op_done.cap, ctx->stream));
-    for (lq_moe* m : ctx->moes) CK(cudaMemsetAsync(m->layer.barrier, 0, 8, ctx->stream));
+    for (lq_moe* m : ctx->moes) CK(cudaMemsetAsync(m->layer.exits, 0, m->sync_bytes, ctx->stream));
     if (h == DEV_ERR_NAN_SCORE) return fail(ctx, LQ_ERR_NAN_SCORE, "NaN gate score or non-finite activation");
     if (h == DEV_ERR_TMA_TIMEOUT) return fail(ctx, LQ_ERR_TIMEOUT, "a bounded device-side wait ran out");
     return fail(ctx, LQ_ERR_CUDA, "device-side internal error");
@@ -2456,17 +2457,26 @@ int lq_moe_create(lq_ctx* ctx, const lq_matrix* gates, const lq_matrix* ups, con
         }
     }
     if (hidden > 0x40000000 || inter > 0x40000000 || !moe_layer_supported(fmt, (int)hidden, (int)inter))
-        return fail(ctx, LQ_REFUSED_UNSUPPORTED, "moe: hidden and inter are multiples of 32, at most 8192");
+        return fail(ctx, LQ_REFUSED_UNSUPPORTED, "moe: hidden and inter are multiples of 32, at most 8192 (NVFP4: 6144)");
+    for (MoeExpert& ex : table) CK(moe_encode_maps(fmt, &ex, (int)hidden, (int)inter));
     lq_moe* h = new lq_moe();
     h->device = ctx->device;
     h->fmt = fmt;
     h->max_tokens = std::min<size_t>(MOE_LAYER_MAX_TOKENS, MOE_LAYER_MAX_PAIRS / std::max<size_t>(k, 1));
     const size_t pairs = h->max_tokens * std::max<size_t>(k, 1);
     const size_t tb = a256(n_experts * sizeof(MoeExpert)), lb = a256(h->max_tokens * n_experts * 4),
-                 ab = a256(pairs * (size_t)inter * 4), pb = a256(pairs * (size_t)hidden * 4);
-    cudaError_t e = cudaMalloc(&h->raw, tb + lb + ab + pb + 256);
+                 ab = a256(pairs * (size_t)inter * 4), pb = a256(pairs * (size_t)hidden * 4), fixed = tb + lb + ab + pb;
+    h->sync_bytes = (MOE_LAYER_SYNC_WORDS + h->max_tokens * (size_t)(hidden / 16)) * 4;
+    cudaError_t e = cudaMalloc(&h->raw, fixed + h->sync_bytes);
     if (e == cudaSuccess) e = cudaMemcpyAsync(h->raw, table.data(), n_experts * sizeof(MoeExpert), cudaMemcpyHostToDevice, ctx->stream);
-    if (e == cudaSuccess) e = cudaMemsetAsync(h->raw + tb + lb + ab + pb, 0, 256, ctx->stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(h->raw + fixed, 0, h->sync_bytes, ctx->stream);
+    int nan_scale = 0;
+    if (fmt == LQ_FMT_MXFP4) {  // (the first counter serves as the answer's place, and is zeroed again)
+        if (e == cudaSuccess)
+            e = launch_moe_nan_scale((const MoeExpert*)h->raw, (int)n_experts, (int)hidden, (int)inter, (int*)(h->raw + fixed), ctx->stream);
+        if (e == cudaSuccess) e = cudaMemcpyAsync(&nan_scale, h->raw + fixed, 4, cudaMemcpyDeviceToHost, ctx->stream);
+        if (e == cudaSuccess) e = cudaMemsetAsync(h->raw + fixed, 0, 4, ctx->stream);
+    }
     if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
     if (e != cudaSuccess) {
         cudaGetLastError();
@@ -2474,12 +2484,22 @@ int lq_moe_create(lq_ctx* ctx, const lq_matrix* gates, const lq_matrix* ups, con
         delete h;
         return cuda_fail(ctx, e, "moe workspace");
     }
+    if (nan_scale) {
+        cudaFree(h->raw);
+        delete h;
+        return fail(ctx, LQ_REFUSED_UNSUPPORTED, "moe: an e8m0 scale is NaN (255)");
+    }
     MoeLayer& L = h->layer;
     L.table = (const MoeExpert*)h->raw;
     L.logits = (float*)(h->raw + tb);
     L.act = (float*)(h->raw + tb + lb);
     L.pair_out = (float*)(h->raw + tb + lb + ab);
-    L.barrier = (unsigned*)(h->raw + tb + lb + ab + pb);
+    L.exits = (unsigned*)(h->raw + fixed);
+    L.route_done = L.exits + 1;
+    L.group_done = L.route_done + 1;
+    L.x_max = L.group_done + MOE_LAYER_MAX_PAIRS;
+    L.act_max = L.x_max + MOE_LAYER_MAX_TOKENS;
+    L.out_done = L.act_max + MOE_LAYER_MAX_PAIRS;
     L.router = router, L.bias = router_bias, L.router_type = router_type;
     L.hidden = (int)hidden, L.inter = (int)inter, L.experts = (int)n_experts, L.top_e = (int)k;
     L.renormalise = renormalise != 0;

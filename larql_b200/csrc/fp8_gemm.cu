@@ -551,31 +551,9 @@ fp8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 }
 
 // ------------------------------------------------------------------ host ----
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeFn encode_fn() {
-    static EncodeFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<EncodeFn>(p);
-    }();
-    return fn;
-}
-
 // [rows][cols] bytes, box of 128 columns; what lies past the ends reads as zero (an e4m3 zero).
 cudaError_t encode_bytes(CUtensorMap* map, const void* base, size_t rows, size_t cols, size_t pitch, int box_rows) {
-    EncodeFn fn = encode_fn();
-    if (!fn) return cudaErrorNotSupported;
-    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
-    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, step[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, step,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+    return encode_tile_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, cols, pitch, box_rows, 128, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <class K>

@@ -1,5 +1,6 @@
 // Internal launch interface between the C-ABI layer and the kernels.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -88,6 +89,8 @@ struct FmtMat {
 
 // launch_util.cu: cudaFuncAttributeMaxDynamicSharedMemorySize, set once per (device, kernel)
 cudaError_t set_max_dyn_smem(const void* func, int bytes);
+cudaError_t encode_tile_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, size_t rows, size_t cols, size_t pitch,
+                            int box_rows, int box_cols, CUtensorMapSwizzle swizzle);
 
 // fmt_kernels.cu
 cudaError_t launch_scan_fmt(const FmtMat& m, const XPrep& xp, float* scores, uint32_t* hist, uint32_t* bound_bits,
@@ -221,7 +224,10 @@ cudaError_t launch_fp8_matmul(const Fp8Product& p, bool overlap, int sm_count, i
 #define MOE_LAYER_MAX_TOKENS 64
 #define MOE_LAYER_MAX_TOP 32
 #define MOE_LAYER_MAX_PAIRS 1024  // tokens x top_e of a launch
+// exits, route_done, group_done, x_max, act_max; out_done lies behind them
+#define MOE_LAYER_SYNC_WORDS (2 + MOE_LAYER_MAX_PAIRS + MOE_LAYER_MAX_TOKENS + MOE_LAYER_MAX_PAIRS)
 struct MoeExpert {
+    CUtensorMap map[3];        // over codes: a stage's columns of 16 rows
     const uint8_t* codes[3];   // gate, up [inter][hidden]; down [hidden][inter]
     const uint8_t* scales[3];
     float ts[3];
@@ -235,11 +241,17 @@ struct MoeLayer {
     void* out;                  // [tokens][hidden]
     uint32_t* idx_out;          // [tokens][top_e] or null
     float* w_out;
-    float *logits, *act, *pair_out;  // workspace: [tokens][experts], [pairs][inter], [pairs][hidden]
-    unsigned* barrier;               // two words, zero between launches but for the generation
-    int n_stages, stage_bytes;       // filled in by the launch
+    // workspace: [tokens][experts], [pairs][inter], [pairs][hidden]
+    float *logits, *act, *pair_out;
+    // counters, zero between launches: CTAs gone, router products done, units done per token group of an expert, results
+    // per token and 16 outputs; bits of the largest |value| per token / pair
+    unsigned *exits, *route_done, *group_done, *x_max, *act_max, *out_done;
+    int terms;                       // f16 terms per activation (filled in by the launch)
+    int n_stages, stage_bytes, scale_slots[2];  // filled in by the launch
     int* err;
 };
+cudaError_t launch_moe_nan_scale(const MoeExpert* table, int experts, int hidden, int inter, int* found, cudaStream_t st);
+cudaError_t moe_encode_maps(int fmt, MoeExpert* ex, int hidden, int inter);
 bool moe_layer_supported(int fmt, int hidden, int inter);
 cudaError_t launch_moe_layer(int fmt, const MoeLayer& L, int sm_count, cudaStream_t st);
 

@@ -7,44 +7,52 @@
 // experts (every feature), the router's product included.  Experts are MXFP4, NVFP4 or FP8_B128, gate and up
 // [inter, hidden], down [hidden, inter].
 //
-// What bounds it is reading the chosen experts' weights once.  One CTA per SM walks its share of the work in phases,
-// a grid barrier between them:
-//   route   the T x E router products (f64 sums: which of two near logits is larger decides a whole expert), spread
-//           over the grid; after the barrier every CTA picks the experts itself (the same result everywhere);
-//   gate/up units of 16 features of one expert for one group of its tokens: act = silu(gate) * up, f32, to global;
-//   down    units of 16 or 32 output rows, one result per (token, expert) pair;
-//   combine the pairs' weighted results in selection order.
-// A producer warp streams the units' rows through a ring in shared memory (bulk copies); it needs only the routing,
-// so it runs ahead across the barrier between gate/up and down.  The products run on the tensor cores (mma.sync
-// m16n8k16, f16 x f16 -> f32): weights are the 16 rows of A, tokens the 8 columns of B.  The codes of all three
-// formats are exact in f16; an f32 activation is brought to [2^14, 2^15) by a power of two per token and split
-// in two f16 terms (22 bits), which take two columns; bf16 activations take one (f16 carries all of their 8 bits).
-// Scales: e8m0 (per row and 32) and FP8 blocks on the f32 accumulators, e4m3 (per row and 16) multiplied into the f16
-// codes, which is exact (2 + 4 significant bits).  The contraction is split over the 8 warps of a CTA and added
-// up in a fixed order: results do not depend on timing.
+// What bounds it is reading the chosen experts' weights once.  One CTA per SM walks its share of the work:
+//   route    the T x E router products (twice f32's precision: which of two near logits is larger decides a whole
+//            expert), spread over the grid; then every CTA picks the experts itself;
+//   gate/up  units of 16 features of one expert for one group of its tokens: act = silu(gate) * up, f32, to global;
+//   down     units of 16 or 32 output rows, as soon as the expert's activations are complete (a counter per group, no
+//            grid barrier); whoever brings the last of a token's top_e results for some rows adds them up, in
+//            selection order.
+// Warps have three jobs.  A producer streams the units' rows through a ring in shared memory (one tile copy per 16
+// rows); it needs only the routing, so it runs ahead from gate/up into down while the activations are still on
+// their way.  16 compute warps multiply, each its part of the contraction, and leave their sums in shared memory.
+// Finishers add the parts up in a fixed order (results do not depend on timing), apply the activation or the
+// routing weight and publish: a publication waits for a fence and an atomic, a microsecond that a unit's
+// multiplication (also a microsecond) must not wait for.
+//
+// The products run on the tensor cores (mma.sync m16n8k16, f16 x f16 -> f32): weights are the 16 rows of A, tokens the 8
+// columns of B.  The codes of all three formats are exact in f16.  An activation is brought to [2^14, 2^15) by a
+// power of two per token; bf16 layers take one f16 term (all of a bf16's bits; activations between the products
+// rounded to f16's 11), f32 and f16 layers two (22 bits, a column each).  Scales: e8m0 (per row and 32) and
+// FP8 blocks multiply the f32 sums of 32 products, e4m3 (per row and 16) the f16 codes, which is exact (2 + 4 bits).
+// (Tried: e4m3 terms and m16n8k32 e4m3 products, which need no conversion of FP8 codes: that form is converted to f16
+// behind the instruction, 32 cycles of a scheduler against 2 x 8.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "../../include/larql_cuda.h"
 #include "codecs.cuh"
 #include "kernels.h"
+#include "tc5.cuh"
 
 namespace lq {
 
 namespace {
 
-constexpr int ML_WARPS = 8, ML_CONSUMERS = ML_WARPS * 32, ML_THREADS = ML_CONSUMERS + 32;
+constexpr int ML_WARPS = 16, ML_CONSUMERS = ML_WARPS * 32, ML_FINISH = 3, ML_THREADS = ML_CONSUMERS + 32 * (1 + ML_FINISH);
 constexpr int ML_MAX_STAGES = 12;
-constexpr int ML_RED_COL = 20;  // floats between two columns of a warp's partial sums (16 rows + padding against conflicts)
+// A warp's partial sums: 16 rows per column, the upper and lower 8 swapped in every second pair of columns so that the
+// lanes of a store (8 rows of four columns 2t) meet in a bank two at most.
+__device__ __forceinline__ int red_at(int col, int row) { return col * 16 + (row ^ ((col & 2) << 2)); }
 
 struct MlSmem {
     uint64_t full[ML_MAX_STAGES], empty[ML_MAX_STAGES];
-    uint64_t sfull[2], sempty[2];
-    double red[ML_WARPS];
-    float amax[16][ML_WARPS];   // per token of the group: the warps' parts of its largest |value|
+    uint64_t rfull[ML_FINISH], rempty[ML_FINISH];  // partial sums of a unit: written by every compute warp / read
+    float2 part[ML_THREADS / 32];
     float unscale[16];          // per token of the group: the power of two its values were divided by
     int gtok[16], gpair[16];    // the group's tokens and (token, slot) pairs
-    int n_active, n_groups;
+    int n_groups, cnt;
     int active[MOE_LAYER_MAX_EXPERTS];
     int gpre[MOE_LAYER_MAX_EXPERTS + 1];     // groups before the active expert
     unsigned mask[MOE_LAYER_MAX_EXPERTS][2]; // tokens that chose the expert
@@ -59,32 +67,90 @@ __device__ __forceinline__ float ld_as_f32(const void* p, int type, size_t at) {
     return __half2float(static_cast<const __half*>(p)[at]);
 }
 
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(ML_CONSUMERS) : "memory"); }
-
-// Grid barrier: the last CTA to arrive opens the next generation.  Bounded; false when it gave up.
-__device__ bool grid_arrive_and_wait(unsigned* bar, unsigned n) {
-    unsigned gen;
-    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(gen) : "l"(bar + 1) : "memory");
-    __threadfence();
-    if (atomicAdd(bar, 1u) == n - 1) {
-        bar[0] = 0;
-        __threadfence();
-        atomicAdd(bar + 1, 1u);
-        return true;
+// Eight consecutive elements, loaded first and converted later so that loads of several operands overlap.  WIDE: the
+// address is a multiple of 16 bytes.
+struct Raw8 {
+    uint4 a, b;
+};
+template <bool WIDE>
+__device__ __forceinline__ Raw8 ld8(const void* p, int type, size_t at) {
+    Raw8 r;
+    if (WIDE) {
+        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + at * (type == LQ_T_F32 ? 4 : 2));
+        r.a = __ldcg(q);
+        r.b = type == LQ_T_F32 ? __ldcg(q + 1) : make_uint4(0, 0, 0, 0);
+    } else if (type == LQ_T_F32) {
+        const uint32_t* q = static_cast<const uint32_t*>(p) + at;
+        r.a = make_uint4(q[0], q[1], q[2], q[3]);
+        r.b = make_uint4(q[4], q[5], q[6], q[7]);
+    } else {
+        const uint16_t* q = static_cast<const uint16_t*>(p) + at;
+        r.a = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
+        r.b = make_uint4(0, 0, 0, 0);
     }
-    const long long t0 = clock64();
-    for (unsigned it = 1;; ++it) {
-        unsigned now;
-        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(bar + 1) : "memory");
-        if (now != gen) return true;
-        if ((it & 255u) == 0 && clock64() - t0 > (1ll << 31)) return false;
+    return r;
+}
+__device__ __forceinline__ void to_f32(const Raw8& r, int type, float (&v)[8]) {
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+    if (type == LQ_T_F32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+    } else if (type == LQ_T_BF16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
     }
 }
 
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(ML_CONSUMERS) : "memory"); }
+
+// Bounded polls (about a second): an mbarrier phase, and a counter that other CTAs raise to at least `target`.
+__device__ __forceinline__ bool ml_wait(uint64_t* bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    for (uint32_t it = 1;; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((it & 255u) == 0 && clock64() - t0 > (1ll << 31)) return false;
+    }
+}
+__device__ bool wait_count(const unsigned* word, unsigned target) {
+    const long long t0 = clock64();
+    for (uint32_t it = 1;; ++it) {
+        unsigned now;
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(word) : "memory");
+        if (now >= target) return true;
+        if ((it & 255u) == 0 && clock64() - t0 > (1ll << 31)) return false;
+    }
+}
+__device__ __forceinline__ unsigned add_release(unsigned* word, unsigned n) {
+    unsigned before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], %2;" : "=r"(before) : "l"(word), "r"(n) : "memory");
+    return before;
+}
+__device__ __forceinline__ void ml_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Four 8 x 16-byte pieces of shared memory, lane l naming row l % 8 of piece l / 8: a lane gets word l % 4 of row l / 4.
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
 }
 // Eight e2m1 codes (low nibble first) -> four f16 pairs.
 __device__ __forceinline__ void e2m1x8(uint32_t w, uint32_t (&h)[4]) {
@@ -105,6 +171,20 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
     return r;
 }
 
+// A sum kept as an f32 and its error: products and additions split by the error-free transformations of Dekker and
+// Knuth (the dot product of Ogita, Rump and Oishi), as precise as if it were summed in twice f32's precision.
+__device__ __forceinline__ float2 pair_add(float2 a, float b) {
+    const float s = __fadd_rn(a.x, b), t = __fsub_rn(s, a.x);
+    const float e = __fadd_rn(__fsub_rn(a.x, __fsub_rn(s, t)), __fsub_rn(b, t));
+    return make_float2(s, __fadd_rn(a.y, e));
+}
+__device__ __forceinline__ float2 pair_fma(float2 a, float x, float y) {
+    const float p = __fmul_rn(x, y), e = __fmaf_rn(x, y, -p);
+    a = pair_add(a, p);
+    a.y = __fadd_rn(a.y, e);
+    return a;
+}
+
 // Bytes of `cols` codes, and of a row's scales.
 template <int FMT>
 __host__ __device__ constexpr int code_bytes(int cols) { return FMT == LQ_FMT_FP8_B128 ? cols : cols / 2; }
@@ -112,20 +192,16 @@ template <int FMT>
 __host__ __device__ constexpr int row_scale_bytes(int cols) {
     return FMT == LQ_FMT_MXFP4 ? cols / 32 : (FMT == LQ_FMT_NVFP4 ? cols / 16 : 0);
 }
-// Distance of two rows of a stage: the eight rows of a fragment load fall into different banks (4 bytes a thread for
-// FP4, 8 for FP8).
-template <int FMT>
-__host__ __device__ constexpr int stage_pitch(int kc) {
-    const int b = code_bytes<FMT>(kc);
-    return FMT == LQ_FMT_FP8_B128 ? (b % 64 == 0 ? b + 32 : b) : (b % 32 == 0 ? b + 16 : b);
-}
 // Distance of two columns of the activations: two columns (a phase of a 16-byte load) fall into different banks.
 __host__ __device__ constexpr int act_pitch(int k) { return (2 * k) % 128 == 0 ? 2 * k + 64 : 2 * k; }
-// Columns of the contraction per stage: at most 1024 (512 for FP8), in equal parts, whole 32s.
+// Columns of the contraction per stage: equal parts of at most 47 blocks of 32 (23 for FP8, and for long rows, whose
+// activations take most of shared memory), an odd number of them.  A
+// stage holds its rows back to back as the tile copy lays them; an odd number of 16-byte pieces per row would put the
+// eight rows of a fragment load into different banks (FP8 rows, 32 bytes a block, keep a two-way conflict).
 template <int FMT>
 __host__ __device__ constexpr int chunk_cols(int k) {
-    const int most = FMT == LQ_FMT_FP8_B128 ? 512 : 1024, n = (k + most - 1) / most;
-    return ((k + n - 1) / n + 31) / 32 * 32;
+    const int blocks = k / 32, most = FMT == LQ_FMT_FP8_B128 || k > 4096 ? 23 : 47, n = (blocks + most - 1) / most;
+    return (((blocks + n - 1) / n) | 1) * 32;
 }
 
 // One phase's products as the kernel walks them.
@@ -133,16 +209,20 @@ struct Walk {
     int k, chunk, n_chunks, pitch;  // contraction, columns per stage, stages per unit, bytes between stage rows
     int units_per_group, tiles;     // 16-row tiles per unit: 2 (gate + up, or 32 rows) or 1
     int is_down;
+    uint8_t* scales;                // [slots] scales of a unit's rows
+    int slots;
 };
 
 template <int FMT>
-__device__ __forceinline__ Walk walk_of(const MoeLayer& L, bool down, int n_groups) {
+__device__ __forceinline__ Walk walk_of(const MoeLayer& L, bool down, int n_groups, uint8_t* sbuf) {
     Walk w;
+    w.scales = sbuf + (down ? 32 * L.scale_slots[0] * row_scale_bytes<FMT>(L.hidden) : 0);
+    w.slots = L.scale_slots[down];
     w.is_down = down;
     w.k = down ? L.inter : L.hidden;
     w.chunk = chunk_cols<FMT>(w.k);
     w.n_chunks = (w.k + w.chunk - 1) / w.chunk;
-    w.pitch = stage_pitch<FMT>(w.chunk);
+    w.pitch = code_bytes<FMT>(w.chunk);
     if (!down) {
         w.tiles = 2;
         w.units_per_group = L.inter / 16;
@@ -160,118 +240,163 @@ __device__ __forceinline__ int expert_of(const MlSmem& sh, int gi, int from) {
     return from;
 }
 
-template <int FMT, int NT, int TERMS>
-__global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const MoeLayer L) {
+// The experts of token t, into shared memory: a warp takes top_e rounds of the largest logit left, the lowest index
+// among equals.  Every CTA does it for every token (a publication by one would cost the others a microsecond more).
+__device__ void route_token(const MoeLayer& L, MlSmem& sh, int t, int lane) {
+    constexpr int PER = MOE_LAYER_MAX_EXPERTS / 32;
+    const int E = L.experts, K = L.top_e;
+    uint32_t key[PER];  // logits as integers of the same order; 0: taken (a NaN, 1, comes last: the weights are NaN then)
+    float mx = -INFINITY, sum = 0.0f, mine = 0.0f;
+    int chosen = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        key[i] = 0;
+        if (i * 32 < E && i * 32 + lane < E) {
+            const float l = __ldcg(L.logits + (size_t)t * E + i * 32 + lane);
+            const uint32_t u = __float_as_uint(l);
+            key[i] = l != l ? 1u : ((u & 0x80000000u) ? ~u : (u | 0x80000000u));
+        }
+    }
+    auto value = [](uint32_t k) { return k == 1u ? __uint_as_float(0x7fc00000u) : __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); };
+    for (int j = 0; j < K; ++j) {
+        uint32_t best = 0, at = 0xffffffffu;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (i * 32 < E && key[i] > best) {
+                best = key[i];
+                at = i * 32 + lane;
+            }
+        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+        const uint32_t e = __reduce_min_sync(0xffffffffu, best == top ? at : 0xffffffffu);
+        if (j == 0) {
+            mx = value(top);
+            if (!L.renormalise) {  // the sum over all experts, before any is taken out
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (i * 32 < E && i * 32 + lane < E) sum += expf(value(key[i]) - mx);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (i * 32 < E && i * 32 + lane == e) key[i] = 0;
+        if (j == lane) {
+            mine = expf(value(top) - mx);
+            chosen = (int)e;
+        }
+    }
+    if (L.renormalise) sum = lane < K ? mine : 0.0f;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane < K) {
+        const float w = mine / sum;
+        sh.idx[t * K + lane] = chosen;
+        sh.w[t * K + lane] = w;
+        atomicOr(&sh.mask[chosen][t >> 5], 1u << (t & 31));
+        if (blockIdx.x == 0) {
+            if (L.idx_out) L.idx_out[(size_t)t * K + lane] = (uint32_t)chosen;
+            if (L.w_out) L.w_out[(size_t)t * K + lane] = w;
+        }
+    }
+}
+
+template <int FMT, int NT>
+__global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_constant__ MoeLayer L) {
     extern __shared__ __align__(128) uint8_t smem[];
-    constexpr int TG = NT * 8 / TERMS;  // tokens per group
-    constexpr int RED = 2 * NT * 8 * ML_RED_COL;  // floats of a warp's partial sums
+    constexpr int RED = NT * 8 * 16;  // floats of a warp's partial sums
     MlSmem& sh = *reinterpret_cast<MlSmem*>(smem);
     uint8_t* p = smem + (sizeof(MlSmem) + 127) / 128 * 128;
-    float* red = reinterpret_cast<float*>(p);                 // [2][ML_WARPS][RED]
-    p += 2 * ML_WARPS * RED * 4;
+    float* red = reinterpret_cast<float*>(p);                 // [ML_FINISH][ML_WARPS][RED]
+    p += ML_FINISH * ML_WARPS * RED * 4;
     uint8_t* xs = p;                                          // [NT * 8] columns of f16
     p += (size_t)NT * 8 * max(act_pitch(L.hidden), act_pitch(L.inter));
-    uint8_t* sbuf = p;                                        // [2] scales of a unit's rows
-    const int sbytes = max(row_scale_bytes<FMT>(L.hidden), row_scale_bytes<FMT>(L.inter)) * 32;
-    p += 2 * sbytes;
-    uint8_t* ring = p;                                        // [n_stages][32 rows]
+    uint8_t* sbuf = p;                                        // scales of the units' rows, [scale_slots] per phase
+    p += 32 * (L.scale_slots[0] * row_scale_bytes<FMT>(L.hidden) + L.scale_slots[1] * row_scale_bytes<FMT>(L.inter));
+    uint8_t* ring = smem + (p - smem + 127) / 128 * 128;      // [n_stages][32 rows]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int T = L.tokens, E = L.experts, K = L.top_e;
+    const int terms = L.terms, TG = NT * 8 / terms;  // columns and tokens per group
+    const bool x_wide = (reinterpret_cast<uintptr_t>(L.x) & 15) == 0;  // (rows are multiples of 32 elements)
 
     if (tid == 0) {
         for (int i = 0; i < L.n_stages; ++i) {
             mbar_init(&sh.full[i], 1);
             mbar_init(&sh.empty[i], ML_WARPS);
         }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.sfull[i], 1);
-            mbar_init(&sh.sempty[i], ML_WARPS);
+        for (int i = 0; i < ML_FINISH; ++i) {
+            mbar_init(&sh.rfull[i], ML_WARPS);
+            mbar_init(&sh.rempty[i], 1);
         }
         sh.failed = 0;
         fence_mbar_init();
     }
     for (int i = tid; i < 2 * E; i += ML_THREADS) sh.mask[i >> 1][i & 1] = 0;
 
-    // ---- route ----
+    // ---- route: an item is one token's product with one expert's row, worked on by as many warps as there are to spare ----
     {
+        constexpr int WARPS = ML_THREADS / 32;
         const int items = T * E;
-        const bool whole = items <= 2 * (int)gridDim.x;  // a product per CTA, or per warp
-        const int step = whole ? gridDim.x : gridDim.x * (ML_THREADS / 32);
-        const int n_thr = whole ? ML_THREADS : 32, me = whole ? tid : lane;
-        for (int it = whole ? blockIdx.x : blockIdx.x * (ML_THREADS / 32) + warp; it < items; it += step) {
-            const int t = it / E, e = it - t * E;
-            double s = 0.0;
-            for (int i = me; i < L.hidden; i += n_thr)
-                s = fma((double)ld_as_f32(L.x, L.type, (size_t)t * L.hidden + i), (double)ld_as_f32(L.router, L.router_type, (size_t)e * L.hidden + i), s);
-            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            if (whole) {
-                __syncthreads();
-                if (lane == 0) reinterpret_cast<double*>(red)[warp] = s;
-                __syncthreads();
-                s = 0.0;
-                for (int i = 0; i < ML_THREADS / 32; ++i) s += reinterpret_cast<double*>(red)[i];
-            }
-            if (me == 0) L.logits[it] = (float)(s + (L.bias ? (double)ld_as_f32(L.bias, L.router_type, e) : 0.0));
-        }
-    }
-    __syncthreads();
-    if (tid == 0 && !grid_arrive_and_wait(L.barrier, gridDim.x)) sh.failed = 1;
-    __syncthreads();
-    for (int t = warp; t < T; t += ML_THREADS / 32) {
-        // a warp per token: K rounds of the largest (logit, lowest index) left
-        constexpr int PER = MOE_LAYER_MAX_EXPERTS / 32;
-        unsigned long long key[PER];
-        float lg[PER];
+        const bool r_wide = (reinterpret_cast<uintptr_t>(L.router) & 15) == 0;
+        const int W = items <= (int)gridDim.x ? WARPS : (items <= 5 * (int)gridDim.x ? 4 : (items <= 10 * (int)gridDim.x ? 2 : 1));
+        const int per_cta = WARPS / W, sub = warp / W, part = (warp % W) * 32 + lane;
+        const int rounds = (items + (int)gridDim.x * per_cta - 1) / ((int)gridDim.x * per_cta);
+        for (int r = 0; r < rounds; ++r) {
+            const int it = (r * per_cta + sub) * gridDim.x + blockIdx.x;
+            const bool on = it < items;
+            const int t = on ? it / E : 0, e = on ? it - t * E : 0;
+            float2 s = make_float2(0.0f, 0.0f);
+            float m = 0.0f;
+            if (on) {
+                auto products = [&](auto wide) {
+#pragma unroll 2
+                    for (int i = part * 8; i < L.hidden; i += W * 256) {
+                        const Raw8 rr = ld8<decltype(wide)::value>(L.router, L.router_type, (size_t)e * L.hidden + i);
+                        const Raw8 xr = ld8<decltype(wide)::value>(L.x, L.type, (size_t)t * L.hidden + i);
+                        float rv[8], xv[8];
+                        to_f32(rr, L.router_type, rv);
+                        to_f32(xr, L.type, xv);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = i * 32 + lane;
-            lg[i] = e < E ? __ldcg(L.logits + (size_t)t * E + e) : -INFINITY;
-            uint32_t u = __float_as_uint(lg[i]);
-            u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-            if (lg[i] != lg[i]) u = 1;  // a NaN is taken last; the weights become NaN all the same
-            key[i] = e < E ? ((unsigned long long)u << 32) | (uint32_t)(0xffffffffu - e) : 0ull;
-        }
-        float mx = -INFINITY, sum = 0.0f, mine = 0.0f;
-        int chosen = 0;
-        for (int j = 0; j < K; ++j) {
-            unsigned long long best = 0;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) best = max(best, key[i]);
-            for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-            const int e = (int)(0xffffffffu - (uint32_t)best);
-            float l = 0.0f;
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (i == (e >> 5)) {
-                    l = lg[i];
-                    if (lane == (e & 31)) key[i] = 0;
+                        for (int j = 0; j < 8; ++j) {
+                            s = pair_fma(s, xv[j], rv[j]);
+                            m = fmaxf(m, fabsf(xv[j]));
+                        }
+                    }
+                };
+                if (x_wide && r_wide) products(std::true_type{});
+                else products(std::false_type{});
+                // the token's largest |value|, for its power of two (bits of non-negative floats order as integers)
+                if (e == 0) {
+                    const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+                    if (lane == 0) atomicMax(L.x_max + t, top);
                 }
-            l = __shfl_sync(0xffffffffu, l, e & 31);
-            if (j == 0) mx = l;
-            if (j == lane) {
-                mine = expf(l - mx);
-                chosen = e;
+            }
+            auto fold = [&](int from) {
+                for (int o = from; o > 0; o >>= 1) {
+                    const float ox = __shfl_down_sync(0xffffffffu, s.x, o), oy = __shfl_down_sync(0xffffffffu, s.y, o);
+                    s = pair_add(s, ox);
+                    s.y = __fadd_rn(s.y, oy);
+                }
+            };
+            fold(16);
+            if (W > 1) {
+                if (lane == 0) sh.part[warp] = s;
+                __syncthreads();
+                s = lane < W ? sh.part[sub * W + lane] : make_float2(0.0f, 0.0f);
+                if (warp % W == 0) fold(16);
+                __syncthreads();
+            }
+            if (on && warp % W == 0 && lane == 0) {
+                if (L.bias) s = pair_add(s, ld_as_f32(L.bias, L.router_type, e));
+                L.logits[it] = __fadd_rn(s.x, s.y);
+                add_release(L.route_done, 1u);
             }
         }
-        if (L.renormalise) {
-            sum = lane < K ? mine : 0.0f;
-        } else {
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (i * 32 + lane < E) sum += expf(lg[i] - mx);
-        }
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane < K) {
-            const float w = mine / sum;
-            sh.idx[t * K + lane] = chosen;
-            sh.w[t * K + lane] = w;
-            atomicOr(&sh.mask[chosen][t >> 5], 1u << (t & 31));
-            if (blockIdx.x == 0) {
-                if (L.idx_out) L.idx_out[(size_t)t * K + lane] = (uint32_t)chosen;
-                if (L.w_out) L.w_out[(size_t)t * K + lane] = w;
-            }
-        }
+        if (tid == 0 && !wait_count(L.route_done, (unsigned)items)) sh.failed = 1;
     }
+    __syncthreads();
+    if (sh.failed) {  // no routing to go by: leave (the counters are cleared by the host)
+        if (tid == 0) set_err(L.err, DEV_ERR_TMA_TIMEOUT);
+        return;
+    }
+    for (int t = warp; t < T; t += ML_THREADS / 32) route_token(L, sh, t, lane);
     __syncthreads();
     if (warp == 0) {  // the chosen experts in order, and their token groups
         int n = 0, groups = 0;
@@ -295,7 +420,6 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const MoeLayer
         }
         if (lane == 0) {
             sh.gpre[n] = groups;
-            sh.n_active = n;
             sh.n_groups = groups;
         }
     }
@@ -307,74 +431,164 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const MoeLayer
         bool ok = true;
         int n = 0, un = 0;  // stages and units so far
         for (int ph = 0; ph < 2 && ok; ++ph) {
-            const Walk w = walk_of<FMT>(L, ph == 1, n_groups);
-            const long long total = (long long)n_groups * w.units_per_group;
-            const long long ua = total * blockIdx.x / gridDim.x, ub = total * (blockIdx.x + 1) / gridDim.x;
-            int a = 0;
-            for (long long u = ua; u < ub && ok; ++u) {
-                const int gi = (int)(u / w.units_per_group), tile = (int)(u - (long long)gi * w.units_per_group);
-                a = expert_of(sh, gi, a);
-                const MoeExpert& ex = L.table[sh.active[a]];
-                const size_t row_bytes = (size_t)code_bytes<FMT>(w.k);
-                if (row_scale_bytes<FMT>(w.k)) {
-                    const int s = un & 1;
-                    if (un >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&sh.sempty[s], (uint32_t)(un / 2 - 1) & 1u));
+            const Walk w = walk_of<FMT>(L, ph == 1, n_groups, sbuf);
+            const int total = n_groups * w.units_per_group;
+            const int ua = (int)((long long)total * blockIdx.x / gridDim.x), ub = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
+            if (ua >= ub) continue;
+            int gi = ua / w.units_per_group, tile = ua - gi * w.units_per_group, a = -1;
+            const CUtensorMap *m0 = nullptr, *m1 = nullptr;
+            const uint8_t *sc0 = nullptr, *sc1 = nullptr;
+            const uint32_t sbytes16 = 16u * row_scale_bytes<FMT>(w.k), code16 = 16u * w.pitch;
+            for (int u = ua; u < ub && ok; ++u, ++un) {
+                if (a < 0 || tile == w.units_per_group) {
+                    if (a >= 0) ++gi, tile = 0;
+                    a = expert_of(sh, gi, max(a, 0));
+                    const MoeExpert& ex = L.table[sh.active[a]];
+                    m0 = &ex.map[w.is_down ? 2 : 0], m1 = &ex.map[w.is_down ? 2 : 1];
+                    sc0 = ex.scales[w.is_down ? 2 : 0], sc1 = ex.scales[w.is_down ? 2 : 1];
+                }
+                const int row0 = (w.is_down ? tile * w.tiles : tile) * 16, row1 = w.is_down ? row0 + 16 : row0;
+                for (int c = 0; c < w.n_chunks; ++c, ++n) {
+                    const int st = n % L.n_stages;
+                    if (n >= L.n_stages) ok = __all_sync(0xffffffffu, ml_wait(&sh.empty[st], (uint32_t)(n / L.n_stages - 1) & 1u));
                     if (!ok) break;
-                    if (lane == 0) {
-                        const uint32_t bytes = 16u * row_scale_bytes<FMT>(w.k);
-                        mbar_expect_tx(&sh.sfull[s], bytes * w.tiles);
-                        for (int i = 0; i < w.tiles; ++i) {
-                            const uint8_t* src = w.is_down ? ex.scales[2] + (size_t)(tile * w.tiles + i) * bytes : ex.scales[i] + (size_t)tile * bytes;
-                            tma_bulk_g2s(sbuf + s * sbytes + i * bytes, src, bytes, &sh.sfull[s]);
+                    if (lane == 0) {  // (columns past the row's end arrive as zeros and count as bytes)
+                        const bool with_scales = sbytes16 && c == 0;
+                        mbar_expect_tx(&sh.full[st], (code16 + (with_scales ? sbytes16 : 0u)) * w.tiles);
+                        uint8_t* dst = ring + (size_t)st * L.stage_bytes;
+                        const int x = code_bytes<FMT>(c * w.chunk) / 4;
+                        tma_load_2d(dst, m0, x, row0, &sh.full[st]);
+                        if (w.tiles == 2) tma_load_2d(dst + code16, m1, x, row1, &sh.full[st]);
+                        if (with_scales) {
+                            // the unit's scales come with its first stage.  Their slot is free: the stage this one replaces was
+                            // consumed, and scale_slots units do not fit between the two
+                            uint8_t* sd = w.scales + (un % w.slots) * 2 * sbytes16;
+                            tma_bulk_g2s(sd, sc0 + (size_t)(row0 >> 4) * sbytes16, sbytes16, &sh.full[st]);
+                            if (w.tiles == 2) tma_bulk_g2s(sd + sbytes16, sc1 + (size_t)(row1 >> 4) * sbytes16, sbytes16, &sh.full[st]);
                         }
                     }
-                }
-                ++un;
-                for (int c = 0; c < w.n_chunks; ++c, ++n) {
-                    const int st = n % L.n_stages, k0 = c * w.chunk;
-                    if (n >= L.n_stages) ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[st], (uint32_t)(n / L.n_stages - 1) & 1u));
-                    if (!ok) break;
-                    const uint32_t bytes = (uint32_t)code_bytes<FMT>(min(w.chunk, w.k - k0));
-                    if (lane == 0) mbar_expect_tx(&sh.full[st], bytes * 16u * w.tiles);
                     __syncwarp();
-                    if (lane < 16 * w.tiles) {
-                        const uint8_t* m = w.is_down ? ex.codes[2] : ex.codes[lane >> 4];
-                        const size_t row = w.is_down ? (size_t)tile * 16 * w.tiles + lane : (size_t)tile * 16 + (lane & 15);
-                        tma_bulk_g2s(ring + (size_t)st * L.stage_bytes + lane * w.pitch, m + row * row_bytes + code_bytes<FMT>(k0), bytes,
-                                     &sh.full[st]);
-                    }
                 }
+                ++tile;
             }
         }
         if (!ok) {  // the copies in flight have to land before the block's shared memory goes away
-            for (int v = max(0, n - L.n_stages); v < n; ++v) mbar_wait(&sh.full[v % L.n_stages], (uint32_t)(v / L.n_stages) & 1u);
-            if (row_scale_bytes<FMT>(L.hidden))
-                for (int v = max(0, un - 2); v < un; ++v) mbar_wait(&sh.sfull[v & 1], (uint32_t)(v / 2) & 1u);
+            for (int v = max(0, n - L.n_stages); v < n; ++v) ml_wait(&sh.full[v % L.n_stages], (uint32_t)(v / L.n_stages) & 1u);
             sh.failed = 1;
         }
     } else {
-        // ---- consumers ----
+        // ---- compute warps and finishers walk the same units ----
+        const bool computes = warp < ML_WARPS;
         const int g = lane >> 2, t4 = lane & 3;
-        bool ok = true;  // a wait that ran out is not waited for again; barriers and arrivals are kept
+        bool ok = true;  // a wait that ran out is not waited for again; barriers, arrivals and counters are kept
         int n = 0, un = 0;
         for (int ph = 0; ph < 2; ++ph) {
-            const Walk w = walk_of<FMT>(L, ph == 1, n_groups);
+            const Walk w = walk_of<FMT>(L, ph == 1, n_groups, sbuf);
             const int xpitch = act_pitch(w.k), srow = row_scale_bytes<FMT>(w.k);
-            const long long total = (long long)n_groups * w.units_per_group;
-            const long long ua = total * blockIdx.x / gridDim.x, ub = total * (blockIdx.x + 1) / gridDim.x;
-            int a = 0, cur = -1, cnt = 0;
-            for (long long u = ua; u < ub; ++u, ++un) {
-                const int gi = (int)(u / w.units_per_group), tile = (int)(u - (long long)gi * w.units_per_group);
-                a = expert_of(sh, gi, a);
+            const int total = n_groups * w.units_per_group;
+            const int ua = (int)((long long)total * blockIdx.x / gridDim.x), ub = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
+            if (ua >= ub) continue;
+            int gi = ua / w.units_per_group, tile = ua - gi * w.units_per_group, a = expert_of(sh, gi, 0);
+            if (!computes) {
+                // ---- finishers: every ML_FINISH-th unit, each with a buffer of its own (it sees all of its phases) ----
+                const int buf = warp - ML_WARPS - 1;
+                for (int u = ua; u < ub; ++u, ++un, ++tile) {
+                    if (tile == w.units_per_group) {
+                        ++gi, tile = 0;
+                        a = expert_of(sh, gi, a);
+                    }
+                    if (un % ML_FINISH != buf) continue;
+                    const MoeExpert& ex = L.table[sh.active[a]];
+                    const int row = lane & 15, half = lane >> 4;
+                    const float ts = ex.ts[w.is_down ? 2 : half];
+                    if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.rfull[buf], (uint32_t)(un / ML_FINISH) & 1u));
+                    const int cnt = sh.cnt;
+                    // lane i keeps what belongs to token i of the group
+                    int pair = 0, t = 0;
+                    float scale = 0.0f;
+                    if (lane < cnt) {
+                        pair = sh.gpair[lane];
+                        t = sh.gtok[lane];
+                        // (the routing weight goes into the power of two, so that only the weighted output has to be in range)
+                        scale = sh.unscale[lane] * (w.is_down ? sh.w[pair] : 1.0f);
+                    }
+                    const float* all = red + (size_t)buf * ML_WARPS * RED;
+                    // two tiles: a half of the lanes each; one tile: the halves take half of the warps' parts each
+                    const int q0 = w.tiles == 2 ? half : half * (ML_WARPS / 2), qs = w.tiles == 2 ? 2 : 1;
+                    float top = 0.0f;
+                    for (int i = 0; i < cnt; ++i) {
+                        float v = 0.0f;
+#pragma unroll
+                        for (int q = 0; q < ML_WARPS / 2; ++q) {
+                            const float* c = all + (size_t)(q0 + q * qs) * RED;
+                            v += terms == 2 ? c[red_at(2 * i, row)] + c[red_at(2 * i + 1, row)] : c[red_at(i, row)];
+                        }
+                        if (w.tiles == 1) v += __shfl_xor_sync(0xffffffffu, v, 16);
+                        v = v * __shfl_sync(0xffffffffu, scale, i) * ts;
+                        const size_t at = (size_t)__shfl_sync(0xffffffffu, pair, i);
+                        if (!w.is_down) {
+                            const float up = __shfl_down_sync(0xffffffffu, v, 16);
+                            const float act = v / (1.0f + expf(-v)) * up;
+                            if (half == 0) __stcg(L.act + at * L.inter + tile * 16 + row, act);
+                            // the pair's largest |value| (a NaN's bits are above every number's)
+                            const unsigned m = __reduce_max_sync(0xffffffffu, half == 0 ? __float_as_uint(act) & 0x7fffffffu : 0u);
+                            if (lane == i) top = __uint_as_float(m);
+                        } else if (w.tiles == 2 || half == 0) {
+                            __stcg(L.pair_out + at * L.hidden + (tile * w.tiles + (w.tiles == 2 ? half : 0)) * 16 + row, v);
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) ml_arrive(&sh.rempty[buf]);
+                    if (!w.is_down) {
+                        if (lane < cnt) atomicMax(L.act_max + pair, __float_as_uint(top));
+                        __threadfence();
+                        __syncwarp();
+                        if (lane == 0) add_release(L.group_done + gi, 1u);
+                        continue;
+                    }
+                    __threadfence();
+                    __syncwarp();
+                    bool last = false;
+                    unsigned* word = L.out_done + (size_t)t * (L.hidden / 16) + tile * w.tiles;
+                    if (lane < cnt) last = add_release(word, 1u) == (unsigned)K - 1;
+                    unsigned done = __ballot_sync(0xffffffffu, last);
+                    if (last) *word = 0;  // ready for the next launch
+                    if (done) __threadfence();
+                    for (; done; done &= done - 1) {
+                        const int tt = __shfl_sync(0xffffffffu, t, __ffs(done) - 1);
+                        if (w.tiles == 1 && half) continue;
+                        const int h = (tile * w.tiles + half) * 16 + row;
+                        float s = 0.0f;
+                        for (int j = 0; j < K; ++j) s += __ldcg(L.pair_out + (size_t)(tt * K + j) * L.hidden + h);
+                        const size_t at = (size_t)tt * L.hidden + h;
+                        if (L.type == LQ_T_F32) static_cast<float*>(L.out)[at] = s;
+                        else if (L.type == LQ_T_BF16) static_cast<__nv_bfloat16*>(L.out)[at] = __float2bfloat16_rn(s);
+                        else static_cast<__half*>(L.out)[at] = __float2half_rn(s);
+                    }
+                    __syncwarp();
+                }
+                continue;
+            }
+            // compute warps: one 16-row tile each, every kgroups-th pair of blocks of the contraction
+            const int my_tile = w.tiles == 2 ? (warp & 1) : 0, kg = w.tiles == 2 ? warp >> 1 : warp, kgroups = ML_WARPS / w.tiles;
+            int cur = -1, cols = 0;
+            for (int u = ua; u < ub; ++u, ++un, ++tile) {
+                if (tile == w.units_per_group) {
+                    ++gi, tile = 0;
+                    a = expert_of(sh, gi, a);
+                }
                 const int e = sh.active[a];
-                const MoeExpert& ex = L.table[e];
                 if (gi != cur) {
                     // the group's tokens: which they are, and their activations as columns of f16
                     cur = gi;
                     const int first = (gi - sh.gpre[a]) * TG;
                     const unsigned long long m0 = sh.mask[e][0] | ((unsigned long long)sh.mask[e][1] << 32);
-                    cnt = min(TG, __popcll(m0) - first);
-                    consumers_sync();  // everyone is done with the previous group
+                    const int cnt = min(TG, __popcll(m0) - first);
+                    cols = (cnt * terms + 7) / 8;
+                    // the finishers are done with the previous group's units, the compute warps with its activations
+                    for (int v = max(0, un - ML_FINISH); v < un; ++v)
+                        if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.rempty[v % ML_FINISH], (uint32_t)(v / ML_FINISH) & 1u));
+                    consumers_sync();
                     if (tid < cnt) {
                         unsigned long long m = m0;
                         for (int i = 0; i < first + tid; ++i) m &= m - 1;
@@ -383,223 +597,284 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const MoeLayer
                         while (sh.idx[t * K + j] != e) ++j;
                         sh.gtok[tid] = t;
                         sh.gpair[tid] = t * K + j;
+                        sh.cnt = cnt;
                     }
+                    // down: the activations of the whole group, from every CTA that made some of them
+                    if (w.is_down && tid == 0 && ok && !wait_count(L.group_done + gi, (unsigned)(L.inter / 16))) sh.failed = 1;
                     consumers_sync();
                     // the warps share the rows out: `per` warps a token
-                    const int per = cnt >= 5 ? 1 : (cnt >= 3 ? 2 : (cnt == 2 ? 4 : 8)), at_once = ML_WARPS / per;
-                    for (int i0 = 0; i0 < cnt; i0 += at_once) {
-                        const int i = i0 + warp / per, part = (warp % per) * 32 + lane;
-                        if (i < cnt) {
-                            float m = 0.0f;
-                            for (int k = part; k < w.k; k += per * 32) {
-                                const float v = w.is_down ? __ldcg(L.act + (size_t)sh.gpair[i] * w.k + k) : ld_as_f32(L.x, L.type, (size_t)sh.gtok[i] * w.k + k);
-                                m = fmaxf(m, fabsf(v));
+                    const int per = cnt >= 9 ? 1 : (cnt >= 5 ? 2 : (cnt >= 3 ? 4 : (cnt == 2 ? 8 : 16)));
+                    const int i = warp / per, part = (warp % per) * 32 + lane;
+                    if (i < cnt) {
+                        // exponent of the largest value -> 2^14 (kept where both powers of two are normal numbers)
+                        const unsigned bits = __ldcg(w.is_down ? L.act_max + sh.gpair[i] : L.x_max + sh.gtok[i]);
+                        const int ex2 = min(max((int)(bits >> 23), 15), 254);
+                        // (an infinity makes the whole token NaN, like a NaN)
+                        const float down = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(127 + 14 + 127 - ex2) << 23);
+                        if (part == 0) sh.unscale[i] = __uint_as_float((uint32_t)(ex2 - 14) << 23);
+                        const size_t row = (size_t)(w.is_down ? sh.gpair[i] : sh.gtok[i]) * w.k;
+                        uint8_t* dst = xs + (size_t)(i * terms) * xpitch;
+                        const void* src = w.is_down ? L.act : L.x;
+                        const int type = w.is_down ? LQ_T_F32 : L.type;
+                        const bool wide = w.is_down || x_wide;
+#pragma unroll 2
+                        for (int k = part * 8; k < w.k; k += per * 256) {
+                            float v[8];
+                            to_f32(wide ? ld8<true>(src, type, row + k) : ld8<false>(src, type, row + k), type, v);
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const float x0 = v[2 * q] * down, x1 = v[2 * q + 1] * down;
+                                const __half2 h = __floats2half2_rn(x0, x1);
+                                const float2 f = __half22float2(h);
+                                const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
+                                hi[q] = *reinterpret_cast<const uint32_t*>(&h);
+                                lo[q] = *reinterpret_cast<const uint32_t*>(&l);
                             }
-                            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                            if (lane == 0) sh.amax[i][warp % per] = m;
-                        }
-                    }
-                    consumers_sync();
-                    for (int i0 = 0; i0 < cnt; i0 += at_once) {
-                        const int i = i0 + warp / per, part = (warp % per) * 32 + lane;
-                        if (i < cnt) {
-                            float m = 0.0f;
-                            for (int q = 0; q < per; ++q) m = fmaxf(m, sh.amax[i][q]);
-                            // exponent of the largest value -> 2^14 (kept where both powers of two are normal numbers)
-                            const int ex2 = min(max((int)(__float_as_uint(m) >> 23), 15), 254);
-                            const float down = __uint_as_float((uint32_t)(127 + 14 + 127 - ex2) << 23);
-                            if (warp % per == 0 && lane == 0) sh.unscale[i] = __uint_as_float((uint32_t)(ex2 - 14) << 23);
-                            for (int k = part; k < w.k; k += per * 32) {
-                                const float v = (w.is_down ? __ldcg(L.act + (size_t)sh.gpair[i] * w.k + k) : ld_as_f32(L.x, L.type, (size_t)sh.gtok[i] * w.k + k)) * down;
-                                const __half hi = __float2half_rn(v);
-                                *reinterpret_cast<__half*>(xs + (size_t)(i * TERMS) * xpitch + 2 * k) = hi;
-                                if (TERMS == 2)
-                                    *reinterpret_cast<__half*>(xs + (size_t)(i * TERMS + 1) * xpitch + 2 * k) = __float2half_rn(v - __half2float(hi));
+                            if (FMT == LQ_FMT_FP8_B128) {
+                                // a lane's 8 columns of a block: 4 of either half (what its two code words hold)
+                                uint8_t* q = dst + 2 * (k & ~31) + ((k & 15) >> 2) * 16 + ((k >> 4) & 1) * 8;
+                                *reinterpret_cast<uint2*>(q) = make_uint2(hi[0], hi[1]);
+                                *reinterpret_cast<uint2*>(q + 16) = make_uint2(hi[2], hi[3]);
+                                if (terms == 2) {
+                                    *reinterpret_cast<uint2*>(q + xpitch) = make_uint2(lo[0], lo[1]);
+                                    *reinterpret_cast<uint2*>(q + xpitch + 16) = make_uint2(lo[2], lo[3]);
+                                }
+                            } else {
+                                *reinterpret_cast<uint4*>(dst + 2 * k) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                                if (terms == 2) *reinterpret_cast<uint4*>(dst + xpitch + 2 * k) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                             }
                         }
                     }
                     consumers_sync();
                 }
-                float acc[2][NT][4];
+                float acc[NT][4], acc2[NT][4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) acc[i][j][q] = 0.0f;
-                if (FMT != LQ_FMT_FP8_B128 && ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.sfull[un & 1], (uint32_t)(un / 2) & 1u));
-                const uint8_t* sc = sbuf + (un & 1) * sbytes;
+                    for (int q = 0; q < 4; ++q) acc[j][q] = acc2[j][q] = 0.0f;
+                const uint8_t* s0 = w.scales + (un % w.slots) * 32 * srow + (my_tile * 16 + g) * srow;
+                const uint8_t* s1 = s0 + 8 * srow;
+                const float* fs = nullptr;
+                if (FMT == LQ_FMT_FP8_B128)
+                    fs = reinterpret_cast<const float*>(L.table[e].scales[w.is_down ? 2 : my_tile]) +
+                         (size_t)((w.is_down ? (tile * w.tiles + my_tile) * 16 : tile * 16) >> 7) * ((w.k + 127) >> 7);
+                // fragment rows: lanes 0-15 name the 16 rows of the first piece, 16-31 those of the second
+                const uint32_t frag = smem_u32(ring) + (uint32_t)((my_tile * 16 + (lane & 15)) * w.pitch + (lane >> 4) * 16);
+                const uint8_t* xcol = xs + (size_t)g * xpitch + t4 * 16;
                 for (int c = 0; c < w.n_chunks; ++c, ++n) {
-                    const int st = n % L.n_stages, k0 = c * w.chunk, blocks = min(w.chunk, w.k - k0) / 32;
-                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.full[st], (uint32_t)(n / L.n_stages) & 1u));
-                    const uint8_t* rows = ring + (size_t)st * L.stage_bytes;
-                    for (int b = warp; b < blocks; b += ML_WARPS) {
-                        const int kb = k0 / 32 + b;  // block of 32 columns of the row
-                        uint4 xb[NT];
+                    const int st = n % L.n_stages, kb0 = c * (w.chunk / 32), blocks = min(w.chunk / 32, w.k / 32 - kb0);
+                    if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.full[st], (uint32_t)(n / L.n_stages) & 1u));
+                    const uint32_t rows = frag + (uint32_t)(st * L.stage_bytes);
+                    // Two blocks of 32 columns at a time, their products interleaved (past the end the second repeats the first with
+                    // a scale of zero); lo and hi are the f16 pairs of rows g and g + 8.
+                    auto products = [&](int kb, int kb2, const uint32_t (&lo)[2][4], const uint32_t (&hi)[2][4], const float (&f0)[2],
+                                        const float (&f1)[2]) {
 #pragma unroll
-                        for (int j = 0; j < NT; ++j)
-                            xb[j] = *reinterpret_cast<const uint4*>(xs + (size_t)(j * 8 + g) * xpitch + kb * 64 + t4 * 16);
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            if (i >= w.tiles) break;
-                            const uint8_t* r0 = rows + (i * 16 + g) * w.pitch;
-                            const uint8_t* r1 = r0 + 8 * w.pitch;
-                            uint32_t h0[4], h1[4];
-                            if (FMT == LQ_FMT_FP8_B128) {
-                                const uint2 q0 = *reinterpret_cast<const uint2*>(r0 + b * 32 + t4 * 8);
-                                const uint2 q1 = *reinterpret_cast<const uint2*>(r1 + b * 32 + t4 * 8);
-                                h0[0] = e4m3x2_f16(q0.x), h0[1] = e4m3x2_f16(q0.x >> 16), h0[2] = e4m3x2_f16(q0.y), h0[3] = e4m3x2_f16(q0.y >> 16);
-                                h1[0] = e4m3x2_f16(q1.x), h1[1] = e4m3x2_f16(q1.x >> 16), h1[2] = e4m3x2_f16(q1.y), h1[3] = e4m3x2_f16(q1.y >> 16);
-                            } else {
-                                e2m1x8(*reinterpret_cast<const uint32_t*>(r0 + b * 16 + t4 * 4), h0);
-                                e2m1x8(*reinterpret_cast<const uint32_t*>(r1 + b * 16 + t4 * 4), h1);
-                            }
-                            const uint8_t* s0 = sc + (i * 16 + g) * srow;
-                            const uint8_t* s1 = s0 + 8 * srow;
+                        for (int j = 0; j < NT; ++j) {
+                            if (NT > 1 && j >= cols) break;
+                            const uint8_t* xj = xcol + (size_t)j * 8 * xpitch;
+                            const uint4 x0 = *reinterpret_cast<const uint4*>(xj + kb * 64);
+                            const uint4 x1 = *reinterpret_cast<const uint4*>(xj + kb2 * 64);
                             if (FMT == LQ_FMT_NVFP4) {
-                                const uint32_t f0 = s0[2 * kb + (t4 >> 1)], f1 = s1[2 * kb + (t4 >> 1)];
-                                const uint32_t m0 = e4m3x2_f16(f0 | (f0 << 8)), m1 = e4m3x2_f16(f1 | (f1 << 8));
+                                mma_f16(acc[j], lo[0][0], hi[0][0], lo[0][1], hi[0][1], x0.x, x0.y);
+                                mma_f16(acc2[j], lo[1][0], hi[1][0], lo[1][1], hi[1][1], x1.x, x1.y);
+                                mma_f16(acc[j], lo[0][2], hi[0][2], lo[0][3], hi[0][3], x0.z, x0.w);
+                                mma_f16(acc2[j], lo[1][2], hi[1][2], lo[1][3], hi[1][3], x1.z, x1.w);
+                            } else {
+                                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f}, h[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                mma_f16(d, lo[0][0], hi[0][0], lo[0][1], hi[0][1], x0.x, x0.y);
+                                mma_f16(h, lo[1][0], hi[1][0], lo[1][1], hi[1][1], x1.x, x1.y);
+                                mma_f16(d, lo[0][2], hi[0][2], lo[0][3], hi[0][3], x0.z, x0.w);
+                                mma_f16(h, lo[1][2], hi[1][2], lo[1][3], hi[1][3], x1.z, x1.w);
 #pragma unroll
                                 for (int q = 0; q < 4; ++q) {
-                                    h0[q] = mul_f16x2(h0[q], m0);
-                                    h1[q] = mul_f16x2(h1[q], m1);
-                                }
-#pragma unroll
-                                for (int j = 0; j < NT; ++j) {
-                                    mma_f16(acc[i][j], h0[0], h1[0], h0[1], h1[1], xb[j].x, xb[j].y);
-                                    mma_f16(acc[i][j], h0[2], h1[2], h0[3], h1[3], xb[j].z, xb[j].w);
-                                }
-                            } else {
-                                float f0, f1;
-                                if (FMT == LQ_FMT_MXFP4) {
-                                    f0 = e8m0_to_f32(s0[kb]);
-                                    f1 = e8m0_to_f32(s1[kb]);
-                                } else {
-                                    const int row = w.is_down ? (tile * w.tiles + i) * 16 : tile * 16;
-                                    const float* fs = reinterpret_cast<const float*>(ex.scales[w.is_down ? 2 : i]);
-                                    f0 = f1 = __ldg(fs + (size_t)(row >> 7) * ((w.k + 127) >> 7) + (kb >> 2));
-                                }
-#pragma unroll
-                                for (int j = 0; j < NT; ++j) {
-                                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                    mma_f16(d, h0[0], h1[0], h0[1], h1[1], xb[j].x, xb[j].y);
-                                    mma_f16(d, h0[2], h1[2], h0[3], h1[3], xb[j].z, xb[j].w);
-                                    acc[i][j][0] = fmaf(d[0], f0, acc[i][j][0]);
-                                    acc[i][j][1] = fmaf(d[1], f0, acc[i][j][1]);
-                                    acc[i][j][2] = fmaf(d[2], f1, acc[i][j][2]);
-                                    acc[i][j][3] = fmaf(d[3], f1, acc[i][j][3]);
+                                    acc[j][q] = fmaf(d[q], q < 2 ? f0[0] : f1[0], acc[j][q]);
+                                    acc2[j][q] = fmaf(h[q], q < 2 ? f0[1] : f1[1], acc2[j][q]);
                                 }
                             }
+                        }
+                    };
+                    if (FMT == LQ_FMT_FP8_B128) {
+                        for (int b = kg; b < blocks; b += 2 * kgroups) {
+                            const bool two = b + kgroups < blocks;
+                            const int b2 = two ? b + kgroups : b;
+                            uint32_t r[2][4], lo[2][4], hi[2][4];
+                            ldmatrix4(r[0], rows + b * 32);  // rows g, g + 8 of the first 16 columns; of the other 16
+                            ldmatrix4(r[1], rows + b2 * 32);
+                            const float f = __ldg(fs + ((kb0 + b) >> 2)), f2 = two ? __ldg(fs + ((kb0 + b2) >> 2)) : 0.0f;
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                lo[q][0] = e4m3x2_f16(r[q][0]), lo[q][1] = e4m3x2_f16(r[q][0] >> 16);
+                                lo[q][2] = e4m3x2_f16(r[q][2]), lo[q][3] = e4m3x2_f16(r[q][2] >> 16);
+                                hi[q][0] = e4m3x2_f16(r[q][1]), hi[q][1] = e4m3x2_f16(r[q][1] >> 16);
+                                hi[q][2] = e4m3x2_f16(r[q][3]), hi[q][3] = e4m3x2_f16(r[q][3] >> 16);
+                            }
+                            const float ff[2] = {f, f2};
+                            products(kb0 + b, kb0 + b2, lo, hi, ff, ff);
+                        }
+                    } else {
+                        for (int b = 2 * kg; b < blocks; b += 2 * kgroups) {
+                            const bool two = b + 1 < blocks;
+                            const int kb = kb0 + b, kb2 = two ? kb + 1 : kb;
+                            uint32_t r[4], lo[2][4], hi[2][4];
+                            ldmatrix4(r, rows + b * 16);  // rows g, g + 8 of block b; of block b + 1 (past the end: any codes)
+                            float f0[2] = {0.0f, 0.0f}, f1[2] = {0.0f, 0.0f};
+                            if (FMT == LQ_FMT_MXFP4) {
+                                // 2^(byte - 127), 0 for 0 (e8m0_to_f32; a NaN scale was refused when the layer was made)
+                                f0[0] = __uint_as_float((uint32_t)s0[kb] << 23);
+                                f1[0] = __uint_as_float((uint32_t)s1[kb] << 23);
+                                f0[1] = two ? __uint_as_float((uint32_t)s0[kb2] << 23) : 0.0f;
+                                f1[1] = two ? __uint_as_float((uint32_t)s1[kb2] << 23) : 0.0f;
+                            }
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                e2m1x8(r[2 * q], lo[q]);
+                                e2m1x8(r[2 * q + 1], hi[q]);
+                                if (FMT == LQ_FMT_NVFP4) {
+                                    const int k2 = 2 * (q ? kb2 : kb) + (t4 >> 1);
+                                    const uint32_t u0 = q && !two ? 0u : s0[k2], u1 = q && !two ? 0u : s1[k2];
+                                    const uint32_t m0 = e4m3x2_f16(u0 | (u0 << 8)), m1 = e4m3x2_f16(u1 | (u1 << 8));
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        lo[q][i] = mul_f16x2(lo[q][i], m0);
+                                        hi[q][i] = mul_f16x2(hi[q][i], m1);
+                                    }
+                                }
+                            }
+                            products(kb, kb2, lo, hi, f0, f1);
                         }
                     }
                     __syncwarp();
-                    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&sh.empty[st])) : "memory");
+                    if (lane == 0) ml_arrive(&sh.empty[st]);
                 }
-                if (FMT != LQ_FMT_FP8_B128 && lane == 0)
-                    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&sh.sempty[un & 1])) : "memory");
-                // the warps' parts, in warp order
-                float* mine = red + ((size_t)(un & 1) * ML_WARPS + warp) * RED;
+                if (un >= ML_FINISH && ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.rempty[un % ML_FINISH], (uint32_t)(un / ML_FINISH - 1) & 1u));
+                float* mine = red + ((size_t)(un % ML_FINISH) * ML_WARPS + warp) * RED;
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        float* q = mine + (i * NT * 8 + j * 8 + 2 * t4) * ML_RED_COL + g;
-                        q[0] = acc[i][j][0];
-                        q[ML_RED_COL] = acc[i][j][1];
-                        q[8] = acc[i][j][2];
-                        q[ML_RED_COL + 8] = acc[i][j][3];
-                    }
-                consumers_sync();
-                const float* all = red + (size_t)(un & 1) * ML_WARPS * RED;
-                auto sum = [&](int i, int tok, int row, float scale) {
-                    float s = 0.0f;
-                    for (int q = 0; q < ML_WARPS; ++q)
-#pragma unroll
-                        for (int m = 0; m < TERMS; ++m) s += all[(size_t)q * RED + (i * NT * 8 + tok * TERMS + m) * ML_RED_COL + row];
-                    return s * scale;
-                };
-                if (!w.is_down) {
-                    const int row = tid & 15, tok = tid >> 4;
-                    if (tok < cnt) {
-                        const float un_x = sh.unscale[tok];
-                        const float gate = sum(0, tok, row, un_x) * ex.ts[0], up = sum(1, tok, row, un_x) * ex.ts[1];
-                        L.act[(size_t)sh.gpair[tok] * L.inter + tile * 16 + row] = gate / (1.0f + expf(-gate)) * up;
-                    }
-                } else {
-                    for (int i = 0; i < w.tiles; ++i) {
-                        const int row = tid & 15, tok = tid >> 4;
-                        // the routing weight goes into the power of two, so that only the weighted output has to be in range
-                        if (tok < cnt)
-                            L.pair_out[(size_t)sh.gpair[tok] * L.hidden + (tile * w.tiles + i) * 16 + row] =
-                                sum(i, tok, row, sh.unscale[tok] * sh.w[sh.gpair[tok]]) * ex.ts[2];
-                    }
+                for (int j = 0; j < NT; ++j) {
+                    if (NT > 1 && j >= cols) break;
+                    const int col = j * 8 + 2 * t4;
+                    mine[red_at(col, g)] = acc[j][0] + acc2[j][0];
+                    mine[red_at(col + 1, g)] = acc[j][1] + acc2[j][1];
+                    mine[red_at(col, g + 8)] = acc[j][2] + acc2[j][2];
+                    mine[red_at(col + 1, g + 8)] = acc[j][3] + acc2[j][3];
                 }
+                __syncwarp();
+                if (lane == 0) ml_arrive(&sh.rfull[un % ML_FINISH]);
             }
-            consumers_sync();
-            if (tid == 0 && !grid_arrive_and_wait(L.barrier, gridDim.x)) sh.failed = 1;
-            consumers_sync();
         }
         if (!ok && lane == 0) sh.failed = 1;
-        // ---- combine ----
-        const long long n_out = (long long)T * L.hidden;
-        for (long long i = (long long)blockIdx.x * ML_CONSUMERS + tid; i < n_out; i += (long long)gridDim.x * ML_CONSUMERS) {
-            const int t = (int)(i / L.hidden), h = (int)(i - (long long)t * L.hidden);
-            float s = 0.0f;
-            for (int j = 0; j < K; ++j) s += __ldcg(L.pair_out + (size_t)(t * K + j) * L.hidden + h);
-            if (L.type == LQ_T_F32) static_cast<float*>(L.out)[i] = s;
-            else if (L.type == LQ_T_BF16) static_cast<__nv_bfloat16*>(L.out)[i] = __float2bfloat16_rn(s);
-            else static_cast<__half*>(L.out)[i] = __float2half_rn(s);
-        }
     }
     __syncthreads();
-    if (tid == 0 && sh.failed) set_err(L.err, DEV_ERR_TMA_TIMEOUT);
+    if (tid == 0) {
+        if (sh.failed) set_err(L.err, DEV_ERR_TMA_TIMEOUT);
+        __threadfence();
+        sh.failed = add_release(L.exits, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (sh.failed) {  // the last CTA: nobody waits any more, the words are zeroed for the next launch
+        for (int i = tid; i < MOE_LAYER_SYNC_WORDS; i += ML_THREADS) L.exits[i] = 0;
+    }
 }
 
-template <int FMT, int NT, int TERMS>
-size_t fixed_smem(int hidden, int inter) {
-    const size_t red = 2 * ML_WARPS * (2 * NT * 8 * ML_RED_COL) * 4;
-    const size_t sb = 2 * (size_t)std::max(row_scale_bytes<FMT>(hidden), row_scale_bytes<FMT>(inter)) * 32;
-    return (sizeof(MlSmem) + 127) / 128 * 128 + red + (size_t)NT * 8 * std::max(act_pitch(hidden), act_pitch(inter)) + sb;
+// Shared memory beside the ring and the scales, a unit's scales, a stage.
+size_t fixed_smem(int nt, int hidden, int inter) {
+    return 128 + (sizeof(MlSmem) + 127) / 128 * 128 + ML_FINISH * (size_t)ML_WARPS * nt * 8 * 16 * 4 +
+           (size_t)nt * 8 * std::max(act_pitch(hidden), act_pitch(inter));
+}
+template <int FMT>
+int stage_size(int hidden, int inter) {
+    return 32 * std::max(code_bytes<FMT>(chunk_cols<FMT>(hidden)), code_bytes<FMT>(chunk_cols<FMT>(inter)));
+}
+// The most stages that fit, and a phase's slots for scales: between a unit's first stage and the stage it replaces lie at
+// most n_stages / chunks of its units.
+template <int FMT>
+int plan_ring(int nt, int hidden, int inter, int (&slots)[2]) {
+    auto chunks = [](int k) { return (k + chunk_cols<FMT>(k) - 1) / chunk_cols<FMT>(k); };
+    for (int n = ML_MAX_STAGES; n >= 2; --n) {
+        slots[0] = (n + chunks(hidden) - 1) / chunks(hidden) + 1;
+        slots[1] = (n + chunks(inter) - 1) / chunks(inter) + 1;
+        const size_t scales = 32 * ((size_t)slots[0] * row_scale_bytes<FMT>(hidden) + (size_t)slots[1] * row_scale_bytes<FMT>(inter));
+        if (fixed_smem(nt, hidden, inter) + scales + (size_t)n * stage_size<FMT>(hidden, inter) <= 227 * 1024) return n;
+    }
+    return 0;
 }
 
-template <int FMT, int NT, int TERMS>
+template <int FMT, int NT>
 cudaError_t launch_layer(MoeLayer L, int sm_count, cudaStream_t st) {
-    const size_t most = 227 * 1024, fixed = fixed_smem<FMT, NT, TERMS>(L.hidden, L.inter);
-    L.stage_bytes = 32 * std::max(stage_pitch<FMT>(chunk_cols<FMT>(L.hidden)), stage_pitch<FMT>(chunk_cols<FMT>(L.inter)));
-    if (fixed + 2 * (size_t)L.stage_bytes > most) return cudaErrorInvalidConfiguration;
-    L.n_stages = (int)std::min<size_t>(ML_MAX_STAGES, (most - fixed) / L.stage_bytes);
-    const void* fn = (const void*)moe_layer_kernel<FMT, NT, TERMS>;
-    cudaError_t e = set_max_dyn_smem(fn, (int)most);
+    L.n_stages = plan_ring<FMT>(NT, L.hidden, L.inter, L.scale_slots);
+    if (L.n_stages == 0) return cudaErrorInvalidConfiguration;
+    L.stage_bytes = stage_size<FMT>(L.hidden, L.inter);
+    const size_t smem = fixed_smem(NT, L.hidden, L.inter) + 32 * ((size_t)L.scale_slots[0] * row_scale_bytes<FMT>(L.hidden) + (size_t)L.scale_slots[1] * row_scale_bytes<FMT>(L.inter)) + (size_t)L.n_stages * L.stage_bytes;
+    const void* fn = (const void*)moe_layer_kernel<FMT, NT>;
+    cudaError_t e = set_max_dyn_smem(fn, 227 * 1024);
     if (e != cudaSuccess) return e;
     void* args[] = {&L};
-    return cudaLaunchCooperativeKernel(fn, dim3(sm_count), dim3(ML_THREADS), args, fixed + (size_t)L.n_stages * L.stage_bytes, st);
+    return cudaLaunchCooperativeKernel(fn, dim3(sm_count), dim3(ML_THREADS), args, smem, st);
 }
 
 template <int FMT>
-cudaError_t launch_fmt(const MoeLayer& L, int sm_count, cudaStream_t st) {
-    // Two column tiles (16 columns) when the tokens fill more than one and the activations leave room for a ring.
-    const int terms = L.type == LQ_T_BF16 ? 1 : 2;
-    const bool wide = L.tokens * terms > 8 &&
-                      (terms == 1 ? fixed_smem<FMT, 2, 1>(L.hidden, L.inter) : fixed_smem<FMT, 2, 2>(L.hidden, L.inter)) <= 150 * 1024;
-    if (terms == 1) return wide ? launch_layer<FMT, 2, 1>(L, sm_count, st) : launch_layer<FMT, 1, 1>(L, sm_count, st);
-    return wide ? launch_layer<FMT, 2, 2>(L, sm_count, st) : launch_layer<FMT, 1, 2>(L, sm_count, st);
+cudaError_t launch_fmt(MoeLayer L, int sm_count, cudaStream_t st) {
+    L.terms = L.type == LQ_T_BF16 ? 1 : 2;
+    // Two tiles of columns when an expert's tokens are likely to fill more than one (an expert with more tokens than a
+    // group holds is read once per group) and shared memory takes them beside a ring that covers the memory's latency.
+    int nt = L.tokens * L.top_e * L.terms > 5 * L.experts && L.tokens * L.terms > 8 ? 2 : 1;
+    int slots[2];
+    if (nt > 1 && (size_t)plan_ring<FMT>(nt, L.hidden, L.inter, slots) * stage_size<FMT>(L.hidden, L.inter) < 48 * 1024) nt = 1;
+    return nt == 1 ? launch_layer<FMT, 1>(L, sm_count, st) : launch_layer<FMT, 2>(L, sm_count, st);
 }
 
 }  // namespace
 
 template <int FMT>
 static bool fits(int hidden, int inter) {
-    const int pitch = std::max(stage_pitch<FMT>(chunk_cols<FMT>(hidden)), stage_pitch<FMT>(chunk_cols<FMT>(inter)));
-    return fixed_smem<FMT, 1, 2>(hidden, inter) + 2 * 32 * (size_t)pitch <= 227 * 1024;
+    int slots[2];
+    return plan_ring<FMT>(1, hidden, inter, slots) > 0;
 }
 bool moe_layer_supported(int fmt, int hidden, int inter) {
     if (hidden <= 0 || inter <= 0 || hidden % 32 || inter % 32 || hidden > 8192 || inter > 8192) return false;
+    if (fmt == LQ_FMT_NVFP4 && (hidden > 6144 || inter > 6144)) return false;
     switch (fmt) {
         case LQ_FMT_MXFP4: return fits<LQ_FMT_MXFP4>(hidden, inter);
         case LQ_FMT_NVFP4: return fits<LQ_FMT_NVFP4>(hidden, inter);
         case LQ_FMT_FP8_B128: return fits<LQ_FMT_FP8_B128>(hidden, inter);
     }
     return false;
+}
+
+// Whether any e8m0 scale of the layer is 255, a NaN: block (expert, matrix) looks through that matrix's scales.
+__global__ void moe_nan_scale_kernel(const MoeExpert* table, int hidden, int inter, int* found) {
+    const size_t n = (size_t)hidden * inter / 32 / 16;  // (rows and columns are multiples of 32)
+    const uint4* s = reinterpret_cast<const uint4*>(table[blockIdx.x].scales[blockIdx.y]);
+    unsigned bad = 0;
+    for (size_t i = threadIdx.x; i < n; i += blockDim.x) {
+        const uint4 v = s[i];
+        bad |= __vcmpeq4(v.x, 0xffffffffu) | __vcmpeq4(v.y, 0xffffffffu) | __vcmpeq4(v.z, 0xffffffffu) | __vcmpeq4(v.w, 0xffffffffu);
+    }
+    if (bad) *found = 1;
+}
+cudaError_t launch_moe_nan_scale(const MoeExpert* table, int experts, int hidden, int inter, int* found, cudaStream_t st) {
+    moe_nan_scale_kernel<<<dim3(experts, 3), 512, 0, st>>>(table, hidden, inter, found);
+    return cudaGetLastError();
+}
+
+template <int FMT>
+static cudaError_t encode_maps(MoeExpert* ex, int hidden, int inter) {
+    for (int i = 0; i < 3; ++i) {
+        const size_t rows = i == 2 ? hidden : inter, bytes = (size_t)code_bytes<FMT>(i == 2 ? inter : hidden);
+        const cudaError_t e = encode_tile_map(&ex->map[i], CU_TENSOR_MAP_DATA_TYPE_UINT32, ex->codes[i], rows, bytes / 4, bytes, 16,
+                                              code_bytes<FMT>(chunk_cols<FMT>(i == 2 ? inter : hidden)) / 4, CU_TENSOR_MAP_SWIZZLE_NONE);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+cudaError_t moe_encode_maps(int fmt, MoeExpert* ex, int hidden, int inter) {
+    switch (fmt) {
+        case LQ_FMT_MXFP4: return encode_maps<LQ_FMT_MXFP4>(ex, hidden, inter);
+        case LQ_FMT_NVFP4: return encode_maps<LQ_FMT_NVFP4>(ex, hidden, inter);
+        case LQ_FMT_FP8_B128: return encode_maps<LQ_FMT_FP8_B128>(ex, hidden, inter);
+    }
+    return cudaErrorInvalidValue;
 }
 
 cudaError_t launch_moe_layer(int fmt, const MoeLayer& L, int sm_count, cudaStream_t st) {

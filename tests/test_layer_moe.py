@@ -273,6 +273,11 @@ def test_moe_refusals(be):
     assert be.moe_create(g, n.mats[1], d, r, 0, 0, 1) is None             # mixed formats
     q8 = larql_b200.DeviceMatrix(larql_b200.FMT_Q8_0, 96, 64, r, 96 * 68)
     assert be.moe_create([q8], [q8], [q8], r, 0, 0, 1) is None
+    nan = a.keep[1].clone()
+    nan[95, 1] = 255
+    torch.cuda.synchronize()
+    bad = larql_b200.DeviceMatrix(larql_b200.FMT_MXFP4, 96, 64, g[0].data_ptr, g[0].data_len, nan.data_ptr(), nan.numel())
+    assert be.moe_create([g[0], bad], u, d, r, 0, 0, 1) is None           # an e8m0 NaN
     big = larql_b200.DeviceMatrix(larql_b200.FMT_MXFP4, 8224, 32, r & ~15, 8224 * 16, r & ~15, 8224)
     down = larql_b200.DeviceMatrix(larql_b200.FMT_MXFP4, 32, 8224, r & ~15, 8224 * 16, r & ~15, 8224)
     assert be.moe_create([big], [big], [down], r, 0, 0, 1) is None
