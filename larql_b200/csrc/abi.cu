@@ -2466,7 +2466,7 @@ int lq_moe_create(lq_ctx* ctx, const lq_matrix* gates, const lq_matrix* ups, con
     const size_t pairs = h->max_tokens * std::max<size_t>(k, 1);
     const size_t tb = a256(n_experts * sizeof(MoeExpert)), lb = a256(h->max_tokens * n_experts * 4),
                  ab = a256(pairs * (size_t)inter * 4), pb = a256(pairs * (size_t)hidden * 4), fixed = tb + lb + ab + pb;
-    h->sync_bytes = (MOE_LAYER_SYNC_WORDS + h->max_tokens * (size_t)(hidden / 16)) * 4;
+    h->sync_bytes = MOE_LAYER_SYNC_WORDS * 4;
     cudaError_t e = cudaMalloc(&h->raw, fixed + h->sync_bytes);
     if (e == cudaSuccess) e = cudaMemcpyAsync(h->raw, table.data(), n_experts * sizeof(MoeExpert), cudaMemcpyHostToDevice, ctx->stream);
     if (e == cudaSuccess) e = cudaMemsetAsync(h->raw + fixed, 0, h->sync_bytes, ctx->stream);
@@ -2496,10 +2496,10 @@ int lq_moe_create(lq_ctx* ctx, const lq_matrix* gates, const lq_matrix* ups, con
     L.pair_out = (float*)(h->raw + tb + lb + ab);
     L.exits = (unsigned*)(h->raw + fixed);
     L.route_done = L.exits + 1;
-    L.group_done = L.route_done + 1;
+    L.down_done = L.route_done + 1;
+    L.group_done = L.down_done + 1;
     L.x_max = L.group_done + MOE_LAYER_MAX_PAIRS;
     L.act_max = L.x_max + MOE_LAYER_MAX_TOKENS;
-    L.out_done = L.act_max + MOE_LAYER_MAX_PAIRS;
     L.router = router, L.bias = router_bias, L.router_type = router_type;
     L.hidden = (int)hidden, L.inter = (int)inter, L.experts = (int)n_experts, L.top_e = (int)k;
     L.renormalise = renormalise != 0;

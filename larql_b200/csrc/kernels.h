@@ -224,8 +224,8 @@ cudaError_t launch_fp8_matmul(const Fp8Product& p, bool overlap, int sm_count, i
 #define MOE_LAYER_MAX_TOKENS 64
 #define MOE_LAYER_MAX_TOP 32
 #define MOE_LAYER_MAX_PAIRS 1024  // tokens x top_e of a launch
-// exits, route_done, group_done, x_max, act_max; out_done lies behind them
-#define MOE_LAYER_SYNC_WORDS (2 + MOE_LAYER_MAX_PAIRS + MOE_LAYER_MAX_TOKENS + MOE_LAYER_MAX_PAIRS)
+// exits, route_done, down_done, group_done, x_max, act_max
+#define MOE_LAYER_SYNC_WORDS (3 + MOE_LAYER_MAX_PAIRS + MOE_LAYER_MAX_TOKENS + MOE_LAYER_MAX_PAIRS)
 struct MoeExpert {
     CUtensorMap map[3];        // over codes: a stage's columns of 16 rows
     const uint8_t* codes[3];   // gate, up [inter][hidden]; down [hidden][inter]
@@ -243,9 +243,9 @@ struct MoeLayer {
     float* w_out;
     // workspace: [tokens][experts], [pairs][inter], [pairs][hidden]
     float *logits, *act, *pair_out;
-    // counters, zero between launches: CTAs gone, router products done, units done per token group of an expert, results
-    // per token and 16 outputs; bits of the largest |value| per token / pair
-    unsigned *exits, *route_done, *group_done, *x_max, *act_max, *out_done;
+    // counters, zero between launches: CTAs gone, router products done, down units done, gate/up units done per token
+    // group of an expert; bits of the largest |value| per token / pair
+    unsigned *exits, *route_done, *down_done, *group_done, *x_max, *act_max;
     int terms;                       // f16 terms per activation (filled in by the launch)
     int n_stages, stage_bytes, scale_slots[2];  // filled in by the launch
     int* err;

@@ -12,14 +12,13 @@
 //            expert), spread over the grid; then every CTA picks the experts itself;
 //   gate/up  units of 16 features of one expert for one group of its tokens: act = silu(gate) * up, f32, to global;
 //   down     units of 16 or 32 output rows, as soon as the expert's activations are complete (a counter per group, no
-//            grid barrier); whoever brings the last of a token's top_e results for some rows adds them up, in
-//            selection order.
+//            grid barrier); when the last unit of all is done, the tokens' results are added up in selection order.
 // Warps have three jobs.  A producer streams the units' rows through a ring in shared memory (one tile copy per 16
 // rows); it needs only the routing, so it runs ahead from gate/up into down while the activations are still on
 // their way.  16 compute warps multiply, each its part of the contraction, and leave their sums in shared memory.
 // Finishers add the parts up in a fixed order (results do not depend on timing), apply the activation or the
-// routing weight and publish: a publication waits for a fence and an atomic, a microsecond that a unit's
-// multiplication (also a microsecond) must not wait for.
+// routing weight, and publish what they finished of a group when they leave it (a fence and an atomic cost a
+// microsecond, as much as a unit's multiplication).
 //
 // The products run on the tensor cores (mma.sync m16n8k16, f16 x f16 -> f32): weights are the 16 rows of A, tokens the 8
 // columns of B.  The codes of all three formats are exact in f16.  An activation is brought to [2^14, 2^15) by a
@@ -194,15 +193,17 @@ __host__ __device__ constexpr int row_scale_bytes(int cols) {
 }
 // Distance of two columns of the activations: two columns (a phase of a 16-byte load) fall into different banks.
 __host__ __device__ constexpr int act_pitch(int k) { return (2 * k) % 128 == 0 ? 2 * k + 64 : 2 * k; }
-// Columns of the contraction per stage: equal parts of at most 47 blocks of 32 (23 for FP8, and for long rows, whose
-// activations take most of shared memory), an odd number of them.  A
-// stage holds its rows back to back as the tile copy lays them; an odd number of 16-byte pieces per row would put the
-// eight rows of a fragment load into different banks (FP8 rows, 32 bytes a block, keep a two-way conflict).
+// Columns of the contraction per stage: equal parts of at most 46 blocks of 32 (22 for FP8, and for long rows, whose
+// activations take most of shared memory), an even number of them.  A stage holds one block more of every row, back to
+// back as the tile copy lays them: an odd number of 16-byte pieces per row puts the eight rows of a fragment load into
+// different banks (FP8 rows, 32 bytes a block, keep a two-way conflict).
 template <int FMT>
 __host__ __device__ constexpr int chunk_cols(int k) {
-    const int blocks = k / 32, most = FMT == LQ_FMT_FP8_B128 || k > 4096 ? 23 : 47, n = (blocks + most - 1) / most;
-    return (((blocks + n - 1) / n) | 1) * 32;
+    const int blocks = k / 32, most = FMT == LQ_FMT_FP8_B128 || k > 4096 ? 22 : 46, n = (blocks + most - 1) / most;
+    return (((blocks + n - 1) / n + 1) & ~1) * 32;
 }
+template <int FMT>
+__host__ __device__ constexpr int stage_cols(int k) { return chunk_cols<FMT>(k) + 32; }
 
 // One phase's products as the kernel walks them.
 struct Walk {
@@ -222,7 +223,7 @@ __device__ __forceinline__ Walk walk_of(const MoeLayer& L, bool down, int n_grou
     w.k = down ? L.inter : L.hidden;
     w.chunk = chunk_cols<FMT>(w.k);
     w.n_chunks = (w.k + w.chunk - 1) / w.chunk;
-    w.pitch = code_bytes<FMT>(w.chunk);
+    w.pitch = code_bytes<FMT>(stage_cols<FMT>(w.k));
     if (!down) {
         w.tiles = 2;
         w.units_per_group = L.inter / 16;
@@ -429,7 +430,8 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
     if (warp == ML_WARPS) {
         // ---- producer: the rows of both phases' units, in order ----
         bool ok = true;
-        int n = 0, un = 0;  // stages and units so far
+        int n = 0, st = 0;  // stages so far, the ring's next place
+        uint32_t lap = 0;   // parity of the ring's lap (an empty barrier's first wait, for parity 1, passes)
         for (int ph = 0; ph < 2 && ok; ++ph) {
             const Walk w = walk_of<FMT>(L, ph == 1, n_groups, sbuf);
             const int total = n_groups * w.units_per_group;
@@ -438,8 +440,9 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
             int gi = ua / w.units_per_group, tile = ua - gi * w.units_per_group, a = -1;
             const CUtensorMap *m0 = nullptr, *m1 = nullptr;
             const uint8_t *sc0 = nullptr, *sc1 = nullptr;
+            int slot = 0;
             const uint32_t sbytes16 = 16u * row_scale_bytes<FMT>(w.k), code16 = 16u * w.pitch;
-            for (int u = ua; u < ub && ok; ++u, ++un) {
+            for (int u = ua; u < ub && ok; ++u) {
                 if (a < 0 || tile == w.units_per_group) {
                     if (a >= 0) ++gi, tile = 0;
                     a = expert_of(sh, gi, max(a, 0));
@@ -449,8 +452,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                 }
                 const int row0 = (w.is_down ? tile * w.tiles : tile) * 16, row1 = w.is_down ? row0 + 16 : row0;
                 for (int c = 0; c < w.n_chunks; ++c, ++n) {
-                    const int st = n % L.n_stages;
-                    if (n >= L.n_stages) ok = __all_sync(0xffffffffu, ml_wait(&sh.empty[st], (uint32_t)(n / L.n_stages - 1) & 1u));
+                    ok = __all_sync(0xffffffffu, ml_wait(&sh.empty[st], lap ^ 1u));
                     if (!ok) break;
                     if (lane == 0) {  // (columns past the row's end arrive as zeros and count as bytes)
                         const bool with_scales = sbytes16 && c == 0;
@@ -462,14 +464,16 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                         if (with_scales) {
                             // the unit's scales come with its first stage.  Their slot is free: the stage this one replaces was
                             // consumed, and scale_slots units do not fit between the two
-                            uint8_t* sd = w.scales + (un % w.slots) * 2 * sbytes16;
+                            uint8_t* sd = w.scales + slot * 2 * sbytes16;
                             tma_bulk_g2s(sd, sc0 + (size_t)(row0 >> 4) * sbytes16, sbytes16, &sh.full[st]);
                             if (w.tiles == 2) tma_bulk_g2s(sd + sbytes16, sc1 + (size_t)(row1 >> 4) * sbytes16, sbytes16, &sh.full[st]);
                         }
                     }
                     __syncwarp();
+                    if (++st == L.n_stages) st = 0, lap ^= 1u;
                 }
                 ++tile;
+                if (++slot == w.slots) slot = 0;
             }
         }
         if (!ok) {  // the copies in flight have to land before the block's shared memory goes away
@@ -481,7 +485,8 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
         const bool computes = warp < ML_WARPS;
         const int g = lane >> 2, t4 = lane & 3;
         bool ok = true;  // a wait that ran out is not waited for again; barriers, arrivals and counters are kept
-        int n = 0, un = 0;
+        int st = 0, rb = 0;               // next place of the ring, buffer of the unit's sums
+        uint32_t lap = 0, rlap = 0;       // parities of their laps
         for (int ph = 0; ph < 2; ++ph) {
             const Walk w = walk_of<FMT>(L, ph == 1, n_groups, sbuf);
             const int xpitch = act_pitch(w.k), srow = row_scale_bytes<FMT>(w.k);
@@ -492,30 +497,42 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
             if (!computes) {
                 // ---- finishers: every ML_FINISH-th unit, each with a buffer of its own (it sees all of its phases) ----
                 const int buf = warp - ML_WARPS - 1;
-                for (int u = ua; u < ub; ++u, ++un, ++tile) {
+                unsigned units = 0, top = 0;  // of this group, not yet published: units, lane i's pair's largest |value|
+                int pair = 0;
+                auto publish = [&]() {
+                    if (units == 0) return;
+                    if (!w.is_down && top) atomicMax(L.act_max + pair, top);
+                    __threadfence();
+                    __syncwarp();
+                    if (lane == 0) add_release(w.is_down ? L.down_done : L.group_done + gi, units);
+                    units = top = 0;
+                };
+                for (int u = ua; u < ub; ++u, ++tile) {
                     if (tile == w.units_per_group) {
+                        if (!w.is_down) publish();
                         ++gi, tile = 0;
                         a = expert_of(sh, gi, a);
                     }
-                    if (un % ML_FINISH != buf) continue;
+                    const bool mine = rb == buf;
+                    const uint32_t parity = rlap;
+                    if (++rb == ML_FINISH) rb = 0, rlap ^= 1u;
+                    if (!mine) continue;
+                    ++units;
                     const MoeExpert& ex = L.table[sh.active[a]];
                     const int row = lane & 15, half = lane >> 4;
                     const float ts = ex.ts[w.is_down ? 2 : half];
-                    if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.rfull[buf], (uint32_t)(un / ML_FINISH) & 1u));
+                    if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.rfull[buf], parity));
                     const int cnt = sh.cnt;
                     // lane i keeps what belongs to token i of the group
-                    int pair = 0, t = 0;
                     float scale = 0.0f;
                     if (lane < cnt) {
                         pair = sh.gpair[lane];
-                        t = sh.gtok[lane];
                         // (the routing weight goes into the power of two, so that only the weighted output has to be in range)
                         scale = sh.unscale[lane] * (w.is_down ? sh.w[pair] : 1.0f);
                     }
                     const float* all = red + (size_t)buf * ML_WARPS * RED;
                     // two tiles: a half of the lanes each; one tile: the halves take half of the warps' parts each
                     const int q0 = w.tiles == 2 ? half : half * (ML_WARPS / 2), qs = w.tiles == 2 ? 2 : 1;
-                    float top = 0.0f;
                     for (int i = 0; i < cnt; ++i) {
                         float v = 0.0f;
 #pragma unroll
@@ -532,47 +549,21 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                             if (half == 0) __stcg(L.act + at * L.inter + tile * 16 + row, act);
                             // the pair's largest |value| (a NaN's bits are above every number's)
                             const unsigned m = __reduce_max_sync(0xffffffffu, half == 0 ? __float_as_uint(act) & 0x7fffffffu : 0u);
-                            if (lane == i) top = __uint_as_float(m);
+                            if (lane == i) top = max(top, m);
                         } else if (w.tiles == 2 || half == 0) {
                             __stcg(L.pair_out + at * L.hidden + (tile * w.tiles + (w.tiles == 2 ? half : 0)) * 16 + row, v);
                         }
                     }
                     __syncwarp();
                     if (lane == 0) ml_arrive(&sh.rempty[buf]);
-                    if (!w.is_down) {
-                        if (lane < cnt) atomicMax(L.act_max + pair, __float_as_uint(top));
-                        __threadfence();
-                        __syncwarp();
-                        if (lane == 0) add_release(L.group_done + gi, 1u);
-                        continue;
-                    }
-                    __threadfence();
-                    __syncwarp();
-                    bool last = false;
-                    unsigned* word = L.out_done + (size_t)t * (L.hidden / 16) + tile * w.tiles;
-                    if (lane < cnt) last = add_release(word, 1u) == (unsigned)K - 1;
-                    unsigned done = __ballot_sync(0xffffffffu, last);
-                    if (last) *word = 0;  // ready for the next launch
-                    if (done) __threadfence();
-                    for (; done; done &= done - 1) {
-                        const int tt = __shfl_sync(0xffffffffu, t, __ffs(done) - 1);
-                        if (w.tiles == 1 && half) continue;
-                        const int h = (tile * w.tiles + half) * 16 + row;
-                        float s = 0.0f;
-                        for (int j = 0; j < K; ++j) s += __ldcg(L.pair_out + (size_t)(tt * K + j) * L.hidden + h);
-                        const size_t at = (size_t)tt * L.hidden + h;
-                        if (L.type == LQ_T_F32) static_cast<float*>(L.out)[at] = s;
-                        else if (L.type == LQ_T_BF16) static_cast<__nv_bfloat16*>(L.out)[at] = __float2bfloat16_rn(s);
-                        else static_cast<__half*>(L.out)[at] = __float2half_rn(s);
-                    }
-                    __syncwarp();
                 }
+                publish();
                 continue;
             }
             // compute warps: one 16-row tile each, every kgroups-th pair of blocks of the contraction
             const int my_tile = w.tiles == 2 ? (warp & 1) : 0, kg = w.tiles == 2 ? warp >> 1 : warp, kgroups = ML_WARPS / w.tiles;
-            int cur = -1, cols = 0;
-            for (int u = ua; u < ub; ++u, ++un, ++tile) {
+            int cur = -1, cols = 0, slot = 0;
+            for (int u = ua; u < ub; ++u, ++tile) {
                 if (tile == w.units_per_group) {
                     ++gi, tile = 0;
                     a = expert_of(sh, gi, a);
@@ -586,8 +577,8 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     const int cnt = min(TG, __popcll(m0) - first);
                     cols = (cnt * terms + 7) / 8;
                     // the finishers are done with the previous group's units, the compute warps with its activations
-                    for (int v = max(0, un - ML_FINISH); v < un; ++v)
-                        if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.rempty[v % ML_FINISH], (uint32_t)(v / ML_FINISH) & 1u));
+                    for (int v = 0; v < ML_FINISH; ++v)
+                        if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.rempty[v], v < rb ? rlap : rlap ^ 1u));
                     consumers_sync();
                     if (tid < cnt) {
                         unsigned long long m = m0;
@@ -653,7 +644,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) acc[j][q] = acc2[j][q] = 0.0f;
-                const uint8_t* s0 = w.scales + (un % w.slots) * 32 * srow + (my_tile * 16 + g) * srow;
+                const uint8_t* s0 = w.scales + slot * 32 * srow + (my_tile * 16 + g) * srow;
                 const uint8_t* s1 = s0 + 8 * srow;
                 const float* fs = nullptr;
                 if (FMT == LQ_FMT_FP8_B128)
@@ -662,9 +653,10 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                 // fragment rows: lanes 0-15 name the 16 rows of the first piece, 16-31 those of the second
                 const uint32_t frag = smem_u32(ring) + (uint32_t)((my_tile * 16 + (lane & 15)) * w.pitch + (lane >> 4) * 16);
                 const uint8_t* xcol = xs + (size_t)g * xpitch + t4 * 16;
-                for (int c = 0; c < w.n_chunks; ++c, ++n) {
-                    const int st = n % L.n_stages, kb0 = c * (w.chunk / 32), blocks = min(w.chunk / 32, w.k / 32 - kb0);
-                    if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.full[st], (uint32_t)(n / L.n_stages) & 1u));
+                if (++slot == w.slots) slot = 0;
+                for (int c = 0; c < w.n_chunks; ++c) {
+                    const int kb0 = c * (w.chunk / 32), blocks = min(w.chunk / 32, w.k / 32 - kb0);
+                    if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.full[st], lap));
                     const uint32_t rows = frag + (uint32_t)(st * L.stage_bytes);
                     // Two blocks of 32 columns at a time, their products interleaved (past the end the second repeats the first with
                     // a scale of zero); lo and hi are the f16 pairs of rows g and g + 8.
@@ -722,10 +714,20 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                             float f0[2] = {0.0f, 0.0f}, f1[2] = {0.0f, 0.0f};
                             if (FMT == LQ_FMT_MXFP4) {
                                 // 2^(byte - 127), 0 for 0 (e8m0_to_f32; a NaN scale was refused when the layer was made)
-                                f0[0] = __uint_as_float((uint32_t)s0[kb] << 23);
-                                f1[0] = __uint_as_float((uint32_t)s1[kb] << 23);
-                                f0[1] = two ? __uint_as_float((uint32_t)s0[kb2] << 23) : 0.0f;
-                                f1[1] = two ? __uint_as_float((uint32_t)s1[kb2] << 23) : 0.0f;
+                                // (kb is even; past the end of a row of odd length the second byte is another scale, dropped)
+                                uint32_t u0, u1;
+                                const uint32_t keep = two ? 0x7f800000u : 0u;
+                                if (srow & 1) {
+                                    u0 = s0[kb] | (uint32_t)s0[kb + 1] << 8;
+                                    u1 = s1[kb] | (uint32_t)s1[kb + 1] << 8;
+                                } else {
+                                    u0 = *reinterpret_cast<const uint16_t*>(s0 + kb);
+                                    u1 = *reinterpret_cast<const uint16_t*>(s1 + kb);
+                                }
+                                f0[0] = __uint_as_float((u0 << 23) & 0x7f800000u);
+                                f1[0] = __uint_as_float((u1 << 23) & 0x7f800000u);
+                                f0[1] = __uint_as_float((u0 << 15) & keep);
+                                f1[1] = __uint_as_float((u1 << 15) & keep);
                             }
 #pragma unroll
                             for (int q = 0; q < 2; ++q) {
@@ -747,9 +749,10 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     }
                     __syncwarp();
                     if (lane == 0) ml_arrive(&sh.empty[st]);
+                    if (++st == L.n_stages) st = 0, lap ^= 1u;
                 }
-                if (un >= ML_FINISH && ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.rempty[un % ML_FINISH], (uint32_t)(un / ML_FINISH - 1) & 1u));
-                float* mine = red + ((size_t)(un % ML_FINISH) * ML_WARPS + warp) * RED;
+                if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.rempty[rb], rlap ^ 1u));
+                float* mine = red + (rb * ML_WARPS + warp) * RED;
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     if (NT > 1 && j >= cols) break;
@@ -760,10 +763,32 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     mine[red_at(col + 1, g + 8)] = acc[j][3] + acc2[j][3];
                 }
                 __syncwarp();
-                if (lane == 0) ml_arrive(&sh.rfull[un % ML_FINISH]);
+                if (lane == 0) ml_arrive(&sh.rfull[rb]);
+                if (++rb == ML_FINISH) rb = 0, rlap ^= 1u;
             }
         }
         if (!ok && lane == 0) sh.failed = 1;
+    }
+    // ---- the tokens' results, when every unit of every CTA is there ----
+    const int n_units = n_groups * walk_of<FMT>(L, true, n_groups, sbuf).units_per_group;
+    if (tid == 0 && !wait_count(L.down_done, (unsigned)n_units)) sh.failed = 1;
+    __syncthreads();
+    for (int i = blockIdx.x * ML_THREADS + tid; i < T * (L.hidden / 4); i += gridDim.x * ML_THREADS) {
+        const int t = i / (L.hidden / 4), h = (i - t * (L.hidden / 4)) * 4;
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int j = 0; j < K; ++j) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(L.pair_out + (size_t)(t * K + j) * L.hidden + h));
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+        const size_t at = (size_t)t * L.hidden + h;
+        const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (L.type == LQ_T_F32) static_cast<float*>(L.out)[at + q] = v[q];
+            else if (L.type == LQ_T_BF16) static_cast<__nv_bfloat16*>(L.out)[at + q] = __float2bfloat16_rn(v[q]);
+            else static_cast<__half*>(L.out)[at + q] = __float2half_rn(v[q]);
+        }
     }
     __syncthreads();
     if (tid == 0) {
@@ -784,7 +809,7 @@ size_t fixed_smem(int nt, int hidden, int inter) {
 }
 template <int FMT>
 int stage_size(int hidden, int inter) {
-    return 32 * std::max(code_bytes<FMT>(chunk_cols<FMT>(hidden)), code_bytes<FMT>(chunk_cols<FMT>(inter)));
+    return 32 * std::max(code_bytes<FMT>(stage_cols<FMT>(hidden)), code_bytes<FMT>(stage_cols<FMT>(inter)));
 }
 // The most stages that fit, and a phase's slots for scales: between a unit's first stage and the stage it replaces lie at
 // most n_stages / chunks of its units.
@@ -863,7 +888,7 @@ static cudaError_t encode_maps(MoeExpert* ex, int hidden, int inter) {
     for (int i = 0; i < 3; ++i) {
         const size_t rows = i == 2 ? hidden : inter, bytes = (size_t)code_bytes<FMT>(i == 2 ? inter : hidden);
         const cudaError_t e = encode_tile_map(&ex->map[i], CU_TENSOR_MAP_DATA_TYPE_UINT32, ex->codes[i], rows, bytes / 4, bytes, 16,
-                                              code_bytes<FMT>(chunk_cols<FMT>(i == 2 ? inter : hidden)) / 4, CU_TENSOR_MAP_SWIZZLE_NONE);
+                                              code_bytes<FMT>(stage_cols<FMT>(i == 2 ? inter : hidden)) / 4, CU_TENSOR_MAP_SWIZZLE_NONE);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
