@@ -141,8 +141,13 @@ __device__ __forceinline__ void ml_arrive(uint64_t* bar) {
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 // Four 8 x 16-byte pieces of shared memory, lane l naming row l % 8 of piece l / 8: a lane gets word l % 4 of row l / 4.
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -150,6 +155,17 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "r"(addr)
                  : "memory");
+}
+// Loads by shared-memory address (ordered against the waits, like them volatile).
+__device__ __forceinline__ uint32_t lds_u8(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint4 lds_128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
 }
 // Eight e2m1 codes (low nibble first) -> four f16 pairs.
 __device__ __forceinline__ void e2m1x8(uint32_t w, uint32_t (&h)[4]) {
@@ -302,11 +318,11 @@ __device__ void route_token(const MoeLayer& L, MlSmem& sh, int t, int lane) {
 template <int FMT, int NT>
 __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_constant__ MoeLayer L) {
     extern __shared__ __align__(128) uint8_t smem[];
-    constexpr int RED = NT * 8 * 16;  // floats of a warp's partial sums
+    constexpr int RED = NT * 8 * 16;  // floats of a warp's partial sums of 16 rows
     MlSmem& sh = *reinterpret_cast<MlSmem*>(smem);
     uint8_t* p = smem + (sizeof(MlSmem) + 127) / 128 * 128;
-    float* red = reinterpret_cast<float*>(p);                 // [ML_FINISH][ML_WARPS][RED]
-    p += ML_FINISH * ML_WARPS * RED * 4;
+    float* red = reinterpret_cast<float*>(p);                 // [finish][ML_WARPS][2 tiles][RED]
+    p += L.finish * ML_WARPS * 2 * RED * 4;
     uint8_t* xs = p;                                          // [NT * 8] columns of f16
     p += (size_t)NT * 8 * max(act_pitch(L.hidden), act_pitch(L.inter));
     uint8_t* sbuf = p;                                        // scales of the units' rows, [scale_slots] per phase
@@ -341,7 +357,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
         const int rounds = (items + (int)gridDim.x * per_cta - 1) / ((int)gridDim.x * per_cta);
         for (int r = 0; r < rounds; ++r) {
             const int it = (r * per_cta + sub) * gridDim.x + blockIdx.x;
-            const bool on = it < items;
+            const bool on = it < items && sub < per_cta;  // (warps beyond the last whole item have none)
             const int t = on ? it / E : 0, e = on ? it - t * E : 0;
             float2 s = make_float2(0.0f, 0.0f);
             float m = 0.0f;
@@ -495,7 +511,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
             if (ua >= ub) continue;
             int gi = ua / w.units_per_group, tile = ua - gi * w.units_per_group, a = expert_of(sh, gi, 0);
             if (!computes) {
-                // ---- finishers: every ML_FINISH-th unit, each with a buffer of its own (it sees all of its phases) ----
+                // ---- finishers: every finish-th unit, each with a buffer of its own (it sees all of its phases) ----
                 const int buf = warp - ML_WARPS - 1;
                 unsigned units = 0, top = 0;  // of this group, not yet published: units, lane i's pair's largest |value|
                 int pair = 0;
@@ -515,7 +531,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     }
                     const bool mine = rb == buf;
                     const uint32_t parity = rlap;
-                    if (++rb == ML_FINISH) rb = 0, rlap ^= 1u;
+                    if (++rb == L.finish) rb = 0, rlap ^= 1u;
                     if (!mine) continue;
                     ++units;
                     const MoeExpert& ex = L.table[sh.active[a]];
@@ -530,16 +546,16 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                         // (the routing weight goes into the power of two, so that only the weighted output has to be in range)
                         scale = sh.unscale[lane] * (w.is_down ? sh.w[pair] : 1.0f);
                     }
-                    const float* all = red + (size_t)buf * ML_WARPS * RED;
-                    // two tiles: a half of the lanes each; one tile: the halves take half of the warps' parts each
-                    const int q0 = w.tiles == 2 ? half : half * (ML_WARPS / 2), qs = w.tiles == 2 ? 2 : 1;
+                    const float* all = red + buf * ML_WARPS * 2 * RED;
+                    // two tiles: a half of the lanes each; one tile: the halves take half of the warps' parts each (an even
+                    // and an odd part at a time, in the order of the warps)
+                    const float* part = all + (w.tiles == 2 ? half * RED : half * (ML_WARPS / 2) * 2 * RED);
+                    const int parts = w.tiles == 2 ? ML_WARPS : ML_WARPS / 2;
                     for (int i = 0; i < cnt; ++i) {
                         float v = 0.0f;
-#pragma unroll
-                        for (int q = 0; q < ML_WARPS / 2; ++q) {
-                            const float* c = all + (size_t)(q0 + q * qs) * RED;
-                            v += terms == 2 ? c[red_at(2 * i, row)] + c[red_at(2 * i + 1, row)] : c[red_at(i, row)];
-                        }
+                        const int c0 = red_at(terms * i, row), c1 = red_at(terms * i + terms - 1, row);
+#pragma unroll 8
+                        for (int q = 0; q < parts; ++q) v += terms == 2 ? part[q * 2 * RED + c0] + part[q * 2 * RED + c1] : part[q * 2 * RED + c0];
                         if (w.tiles == 1) v += __shfl_xor_sync(0xffffffffu, v, 16);
                         v = v * __shfl_sync(0xffffffffu, scale, i) * ts;
                         const size_t at = (size_t)__shfl_sync(0xffffffffu, pair, i);
@@ -560,8 +576,11 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                 publish();
                 continue;
             }
-            // compute warps: one 16-row tile each, every kgroups-th pair of blocks of the contraction
-            const int my_tile = w.tiles == 2 ? (warp & 1) : 0, kg = w.tiles == 2 ? warp >> 1 : warp, kgroups = ML_WARPS / w.tiles;
+            // A compute warp takes every 16th block of the contraction, of both tiles; with one tile, two blocks at a time.
+            constexpr bool F8 = FMT == LQ_FMT_FP8_B128;
+            const bool pairs = w.tiles == 1;
+            const int b0 = pairs && !F8 ? 2 * warp : warp;
+            const int tile2 = pairs ? 0 : 16 * w.pitch, scale2 = pairs ? 1 : 16 * srow;
             int cur = -1, cols = 0, slot = 0;
             for (int u = ua; u < ub; ++u, ++tile) {
                 if (tile == w.units_per_group) {
@@ -577,7 +596,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     const int cnt = min(TG, __popcll(m0) - first);
                     cols = (cnt * terms + 7) / 8;
                     // the finishers are done with the previous group's units, the compute warps with its activations
-                    for (int v = 0; v < ML_FINISH; ++v)
+                    for (int v = 0; v < L.finish; ++v)
                         if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.rempty[v], v < rb ? rlap : rlap ^ 1u));
                     consumers_sync();
                     if (tid < cnt) {
@@ -597,21 +616,27 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     const int per = cnt >= 9 ? 1 : (cnt >= 5 ? 2 : (cnt >= 3 ? 4 : (cnt == 2 ? 8 : 16)));
                     const int i = warp / per, part = (warp % per) * 32 + lane;
                     if (i < cnt) {
+                        const void* src = w.is_down ? L.act : L.x;
+                        const int type = w.is_down ? LQ_T_F32 : L.type;
+                        const bool wide = w.is_down || x_wide;
+                        const size_t row = (size_t)(w.is_down ? sh.gpair[i] : sh.gtok[i]) * w.k;
+                        auto fetch = [&](int k) { return wide ? ld8<true>(src, type, row + k) : ld8<false>(src, type, row + k); };
+                        Raw8 next[2];  // (on their way while the largest value is looked up)
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+                            if (part * 8 + q * per * 256 < w.k) next[q] = fetch(part * 8 + q * per * 256);
                         // exponent of the largest value -> 2^14 (kept where both powers of two are normal numbers)
                         const unsigned bits = __ldcg(w.is_down ? L.act_max + sh.gpair[i] : L.x_max + sh.gtok[i]);
                         const int ex2 = min(max((int)(bits >> 23), 15), 254);
                         // (an infinity makes the whole token NaN, like a NaN)
                         const float down = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(127 + 14 + 127 - ex2) << 23);
                         if (part == 0) sh.unscale[i] = __uint_as_float((uint32_t)(ex2 - 14) << 23);
-                        const size_t row = (size_t)(w.is_down ? sh.gpair[i] : sh.gtok[i]) * w.k;
                         uint8_t* dst = xs + (size_t)(i * terms) * xpitch;
-                        const void* src = w.is_down ? L.act : L.x;
-                        const int type = w.is_down ? LQ_T_F32 : L.type;
-                        const bool wide = w.is_down || x_wide;
-#pragma unroll 2
                         for (int k = part * 8; k < w.k; k += per * 256) {
                             float v[8];
-                            to_f32(wide ? ld8<true>(src, type, row + k) : ld8<false>(src, type, row + k), type, v);
+                            to_f32(next[0], type, v);
+                            next[0] = next[1];
+                            if (k + per * 512 < w.k) next[1] = fetch(k + per * 512);
                             uint32_t hi[4], lo[4];
 #pragma unroll
                             for (int q = 0; q < 4; ++q) {
@@ -644,39 +669,89 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) acc[j][q] = acc2[j][q] = 0.0f;
-                const uint8_t* s0 = w.scales + slot * 32 * srow + (my_tile * 16 + g) * srow;
-                const uint8_t* s1 = s0 + 8 * srow;
-                const float* fs = nullptr;
-                if (FMT == LQ_FMT_FP8_B128)
-                    fs = reinterpret_cast<const float*>(L.table[e].scales[w.is_down ? 2 : my_tile]) +
-                         (size_t)((w.is_down ? (tile * w.tiles + my_tile) * 16 : tile * 16) >> 7) * ((w.k + 127) >> 7);
-                // fragment rows: lanes 0-15 name the 16 rows of the first piece, 16-31 those of the second
-                const uint32_t frag = smem_u32(ring) + (uint32_t)((my_tile * 16 + (lane & 15)) * w.pitch + (lane >> 4) * 16);
-                const uint8_t* xcol = xs + (size_t)g * xpitch + t4 * 16;
+                const uint32_t s0 = smem_u32(w.scales) + (uint32_t)(slot * 32 * srow + g * srow);
+                const float *fs = nullptr, *fs2 = nullptr;
+                if (F8) {
+                    const int row_blocks = (w.k + 127) >> 7, row = (w.is_down ? tile * w.tiles : tile) * 16;
+                    fs = reinterpret_cast<const float*>(L.table[e].scales[w.is_down ? 2 : 0]) + (size_t)(row >> 7) * row_blocks;
+                    // (32 rows of a down unit start at a multiple of 32: one row of scale blocks)
+                    fs2 = w.is_down ? fs : reinterpret_cast<const float*>(L.table[e].scales[1]) + (size_t)(row >> 7) * row_blocks;
+                }
+                // fragment rows: FP4: lanes 0-15 name the rows of the first block, 16-31 those of the second; FP8: the halves
+                // of a block
+                const uint32_t frag = smem_u32(ring) + (uint32_t)((lane & 15) * w.pitch + (lane >> 4) * (F8 || pairs ? 16 : tile2));
+                const uint32_t xcol = smem_u32(xs) + (uint32_t)(g * xpitch + t4 * 16);
                 if (++slot == w.slots) slot = 0;
                 for (int c = 0; c < w.n_chunks; ++c) {
                     const int kb0 = c * (w.chunk / 32), blocks = min(w.chunk / 32, w.k / 32 - kb0);
                     if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.full[st], lap));
-                    const uint32_t rows = frag + (uint32_t)(st * L.stage_bytes);
-                    // Two blocks of 32 columns at a time, their products interleaved (past the end the second repeats the first with
-                    // a scale of zero); lo and hi are the f16 pairs of rows g and g + 8.
-                    auto products = [&](int kb, int kb2, const uint32_t (&lo)[2][4], const uint32_t (&hi)[2][4], const float (&f0)[2],
-                                        const float (&f1)[2]) {
+                    // addresses of the warp's first block; the others lie at constant distances
+                    const uint32_t ra = frag + (uint32_t)(st * L.stage_bytes + b0 * (F8 ? 32 : 16));
+                    const uint32_t sa = s0 + (FMT == LQ_FMT_NVFP4 ? 2 * (kb0 + b0) + (t4 >> 1) : kb0 + b0), sb = sa + 8 * srow;
+                    const uint32_t sc = sa + (FMT == LQ_FMT_NVFP4 && pairs ? 2 : scale2), sd = sc + 8 * srow;
+                    const uint32_t xa = xcol + (uint32_t)((kb0 + b0) * 64);
+                    // one step: block b0 + at of both tiles (PAIRS: blocks b0 + at and, `two`, b0 + at + D2 of the one tile)
+                    auto step = [&](auto pairs_tag, int at, bool two) {
+                        constexpr bool PAIRS = decltype(pairs_tag)::value;
+                        constexpr int D2 = PAIRS ? (F8 ? ML_WARPS : 1) : 0;
+                        // lo and hi: the f16 pairs of rows g and g + 8 of the first and the second block
+                        uint32_t lo[2][4], hi[2][4];
+                        float f0[2] = {0.0f, 0.0f}, f1[2] = {0.0f, 0.0f};
+                        const int d2 = PAIRS && !two ? 0 : D2;  // (past the end the second repeats the first, scaled by zero)
+                        if (F8) {
+                            uint32_t r[2][4];
+                            ldmatrix4(r[0], ra + at * 32);
+                            ldmatrix4(r[1], ra + tile2 + (at + d2) * 32);
+                            f0[0] = f1[0] = __ldg(fs + ((kb0 + b0 + at) >> 2));
+                            f0[1] = f1[1] = !PAIRS || two ? __ldg(fs2 + ((kb0 + b0 + at + d2) >> 2)) : 0.0f;
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                lo[q][0] = e4m3x2_f16(r[q][0]), lo[q][1] = e4m3x2_f16(r[q][0] >> 16);
+                                lo[q][2] = e4m3x2_f16(r[q][2]), lo[q][3] = e4m3x2_f16(r[q][2] >> 16);
+                                hi[q][0] = e4m3x2_f16(r[q][1]), hi[q][1] = e4m3x2_f16(r[q][1] >> 16);
+                                hi[q][2] = e4m3x2_f16(r[q][3]), hi[q][3] = e4m3x2_f16(r[q][3] >> 16);
+                            }
+                        } else {
+                            constexpr int SB = FMT == LQ_FMT_NVFP4 ? 2 : 1;  // scales per block
+                            uint32_t r[4];
+                            ldmatrix4(r, ra + at * 16);  // (one tile, past the end: any codes)
+                            const uint32_t u[4] = {lds_u8(sa + at * SB), lds_u8(sb + at * SB), !PAIRS || two ? lds_u8(sc + at * SB) : 0u,
+                                                   !PAIRS || two ? lds_u8(sd + at * SB) : 0u};
+                            if (FMT == LQ_FMT_MXFP4) {
+                                // 2^(byte - 127), 0 for 0 (e8m0_to_f32; a NaN scale was refused when the layer was made)
+                                f0[0] = __uint_as_float(u[0] << 23), f1[0] = __uint_as_float(u[1] << 23);
+                                f0[1] = __uint_as_float(u[2] << 23), f1[1] = __uint_as_float(u[3] << 23);
+                            }
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                e2m1x8(r[2 * q], lo[q]);
+                                e2m1x8(r[2 * q + 1], hi[q]);
+                                if (FMT == LQ_FMT_NVFP4) {
+                                    const uint32_t m0 = e4m3x2_f16(u[2 * q] | (u[2 * q] << 8)), m1 = e4m3x2_f16(u[2 * q + 1] | (u[2 * q + 1] << 8));
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        lo[q][i] = mul_f16x2(lo[q][i], m0);
+                                        hi[q][i] = mul_f16x2(hi[q][i], m1);
+                                    }
+                                }
+                            }
+                        }
 #pragma unroll
                         for (int j = 0; j < NT; ++j) {
                             if (NT > 1 && j >= cols) break;
-                            const uint8_t* xj = xcol + (size_t)j * 8 * xpitch;
-                            const uint4 x0 = *reinterpret_cast<const uint4*>(xj + kb * 64);
-                            const uint4 x1 = *reinterpret_cast<const uint4*>(xj + kb2 * 64);
+                            const uint32_t xj = xa + j * 8 * xpitch + at * 64;
+                            const uint4 x0 = lds_128(xj);
+                            uint4 x1 = x0;
+                            if (PAIRS) x1 = lds_128(xj + d2 * 64);
                             if (FMT == LQ_FMT_NVFP4) {
                                 mma_f16(acc[j], lo[0][0], hi[0][0], lo[0][1], hi[0][1], x0.x, x0.y);
                                 mma_f16(acc2[j], lo[1][0], hi[1][0], lo[1][1], hi[1][1], x1.x, x1.y);
                                 mma_f16(acc[j], lo[0][2], hi[0][2], lo[0][3], hi[0][3], x0.z, x0.w);
                                 mma_f16(acc2[j], lo[1][2], hi[1][2], lo[1][3], hi[1][3], x1.z, x1.w);
                             } else {
-                                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f}, h[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                mma_f16(d, lo[0][0], hi[0][0], lo[0][1], hi[0][1], x0.x, x0.y);
-                                mma_f16(h, lo[1][0], hi[1][0], lo[1][1], hi[1][1], x1.x, x1.y);
+                                float d[4], h[4];
+                                mma_f16_new(d, lo[0][0], hi[0][0], lo[0][1], hi[0][1], x0.x, x0.y);
+                                mma_f16_new(h, lo[1][0], hi[1][0], lo[1][1], hi[1][1], x1.x, x1.y);
                                 mma_f16(d, lo[0][2], hi[0][2], lo[0][3], hi[0][3], x0.z, x0.w);
                                 mma_f16(h, lo[1][2], hi[1][2], lo[1][3], hi[1][3], x1.z, x1.w);
 #pragma unroll
@@ -687,84 +762,42 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                             }
                         }
                     };
-                    if (FMT == LQ_FMT_FP8_B128) {
-                        for (int b = kg; b < blocks; b += 2 * kgroups) {
-                            const bool two = b + kgroups < blocks;
-                            const int b2 = two ? b + kgroups : b;
-                            uint32_t r[2][4], lo[2][4], hi[2][4];
-                            ldmatrix4(r[0], rows + b * 32);  // rows g, g + 8 of the first 16 columns; of the other 16
-                            ldmatrix4(r[1], rows + b2 * 32);
-                            const float f = __ldg(fs + ((kb0 + b) >> 2)), f2 = two ? __ldg(fs + ((kb0 + b2) >> 2)) : 0.0f;
+                    const int left = blocks - b0;  // (at most 46 blocks a stage, 22 for FP8)
+                    if (!pairs) {
 #pragma unroll
-                            for (int q = 0; q < 2; ++q) {
-                                lo[q][0] = e4m3x2_f16(r[q][0]), lo[q][1] = e4m3x2_f16(r[q][0] >> 16);
-                                lo[q][2] = e4m3x2_f16(r[q][2]), lo[q][3] = e4m3x2_f16(r[q][2] >> 16);
-                                hi[q][0] = e4m3x2_f16(r[q][1]), hi[q][1] = e4m3x2_f16(r[q][1] >> 16);
-                                hi[q][2] = e4m3x2_f16(r[q][3]), hi[q][3] = e4m3x2_f16(r[q][3] >> 16);
-                            }
-                            const float ff[2] = {f, f2};
-                            products(kb0 + b, kb0 + b2, lo, hi, ff, ff);
-                        }
+                        for (int i = 0; i < (F8 ? 2 : 3); ++i)
+                            if (i * ML_WARPS < left) step(std::false_type{}, i * ML_WARPS, true);
+                    } else if (F8) {
+                        if (left > 0) step(std::true_type{}, 0, left > ML_WARPS);
                     } else {
-                        for (int b = 2 * kg; b < blocks; b += 2 * kgroups) {
-                            const bool two = b + 1 < blocks;
-                            const int kb = kb0 + b, kb2 = two ? kb + 1 : kb;
-                            uint32_t r[4], lo[2][4], hi[2][4];
-                            ldmatrix4(r, rows + b * 16);  // rows g, g + 8 of block b; of block b + 1 (past the end: any codes)
-                            float f0[2] = {0.0f, 0.0f}, f1[2] = {0.0f, 0.0f};
-                            if (FMT == LQ_FMT_MXFP4) {
-                                // 2^(byte - 127), 0 for 0 (e8m0_to_f32; a NaN scale was refused when the layer was made)
-                                // (kb is even; past the end of a row of odd length the second byte is another scale, dropped)
-                                uint32_t u0, u1;
-                                const uint32_t keep = two ? 0x7f800000u : 0u;
-                                if (srow & 1) {
-                                    u0 = s0[kb] | (uint32_t)s0[kb + 1] << 8;
-                                    u1 = s1[kb] | (uint32_t)s1[kb + 1] << 8;
-                                } else {
-                                    u0 = *reinterpret_cast<const uint16_t*>(s0 + kb);
-                                    u1 = *reinterpret_cast<const uint16_t*>(s1 + kb);
-                                }
-                                f0[0] = __uint_as_float((u0 << 23) & 0x7f800000u);
-                                f1[0] = __uint_as_float((u1 << 23) & 0x7f800000u);
-                                f0[1] = __uint_as_float((u0 << 15) & keep);
-                                f1[1] = __uint_as_float((u1 << 15) & keep);
-                            }
 #pragma unroll
-                            for (int q = 0; q < 2; ++q) {
-                                e2m1x8(r[2 * q], lo[q]);
-                                e2m1x8(r[2 * q + 1], hi[q]);
-                                if (FMT == LQ_FMT_NVFP4) {
-                                    const int k2 = 2 * (q ? kb2 : kb) + (t4 >> 1);
-                                    const uint32_t u0 = q && !two ? 0u : s0[k2], u1 = q && !two ? 0u : s1[k2];
-                                    const uint32_t m0 = e4m3x2_f16(u0 | (u0 << 8)), m1 = e4m3x2_f16(u1 | (u1 << 8));
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        lo[q][i] = mul_f16x2(lo[q][i], m0);
-                                        hi[q][i] = mul_f16x2(hi[q][i], m1);
-                                    }
-                                }
-                            }
-                            products(kb, kb2, lo, hi, f0, f1);
-                        }
+                        for (int i = 0; i < 2; ++i)
+                            if (i * 2 * ML_WARPS < left) step(std::true_type{}, i * 2 * ML_WARPS, left > i * 2 * ML_WARPS + 1);
                     }
                     __syncwarp();
                     if (lane == 0) ml_arrive(&sh.empty[st]);
                     if (++st == L.n_stages) st = 0, lap ^= 1u;
                 }
                 if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.rempty[rb], rlap ^ 1u));
-                float* mine = red + (rb * ML_WARPS + warp) * RED;
+                float* mine = red + (rb * ML_WARPS + warp) * 2 * RED;
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     if (NT > 1 && j >= cols) break;
                     const int col = j * 8 + 2 * t4;
-                    mine[red_at(col, g)] = acc[j][0] + acc2[j][0];
-                    mine[red_at(col + 1, g)] = acc[j][1] + acc2[j][1];
-                    mine[red_at(col, g + 8)] = acc[j][2] + acc2[j][2];
-                    mine[red_at(col + 1, g + 8)] = acc[j][3] + acc2[j][3];
+                    const int at[4] = {red_at(col, g), red_at(col + 1, g), red_at(col, g + 8), red_at(col + 1, g + 8)};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if (w.tiles == 2) {
+                            mine[at[q]] = acc[j][q];
+                            mine[RED + at[q]] = acc2[j][q];
+                        } else {
+                            mine[at[q]] = acc[j][q] + acc2[j][q];
+                        }
+                    }
                 }
                 __syncwarp();
                 if (lane == 0) ml_arrive(&sh.rfull[rb]);
-                if (++rb == ML_FINISH) rb = 0, rlap ^= 1u;
+                if (++rb == L.finish) rb = 0, rlap ^= 1u;
             }
         }
         if (!ok && lane == 0) sh.failed = 1;
@@ -803,39 +836,52 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
 }
 
 // Shared memory beside the ring and the scales, a unit's scales, a stage.
-size_t fixed_smem(int nt, int hidden, int inter) {
-    return 128 + (sizeof(MlSmem) + 127) / 128 * 128 + ML_FINISH * (size_t)ML_WARPS * nt * 8 * 16 * 4 +
+size_t fixed_smem(int nt, int finish, int hidden, int inter) {
+    return 128 + (sizeof(MlSmem) + 127) / 128 * 128 + finish * (size_t)ML_WARPS * 2 * nt * 8 * 16 * 4 +
            (size_t)nt * 8 * std::max(act_pitch(hidden), act_pitch(inter));
 }
 template <int FMT>
 int stage_size(int hidden, int inter) {
     return 32 * std::max(code_bytes<FMT>(stage_cols<FMT>(hidden)), code_bytes<FMT>(stage_cols<FMT>(inter)));
 }
-// The most stages that fit, and a phase's slots for scales: between a unit's first stage and the stage it replaces lie at
-// most n_stages / chunks of its units.
+// How shared memory is dealt out.
+struct Plan {
+    int stages, finish;  // of the ring; finishers at work (a buffer of partial sums each)
+    int slots[2];        // scales of units, per phase
+    size_t bytes;
+};
+// The most stages that fit, with fewer finishers where that leaves under three.  Between a unit's first stage and the stage it
+// replaces lie at most stages / chunks units of a phase: so many slots its scales need, and one.
 template <int FMT>
-int plan_ring(int nt, int hidden, int inter, int (&slots)[2]) {
+Plan plan_ring(int nt, int hidden, int inter) {
     auto chunks = [](int k) { return (k + chunk_cols<FMT>(k) - 1) / chunk_cols<FMT>(k); };
-    for (int n = ML_MAX_STAGES; n >= 2; --n) {
-        slots[0] = (n + chunks(hidden) - 1) / chunks(hidden) + 1;
-        slots[1] = (n + chunks(inter) - 1) / chunks(inter) + 1;
-        const size_t scales = 32 * ((size_t)slots[0] * row_scale_bytes<FMT>(hidden) + (size_t)slots[1] * row_scale_bytes<FMT>(inter));
-        if (fixed_smem(nt, hidden, inter) + scales + (size_t)n * stage_size<FMT>(hidden, inter) <= 227 * 1024) return n;
+    Plan p = {};
+    for (int finish = ML_FINISH; finish >= 1; --finish) {
+        for (int n = ML_MAX_STAGES; n >= 2; --n) {
+            const int slots[2] = {(n + chunks(hidden) - 1) / chunks(hidden) + 1, (n + chunks(inter) - 1) / chunks(inter) + 1};
+            const size_t scales = 32 * ((size_t)slots[0] * row_scale_bytes<FMT>(hidden) + (size_t)slots[1] * row_scale_bytes<FMT>(inter));
+            const size_t bytes = fixed_smem(nt, finish, hidden, inter) + scales + (size_t)n * stage_size<FMT>(hidden, inter);
+            if (bytes <= 227 * 1024) {
+                if (n > p.stages) p = Plan{n, finish, {slots[0], slots[1]}, bytes};
+                break;
+            }
+        }
+        if (p.stages >= 3) break;
     }
-    return 0;
+    return p;
 }
 
 template <int FMT, int NT>
 cudaError_t launch_layer(MoeLayer L, int sm_count, cudaStream_t st) {
-    L.n_stages = plan_ring<FMT>(NT, L.hidden, L.inter, L.scale_slots);
-    if (L.n_stages == 0) return cudaErrorInvalidConfiguration;
+    const Plan p = plan_ring<FMT>(NT, L.hidden, L.inter);
+    if (p.stages == 0) return cudaErrorInvalidConfiguration;
+    L.n_stages = p.stages, L.finish = p.finish, L.scale_slots[0] = p.slots[0], L.scale_slots[1] = p.slots[1];
     L.stage_bytes = stage_size<FMT>(L.hidden, L.inter);
-    const size_t smem = fixed_smem(NT, L.hidden, L.inter) + 32 * ((size_t)L.scale_slots[0] * row_scale_bytes<FMT>(L.hidden) + (size_t)L.scale_slots[1] * row_scale_bytes<FMT>(L.inter)) + (size_t)L.n_stages * L.stage_bytes;
     const void* fn = (const void*)moe_layer_kernel<FMT, NT>;
     cudaError_t e = set_max_dyn_smem(fn, 227 * 1024);
     if (e != cudaSuccess) return e;
     void* args[] = {&L};
-    return cudaLaunchCooperativeKernel(fn, dim3(sm_count), dim3(ML_THREADS), args, smem, st);
+    return cudaLaunchCooperativeKernel(fn, dim3(sm_count), dim3(ML_THREADS), args, p.bytes, st);
 }
 
 template <int FMT>
@@ -844,8 +890,7 @@ cudaError_t launch_fmt(MoeLayer L, int sm_count, cudaStream_t st) {
     // Two tiles of columns when an expert's tokens are likely to fill more than one (an expert with more tokens than a
     // group holds is read once per group) and shared memory takes them beside a ring that covers the memory's latency.
     int nt = L.tokens * L.top_e * L.terms > 5 * L.experts && L.tokens * L.terms > 8 ? 2 : 1;
-    int slots[2];
-    if (nt > 1 && (size_t)plan_ring<FMT>(nt, L.hidden, L.inter, slots) * stage_size<FMT>(L.hidden, L.inter) < 48 * 1024) nt = 1;
+    if (nt > 1 && (size_t)plan_ring<FMT>(nt, L.hidden, L.inter).stages * stage_size<FMT>(L.hidden, L.inter) < 48 * 1024) nt = 1;
     return nt == 1 ? launch_layer<FMT, 1>(L, sm_count, st) : launch_layer<FMT, 2>(L, sm_count, st);
 }
 
@@ -853,8 +898,7 @@ cudaError_t launch_fmt(MoeLayer L, int sm_count, cudaStream_t st) {
 
 template <int FMT>
 static bool fits(int hidden, int inter) {
-    int slots[2];
-    return plan_ring<FMT>(1, hidden, inter, slots) > 0;
+    return plan_ring<FMT>(1, hidden, inter).stages > 0;
 }
 bool moe_layer_supported(int fmt, int hidden, int inter) {
     if (hidden <= 0 || inter <= 0 || hidden % 32 || inter % 32 || hidden > 8192 || inter > 8192) return false;
