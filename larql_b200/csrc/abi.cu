@@ -2319,7 +2319,7 @@ int lq_dev_block_norm(lq_ctx* ctx, const lq_block_norm_args* q) {
     a.gate_group = (long long)std::min<size_t>(std::max<size_t>(q->gate_group, 1), 0x7fffffffu);
     a.rows = (int)q->rows, a.cols = (int)q->cols, a.gate_cols = (int)q->gate_cols;
     a.w_type = q->w_type, a.post_norm = q->post_norm != 0;
-    a.w_offset = q->w_offset, a.h_scale = q->h_scale, a.y_scale = q->y_scale, a.eps = q->eps;
+    a.w_offset = q->w_offset, a.h_scale = q->h_scale, a.y_scale = q->y_scale, a.eps = q->eps, a.err = ctx->d_err;
     CK(launch_block_norm(a, q->type, ctx->sm_count, ctx->stream));
     ctx->launches += 1;
     return LQ_OK;

@@ -7,8 +7,10 @@
 // run_ffn's norm -> FFN -> residual add (crates/larql-compute/src/forward/layer.rs:61-127) with the post-FFN
 // norm, the learned weights and the residual multiplier of layers that have them.
 //
-// Everything is kept in f32 between the loads and the stores (n is taken from the unrounded h'), the squares are
-// summed in f64: v^2 of a bf16 or f32 activation can leave f32's range, and the sum costs nothing beside the loads.
+// What bounds it is reading h, y, gate and writing h', n once (one token: the two reductions' latency).  Everything is
+// kept in f32 between the loads and the stores, n is taken from the unrounded h'.  A row's squares are summed in f32,
+// pairwise over the threads; when that sum leaves f32's range the row is summed again relative to its largest value
+// (f64 sums, which need no branch, cost 36 us of 159 at 4096 x 8192 bf16: the conversions run at a few lanes a cycle).  Underflow needs no branch: what a square loses is below 2^-149 and eps is at least 2^-126.
 // rms is at least sqrt(eps) >= 2^-63, so 1 / rms is a normal f32 and one multiply per element replaces a division.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -38,10 +40,14 @@ struct alignas(VEC * sizeof(T)) Pack {
     T v[VEC];
 };
 
-// Weights come in any of the three types, whatever the activation's: VEC of them as f32.
-template <int VEC>
+// VEC weights as f32: of the activation's type (SAME: one access), or of any type, element by element.
+template <class T, int VEC, bool SAME>
 __device__ __forceinline__ void load_w(const void* w, int type, size_t at, float (&out)[VEC]) {
-    if (type == LQ_T_F32) {
+    if (SAME) {
+        const Pack<T, VEC> p = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(w) + at);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[i] = to_f32(p.v[i]);
+    } else if (type == LQ_T_F32) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) out[i] = static_cast<const float*>(w)[at + i];
     } else if (type == LQ_T_BF16) {
@@ -53,98 +59,109 @@ __device__ __forceinline__ void load_w(const void* w, int type, size_t at, float
     }
 }
 
-// Sum over the threads of a row: one warp (WARP) or the whole block.
-template <bool WARP>
-__device__ __forceinline__ double row_sum(double s, double* red) {
+// Over the threads of a row, one warp (WARP) or the whole block: the sum, or the maximum of non-negative values.
+template <bool WARP, bool MAX>
+__device__ __forceinline__ float row_reduce(float s, float* red) {
+    auto op = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    for (int o = 16; o > 0; o >>= 1) s = op(s, __shfl_xor_sync(0xffffffffu, s, o));
     if (WARP) return s;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockDim.x >> 5;
-    __syncthreads();  // the previous sum has been read
+    __syncthreads();  // the previous result has been read
     if (lane == 0) red[warp] = s;
     __syncthreads();
-    s = lane < n ? red[lane] : 0.0;
+    s = lane < n ? red[lane] : 0.0f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    for (int o = 16; o > 0; o >>= 1) s = op(s, __shfl_xor_sync(0xffffffffu, s, o));
     return s;
 }
 
+// 1 / rms of the row whose elements the threads hold N each (zero past the end).
+template <bool WARP, int N>
+__device__ __forceinline__ float inverse_rms(const float (&v)[N], float inv_cols, float eps, float* red) {
+    float q[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i] = v[i] * v[i];
+#pragma unroll
+    for (int n = N / 2; n > 0; n >>= 1)
+#pragma unroll
+        for (int i = 0; i < n; ++i) q[i] += q[i + n];
+    const float s = row_reduce<WARP, false>(q[0], red);
+    if (s <= 1e38f) return 1.0f / sqrtf(s * inv_cols + eps);
+    if (s != s) return s;
+    float m = 0.0f;  // beyond f32 (the same for every thread of the row)
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(v[i]));
+    m = row_reduce<WARP, true>(m, red);
+    if (m > 3.4e38f) return 0.0f;  // an infinity: finite / inf, and inf * 0 = NaN where it stands
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t = fmaf(v[i] / m, v[i] / m, t);
+    t = row_reduce<WARP, false>(t, red);
+    return 1.0f / m / sqrtf(t * inv_cols);  // (eps is nothing beside such values)
+}
+
 // One row per warp (WARP: blockDim = 32 x rows) or per block; a thread holds NV packs of VEC elements.
-template <class T, int VEC, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) block_norm_kernel(const BlockNorm a) {
-    __shared__ double red[32];
+template <class T, int VEC, int NV, bool WARP, bool SAME, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_kernel(const BlockNorm a) {
+    __shared__ float red[32];
     const int tid = threadIdx.x, step = blockDim.x;
     const int n_pack = a.cols / VEC;
-    const double inv_cols = 1.0 / (double)a.cols;
+    const float inv_cols = 1.0f / (float)a.cols, eps = (float)a.eps;
     using P = Pack<T, VEC>;
     const int rows_per = WARP ? blockDim.y : 1;
     for (int row = blockIdx.x * rows_per + (WARP ? threadIdx.y : 0); row < a.rows; row += gridDim.x * rows_per) {
-        P h[NV], y[NV], g[NV];
+        P h[NV], g[NV];
+        float v[NV * VEC];  // y, then z, then h'
         const T* hp = static_cast<const T*>(a.h) + (size_t)row * a.h_stride;
         const T* yp = static_cast<const T*>(a.y) + (a.y ? (size_t)row * a.y_stride : 0);
-        const T* gp = static_cast<const T*>(a.gate) + (a.gate ? (size_t)(row / a.gate_group) * a.gate_stride : 0);
+        const T* gp = static_cast<const T*>(a.gate) + (a.gate ? (size_t)(row / (int)a.gate_group) * a.gate_stride : 0);
         const bool gate_vec = a.gate && a.gate_cols != 1;
         float gs = a.y_scale;
         if (a.gate && a.gate_cols == 1) gs *= to_f32(gp[0]);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int p = tid + i * step;
+            P y = {};
             if (p < n_pack) {
-                if (a.y) y[i] = *reinterpret_cast<const P*>(yp + (size_t)p * VEC);
+                if (a.y) y = *reinterpret_cast<const P*>(yp + (size_t)p * VEC);
                 h[i] = *reinterpret_cast<const P*>(hp + (size_t)p * VEC);
                 if (gate_vec) g[i] = *reinterpret_cast<const P*>(gp + (size_t)p * VEC);
             }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[i * VEC + j] = to_f32(y.v[j]);
         }
-        float v[NV * VEC];
         float inv = 1.0f;
-        if (a.post_norm) {
-            double s = 0.0;
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (tid + i * step < n_pack)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        const double d = (double)to_f32(y[i].v[j]);
-                        s = fma(d, d, s);
-                    }
-            s = row_sum<WARP>(s, red);
-            inv = (float)(1.0 / sqrt(s * inv_cols + a.eps));
-        }
-        double s = 0.0;
+        if (a.post_norm) inv = inverse_rms<WARP>(v, inv_cols, eps, red);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int p = tid + i * step;
             if (p < n_pack) {
-                float w[VEC];
-                if (a.post_norm && a.post_w) load_w<VEC>(a.post_w, a.w_type, (size_t)p * VEC, w);
+                if (a.post_norm) {
+                    float w[VEC];
+                    if (a.post_w) load_w<T, VEC, SAME>(a.post_w, a.w_type, (size_t)p * VEC, w);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[i * VEC + j] *= a.post_w ? inv * (a.w_offset + w[j]) : inv;
+                }
                 P o;
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     float x = a.h_scale * to_f32(h[i].v[j]);
-                    if (a.y) {
-                        float z = to_f32(y[i].v[j]);
-                        if (a.post_norm) {
-                            z *= inv;
-                            if (a.post_w) z *= a.w_offset + w[j];
-                        }
-                        x = fmaf(gate_vec ? gs * to_f32(g[i].v[j]) : gs, z, x);
-                    }
+                    if (a.y) x = fmaf(gate_vec ? gs * to_f32(g[i].v[j]) : gs, v[i * VEC + j], x);
                     v[i * VEC + j] = x;
                     o.v[j] = from_f32<T>(x);
-                    s = fma((double)x, (double)x, s);
                 }
                 if (a.h_out) *reinterpret_cast<P*>(static_cast<T*>(a.h_out) + (size_t)row * a.h_out_stride + (size_t)p * VEC) = o;
             }
         }
         if (a.n_out) {
-            s = row_sum<WARP>(s, red);
-            inv = (float)(1.0 / sqrt(s * inv_cols + a.eps));
+            inv = inverse_rms<WARP>(v, inv_cols, eps, red);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int p = tid + i * step;
                 if (p < n_pack) {
                     float w[VEC];
-                    if (a.pre_w) load_w<VEC>(a.pre_w, a.w_type, (size_t)p * VEC, w);
+                    if (a.pre_w) load_w<T, VEC, SAME>(a.pre_w, a.w_type, (size_t)p * VEC, w);
                     P o;
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) {
@@ -159,32 +176,161 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) block_norm_kernel(const Blo
     }
 }
 
-template <class T, int VEC, int NV>
+// Many long rows: a block walks its rows with the next one's operands on their way into shared memory (bulk copies), so
+// that the memory is never idle during a row's two reductions.  4096 x 8192 bf16 with a full gate: 74 us against 98
+// with loads into registers.
+template <class T, int VEC, int NV, bool SAME, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_stream_kernel(const BlockNorm a, int gate_rows) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float red[32];
+    __shared__ uint64_t full[2];
+    const int tid = threadIdx.x, step = blockDim.x;
+    const int n_pack = a.cols / VEC;
+    const float inv_cols = 1.0f / (float)a.cols, eps = (float)a.eps;
+    using P = Pack<T, VEC>;
+    const uint32_t row_bytes = (uint32_t)a.cols * sizeof(T), stage = row_bytes * (gate_rows ? 3 : 2);
+    auto issue = [&](int s, int row) {  // h, y and the row's own gate row, behind one another
+        uint8_t* dst = smem + (size_t)s * stage;
+        mbar_expect_tx(&full[s], stage);
+        tma_bulk_g2s(dst, static_cast<const T*>(a.h) + (size_t)row * a.h_stride, row_bytes, &full[s]);
+        tma_bulk_g2s(dst + row_bytes, static_cast<const T*>(a.y) + (size_t)row * a.y_stride, row_bytes, &full[s]);
+        if (gate_rows) tma_bulk_g2s(dst + 2 * row_bytes, static_cast<const T*>(a.gate) + (size_t)row * a.gate_stride, row_bytes, &full[s]);
+    };
+    if (tid == 0) {
+        mbar_init(&full[0], 1);
+        mbar_init(&full[1], 1);
+        fence_mbar_init();
+        issue(0, blockIdx.x);  // (the grid is no larger than the rows)
+        if (blockIdx.x + gridDim.x < (unsigned)a.rows) issue(1, blockIdx.x + gridDim.x);
+    }
+    __syncthreads();
+    bool ok = true;
+    int s = 0;
+    uint32_t phase = 0;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        if (ok) ok = mbar_wait(&full[s], phase);
+        const T* hs = reinterpret_cast<const T*>(smem + (size_t)s * stage);
+        const T* ys = hs + a.cols;
+        const T* gp = gate_rows ? ys + a.cols : static_cast<const T*>(a.gate) + (a.gate ? (size_t)(row / a.gate_group) * a.gate_stride : 0);
+        const bool gate_vec = a.gate && a.gate_cols != 1;
+        float gs = a.y_scale;
+        if (a.gate && a.gate_cols == 1) gs *= to_f32(gp[0]);
+        float v[NV * VEC];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int p = tid + i * step;
+            P y = {};
+            if (p < n_pack) y = *reinterpret_cast<const P*>(ys + p * VEC);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[i * VEC + j] = to_f32(y.v[j]);
+        }
+        float inv = 1.0f;
+        if (a.post_norm) inv = inverse_rms<false>(v, inv_cols, eps, red);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int p = tid + i * step;
+            if (p < n_pack) {
+                if (a.post_norm) {
+                    float w[VEC];
+                    if (a.post_w) load_w<T, VEC, SAME>(a.post_w, a.w_type, (size_t)p * VEC, w);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[i * VEC + j] *= a.post_w ? inv * (a.w_offset + w[j]) : inv;
+                }
+                const P h = *reinterpret_cast<const P*>(hs + p * VEC);
+                P g = {}, o;
+                if (gate_vec) g = *reinterpret_cast<const P*>(gp + p * VEC);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float x = fmaf(gate_vec ? gs * to_f32(g.v[j]) : gs, v[i * VEC + j], a.h_scale * to_f32(h.v[j]));
+                    v[i * VEC + j] = x;
+                    o.v[j] = from_f32<T>(x);
+                }
+                if (a.h_out) *reinterpret_cast<P*>(static_cast<T*>(a.h_out) + (size_t)row * a.h_out_stride + (size_t)p * VEC) = o;
+            }
+        }
+        if (a.n_out) inv = inverse_rms<false>(v, inv_cols, eps, red);
+        else __syncthreads();
+        // (everyone has read the stage: the reduction above was a barrier)
+        if (tid == 0 && ok && row + 2ll * gridDim.x < a.rows) issue(s, (int)(row + 2ll * gridDim.x));
+        if (a.n_out) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int p = tid + i * step;
+                if (p < n_pack) {
+                    float w[VEC];
+                    if (a.pre_w) load_w<T, VEC, SAME>(a.pre_w, a.w_type, (size_t)p * VEC, w);
+                    P o;
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) {
+                        float x = v[i * VEC + j] * inv;
+                        if (a.pre_w) x *= a.w_offset + w[j];
+                        o.v[j] = from_f32<T>(x);
+                    }
+                    *reinterpret_cast<P*>(static_cast<T*>(a.n_out) + (size_t)row * a.n_out_stride + (size_t)p * VEC) = o;
+                }
+            }
+        }
+        s ^= 1;
+        if (s == 0) phase ^= 1;
+    }
+    if (!ok && tid == 0) set_err(a.err, DEV_ERR_TMA_TIMEOUT);
+}
+
+template <class T, int VEC, int NV, bool SAME, int THREADS>
+cudaError_t launch_stream(const BlockNorm& a, int threads, int gate_rows, size_t smem, int sm_count, cudaStream_t st) {
+    auto* fn = block_norm_stream_kernel<T, VEC, NV, SAME, THREADS>;
+    cudaError_t e = set_max_dyn_smem((const void*)fn, 224 * 1024 * THREADS / 1024);
+    if (e != cudaSuccess) return e;
+    fn<<<std::min(a.rows, sm_count * (1024 / THREADS)), threads, smem, st>>>(a, gate_rows);
+    return cudaGetLastError();
+}
+
+template <class T, int VEC, int NV, bool SAME>
 cudaError_t launch_norm(const BlockNorm& a, int sm_count, cudaStream_t st) {
     const int n_pack = a.cols / VEC;
     if (n_pack <= 32 * NV) {
-        const int grid = (int)min((long long)(a.rows + 7) / 8, (long long)sm_count * 32);
-        block_norm_kernel<T, VEC, NV, true><<<grid, dim3(32, 8), 0, st>>>(a);
-    } else {
-        const int threads = ((n_pack + NV - 1) / NV + 31) / 32 * 32;
-        const int grid = (int)min((long long)a.rows, (long long)sm_count * 32);
-        block_norm_kernel<T, VEC, NV, false><<<grid, threads, 0, st>>>(a);
+        const int grid = (int)std::min<long long>(((long long)a.rows + 7) / 8, (long long)sm_count * 32);
+        block_norm_kernel<T, VEC, NV, true, SAME, 256><<<grid, dim3(32, 8), 0, st>>>(a);
+        return cudaGetLastError();
     }
+    const int threads = ((n_pack + NV - 1) / NV + 31) / 32 * 32;
+    if constexpr (VEC > 1) {
+        // Streaming pays from two rows per resident block on, for rows long enough to hide a copy's latency; its outputs may
+        // be the rows of h or y (a row is written after it was read) but not lie in rows that are read later.
+        const int gate_rows = a.gate && a.gate_cols != 1 && a.gate_group == 1;
+        const int resident = threads <= 256 ? 4 : (threads <= 512 ? 2 : 1);
+        const size_t smem = 2 * (size_t)a.cols * sizeof(T) * (gate_rows ? 3 : 2);
+        if (a.y && threads > 128 && a.rows >= 2 * resident * sm_count && smem <= (size_t)(224 * 1024 / resident)) {
+            if (resident == 4) return launch_stream<T, VEC, NV, SAME, 256>(a, threads, gate_rows, smem, sm_count, st);
+            if (resident == 2) return launch_stream<T, VEC, NV, SAME, 512>(a, threads, gate_rows, smem, sm_count, st);
+            return launch_stream<T, VEC, NV, SAME, 1024>(a, threads, gate_rows, smem, sm_count, st);
+        }
+    }
+    const int grid = (int)std::min<long long>(a.rows, (long long)sm_count * 32);
+    if (threads <= 256) block_norm_kernel<T, VEC, NV, false, SAME, 256><<<grid, threads, 0, st>>>(a);
+    else if (threads <= 512) block_norm_kernel<T, VEC, NV, false, SAME, 512><<<grid, threads, 0, st>>>(a);
+    else block_norm_kernel<T, VEC, NV, false, SAME, 1024><<<grid, threads, 0, st>>>(a);
     return cudaGetLastError();
 }
 
 template <class T>
-cudaError_t launch_norm_t(const BlockNorm& a, int sm_count, cudaStream_t st) {
+cudaError_t launch_norm_t(const BlockNorm& a, int type, int sm_count, cudaStream_t st) {
     constexpr int VEC = 16 / (int)sizeof(T);
-    // 16-byte accesses need every row of every operand to start on one, weights included (a pack of VEC weights)
-    const size_t z = sizeof(T), wz = a.w_type == LQ_T_F32 ? 4 : 2;
+    // 16-byte accesses need every row of every operand to start on a multiple of 16 bytes; weights of the activation's type
+    // are read the same way, others element by element.
+    const size_t z = sizeof(T);
     auto fits = [&](const void* p, long long stride) { return !p || (((uintptr_t)p | (size_t)stride * z) & 15) == 0; };
     const bool vec = a.cols % VEC == 0 && fits(a.h, a.h_stride) && fits(a.y, a.y_stride) &&
                      fits(a.h_out, a.h_out_stride) && fits(a.n_out, a.n_out_stride) &&
-                     (a.gate_cols == 1 || fits(a.gate, a.gate_stride)) &&
-                     (((uintptr_t)a.post_w | (uintptr_t)a.pre_w) & (wz - 1)) == 0;
-    if (vec) return launch_norm<T, VEC, 16 / VEC>(a, sm_count, st);
-    return launch_norm<T, 1, 16>(a, sm_count, st);
+                     (a.gate_cols == 1 || fits(a.gate, a.gate_stride));
+    const bool same = a.w_type == type && fits(a.post_w, 0) && fits(a.pre_w, 0);
+    if (!vec) return a.cols <= 8192 ? launch_norm<T, 1, 8, false>(a, sm_count, st) : launch_norm<T, 1, 16, false>(a, sm_count, st);
+    // 16 elements a thread hold fewer threads to a row (two rows of 8192 share an SM); 8 where the registers of 16 f32
+    // elements of three operands do not fit, and for few rows, whose latency more threads cut
+    constexpr int WIDE = 16 / VEC, NARROW = 8 / VEC;
+    const bool narrow = a.cols <= 8192 && (sizeof(T) == 4 || a.rows <= sm_count);
+    if (narrow) return same ? launch_norm<T, VEC, NARROW, true>(a, sm_count, st) : launch_norm<T, VEC, NARROW, false>(a, sm_count, st);
+    return same ? launch_norm<T, VEC, WIDE, true>(a, sm_count, st) : launch_norm<T, VEC, WIDE, false>(a, sm_count, st);
 }
 
 }  // namespace
@@ -192,9 +338,9 @@ cudaError_t launch_norm_t(const BlockNorm& a, int sm_count, cudaStream_t st) {
 cudaError_t launch_block_norm(const BlockNorm& a, int type, int sm_count, cudaStream_t st) {
     if (a.rows <= 0) return cudaSuccess;
     switch (type) {
-        case LQ_T_F32: return launch_norm_t<float>(a, sm_count, st);
-        case LQ_T_BF16: return launch_norm_t<__nv_bfloat16>(a, sm_count, st);
-        case LQ_T_F16: return launch_norm_t<__half>(a, sm_count, st);
+        case LQ_T_F32: return launch_norm_t<float>(a, type, sm_count, st);
+        case LQ_T_BF16: return launch_norm_t<__nv_bfloat16>(a, type, sm_count, st);
+        case LQ_T_F16: return launch_norm_t<__half>(a, type, sm_count, st);
     }
     return cudaErrorInvalidValue;
 }

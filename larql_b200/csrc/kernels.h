@@ -197,6 +197,7 @@ struct BlockNorm {
     int rows, cols, gate_cols, w_type, post_norm;
     float w_offset, h_scale, y_scale;
     double eps;
+    int* err;
 };
 cudaError_t launch_block_norm(const BlockNorm& a, int type, int sm_count, cudaStream_t st);
 
