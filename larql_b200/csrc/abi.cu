@@ -2371,7 +2371,7 @@ int lq_dev_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const void* x, int x_type
     const size_t kb = (cols + 127) / 128, chunk = 32768;  // (bounds the codes' workspace)
     for (size_t t0 = 0; t0 < tokens; t0 += chunk) {
         const size_t n = std::min(chunk, tokens - t0);
-        Fp8Product p;
+        Fp8Product p = {};
         p.w = (const uint8_t*)w->data;
         p.w_scales = (const float*)w->scales;
         p.rows = rows, p.cols = cols, p.tokens = n;
@@ -2388,8 +2388,8 @@ int lq_dev_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const void* x, int x_type
             p.code_pitch = pitch;
             p.scales = (const float*)(ctx->op_codes.p + a256(n * pitch));
         }
-        if ((rc = ensure_op(ctx, ctx->op_part, fp8_part_bytes(n, ctx->sm_count)))) return rc;
-        if ((rc = ensure_op(ctx, ctx->op_done, fp8_tile_count(n, rows) * sizeof(unsigned)))) return rc;
+        if ((rc = ensure_op(ctx, ctx->op_part, fp8_part_bytes(n, rows, cols, ctx->sm_count)))) return rc;
+        if ((rc = ensure_op(ctx, ctx->op_done, fp8_tile_count(n, rows, cols, ctx->sm_count) * sizeof(unsigned)))) return rc;
         p.part = (float*)ctx->op_part.p;
         p.done = (unsigned*)ctx->op_done.p;
         if (!coded) {

@@ -20,6 +20,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cmath>
+
 #include "../../include/larql_cuda.h"
 #include "kernels.h"
 #include "tc5.cuh"
@@ -70,50 +72,75 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return r;
 }
 
-// 16 threads per (token, block of 128), 8 consecutive elements each.  The quotient is the correctly rounded one
-// (and not x times 1 / s): the codes are defined by it, and the tests hold them to the definition bit for bit.
+// The correctly rounded quotient x / s, from r = 1 / s correctly rounded: a product, its exact remainder, one correction
+// (Markstein's theorem).  Valid where no step under- or overflows; quotients below 2^-10 may be off, their code is 0
+// either way.
+__device__ __forceinline__ float quotient(float x, float s, float r) {
+    const float q = __fmul_rn(x, r);
+    return copysignf(__fmaf_rn(__fmaf_rn(-q, s, x), r, q), x);  // (s > 0; the correction of a zero would drop its sign)
+}
+
+// 16 threads per (token, block of 128), 8 consecutive elements each; QU such blocks are on their way at a time.  The
+// quotient is the correctly rounded one (and not x times 1 / s): the codes are defined by it, and the tests hold them to
+// the definition bit for bit.
+constexpr int QU = 4;
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__ x, long long x_stride, long long units,
                                                            int kb_n, int cols, uint8_t* __restrict__ codes,
                                                            long long code_pitch, float* __restrict__ scales, int wide_store) {
     pdl_launch_next();
     const int sub = threadIdx.x & 15;
-    for (long long u0 = (long long)blockIdx.x * 16; u0 < units; u0 += (long long)gridDim.x * 16) {
-        const long long u = u0 + (threadIdx.x >> 4);
-        const bool on = u < units;
-        const long long t = on ? u / kb_n : 0;
-        const int kb = on ? (int)(u - t * kb_n) : 0, k0 = kb * 128 + sub * 8;
-        float v[8];
+    for (long long u0 = (long long)blockIdx.x * (16 * QU); u0 < units; u0 += (long long)gridDim.x * (16 * QU)) {
+        float v[QU][8];
+        long long t[QU];
+        int k0[QU];
+        bool on[QU];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        if (on) {
-            const T* p = x + t * x_stride + k0;
-            if (VEC) {
-                if (k0 < cols) ld8(p, v);
-            } else {
+        for (int n = 0; n < QU; ++n) {
+            const long long u = u0 + n * 16 + (threadIdx.x >> 4);
+            on[n] = u < units;
+            t[n] = units <= 0x7fffffff ? (long long)((unsigned)u / (unsigned)kb_n) : u / kb_n;
+            k0[n] = (int)(u - t[n] * kb_n) * 128 + sub * 8;
+            on[n] = on[n] && k0[n] < cols;  // (a block past its last column takes part in its reduction with zeros)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (k0 + i < cols) v[i] = ld_f32(p + i);
+            for (int i = 0; i < 8; ++i) v[n][i] = 0.0f;
+            if (on[n]) {
+                const T* p = x + t[n] * x_stride + k0[n];
+                if (VEC) {
+                    ld8(p, v[n]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (k0[n] + i < cols) v[n][i] = ld_f32(p + i);
+                }
             }
         }
-        float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(v[i]));
+        for (int n = 0; n < QU; ++n) {
+            float m = 0.0f;
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float s = max_nan(__fdiv_rn(m, F8_MAX), F8_MIN_SCALE);
-        uint32_t w[4];
+            for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(v[n][i]));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = e4m3x2(__fdiv_rn(v[2 * i], s), __fdiv_rn(v[2 * i + 1], s));
-        if (on) {
-            if (sub == 0) scales[t * kb_n + kb] = s;
-            uint8_t* q = codes + t * code_pitch + k0;
+            for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const float s = max_nan(__fdiv_rn(m, F8_MAX), F8_MIN_SCALE);
+            uint32_t w[4];
+            if (s > 0x1p-100f && s < 0x1p100f) {
+                const float r = __frcp_rn(s);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = e4m3x2(quotient(v[n][2 * i], s, r), quotient(v[n][2 * i + 1], s, r));
+            } else {  // tiny, huge, infinite or NaN
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = e4m3x2(__fdiv_rn(v[n][2 * i], s), __fdiv_rn(v[n][2 * i + 1], s));
+            }
+            if (!on[n]) continue;
+            if (sub == 0) scales[t[n] * kb_n + (k0[n] >> 7)] = s;
+            uint8_t* q = codes + t[n] * code_pitch + k0[n];
             if (wide_store) {  // cols (and the pitch) are multiples of 8
-                if (k0 < cols) *reinterpret_cast<uint2*>(q) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+                *reinterpret_cast<uint2*>(q) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (k0 + i < cols) q[i] = (uint8_t)(w[i >> 1] >> (8 * (i & 1)));
+                    if (k0[n] + i < cols) q[i] = (uint8_t)(w[i >> 1] >> (8 * (i & 1)));
             }
         }
     }
@@ -142,6 +169,7 @@ struct F8Args {
     long long out_stride;
     int out_type;
     int tokens, rows, kb_n;
+    int whole;         // few-token kernel: a CTA's run is whole tiles (nothing to join)
     float* part;       // few-token kernel: [grid][2][NT][128] partial tiles
     unsigned* done;    // few-token kernel: k blocks finished per tile (zero between launches)
     int* err;
@@ -152,14 +180,14 @@ constexpr int FEW_BUFS = 4;  // accumulator buffers in tensor memory
 
 constexpr int few_stage_bytes(int nt) { return 128 * 128 + nt * 128; }
 constexpr int few_stages(int nt) { return nt <= 16 ? 11 : (nt <= 32 ? 10 : (nt <= 64 ? 8 : 6)); }
-constexpr int few_promo_warps(int nt) { return nt <= 64 ? 4 : 8; }
-constexpr int few_threads(int nt) { return 64 + 32 * few_promo_warps(nt); }
+constexpr int few_promo_warps(int nt) { return nt <= 64 ? nt / 4 : 16; }  // 16 columns a warp, 32 at the widest
+constexpr int few_threads(int nt) { return 128 + 32 * few_promo_warps(nt); }  // (two warps idle: a warp reads the TMEM lanes of its rank of 4)
 
 template <int NT>
 struct FewSmem {
     uint64_t full[few_stages(NT)], empty[few_stages(NT)];
     uint64_t acc_full[FEW_BUFS], acc_empty[FEW_BUFS];
-    float sx[few_promo_warps(NT)][2][NT];  // the scales of a k block's tokens, per warp
+    alignas(16) float sx[few_promo_warps(NT)][2][NT];  // the scales of a k block's tokens, per warp
     uint32_t tmem;
     int failed;
     int last;
@@ -177,7 +205,9 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int tok_tiles = (a.tokens + NT - 1) / NT, row_tiles = (a.rows + 127) / 128;
     const long long units = (long long)row_tiles * tok_tiles * a.kb_n;
-    const long long u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+    const long long tiles = (long long)row_tiles * tok_tiles;
+    const long long u0 = a.whole ? tiles * blockIdx.x / gridDim.x * a.kb_n : units * blockIdx.x / gridDim.x;
+    const long long u1 = a.whole ? tiles * (blockIdx.x + 1) / gridDim.x * a.kb_n : units * (blockIdx.x + 1) / gridDim.x;
 
     if (tid == 0) {
         for (int i = 0; i < STAGES; ++i) {
@@ -202,39 +232,42 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     if (warp == 0) {
         // ---- producer: weight and token tiles of the run's units ----
         if (lane == 0) {
-            auto coords = [&](long long u, int& row, int& tok, int& k) {
-                const long long tile = u / a.kb_n;
-                k = (int)(u - tile * a.kb_n) * 128;
-                row = (int)(tile / tok_tiles) * 128;
-                tok = (int)(tile % tok_tiles) * NT;
+            // position of a unit, stepped along: row tile, token tile (innermost after k), k block
+            struct Pos {
+                int row, tok, kb;
+            };
+            const long long tile0 = u0 / a.kb_n;
+            const Pos begin{(int)(tile0 / tok_tiles), (int)(tile0 % tok_tiles), (int)(u0 - tile0 * a.kb_n)};
+            auto next = [&](Pos& p) {
+                if (++p.kb == a.kb_n) {
+                    p.kb = 0;
+                    if (++p.tok == tok_tiles) p.tok = 0, ++p.row;
+                }
             };
             // the weight does not depend on the kernel before this one (the quantisation of the tokens)
-            const long long head = min(u1, u0 + STAGES);
-            int row, tok, k;
-            for (long long u = u0; u < head; ++u) {
-                const int st = (int)(u - u0);
-                coords(u, row, tok, k);
+            const int head = (int)min(u1 - u0, (long long)STAGES);
+            Pos p = begin;
+            for (int st = 0; st < head; ++st, next(p)) {
                 mbar_expect_tx(&sh.full[st], STAGE);
-                tma_load_2d(ring + st * STAGE, &map_w, k, row, &sh.full[st]);
+                tma_load_2d(ring + st * STAGE, &map_w, p.kb * 128, p.row * 128, &sh.full[st]);
             }
+            Pos px = begin;
             pdl_wait();
-            for (long long u = u0; u < head; ++u) {
-                const int st = (int)(u - u0);
-                coords(u, row, tok, k);
-                tma_load_2d(ring + st * STAGE + 128 * 128, &map_x, k, tok, &sh.full[st]);
-            }
+            for (int st = 0; st < head; ++st, next(px))
+                tma_load_2d(ring + st * STAGE + 128 * 128, &map_x, px.kb * 128, px.tok * NT, &sh.full[st]);
             bool ok = true;
-            long long u = head;
-            for (; u < u1; ++u) {
-                const int n = (int)(u - u0), st = n % STAGES;
-                if (!mbar_wait(&sh.empty[st], (uint32_t)(n / STAGES - 1) & 1u)) {
+            long long u = u0 + head;
+            int st = head == STAGES ? 0 : head;
+            uint32_t lap = 0;  // parity of the lap whose reads free a stage
+            for (; u < u1; ++u, next(p)) {
+                if (!mbar_wait(&sh.empty[st], lap)) {
                     ok = false;
                     break;
                 }
-                coords(u, row, tok, k);
                 mbar_expect_tx(&sh.full[st], STAGE);
-                tma_load_2d(ring + st * STAGE, &map_w, k, row, &sh.full[st]);
-                tma_load_2d(ring + st * STAGE + 128 * 128, &map_x, k, tok, &sh.full[st]);
+                tma_load_2d(ring + st * STAGE, &map_w, p.kb * 128, p.row * 128, &sh.full[st]);
+                tma_load_2d(ring + st * STAGE + 128 * 128, &map_x, p.kb * 128, p.tok * NT, &sh.full[st]);
+                if (++st == STAGES) st = 0, lap ^= 1u;
             }
             if (!ok) {  // the copies in flight have to land before the block's shared memory goes away
                 for (long long v = max(u0, u - STAGES); v < u; ++v) {
@@ -248,10 +281,11 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     } else if (warp == 1) {
         // ---- tensor core: one accumulator buffer per k block ----
         bool ok = true;
+        int st = 0, buf = 0;
+        uint32_t lap = 0, blap = 0;
         for (long long u = u0; u < u1; ++u) {
-            const int n = (int)(u - u0), st = n % STAGES, buf = n % FEW_BUFS;
-            ok = mbar_wait(&sh.full[st], (uint32_t)(n / STAGES) & 1u);
-            if (ok && n >= FEW_BUFS) ok = mbar_wait(&sh.acc_empty[buf], (uint32_t)(n / FEW_BUFS - 1) & 1u);
+            ok = mbar_wait(&sh.full[st], lap);
+            if (ok) ok = mbar_wait(&sh.acc_empty[buf], blap ^ 1u);  // (the first lap's wait passes)
             if (!__all_sync(0xffffffffu, ok)) break;
             tc5_fence_after();
             if (elect_one()) {
@@ -263,12 +297,14 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 umma_commit1(&sh.acc_full[buf]);
             }
             __syncwarp();
+            if (++st == STAGES) st = 0, lap ^= 1u;
+            if (++buf == FEW_BUFS) buf = 0, blap ^= 1u;
         }
         if (!__all_sync(0xffffffffu, ok) && lane == 0) sh.failed = 1;
-    } else {
+    } else if (warp >= 4) {
         // ---- promotion: thread = row of the weight (TMEM lane); COLS tokens ----
         pdl_wait();  // the tokens' scales
-        const int pw = warp - 2, quarter = warp & 3, col0 = (pw >> 2) * COLS;
+        const int pw = warp - 4, quarter = warp & 3, col0 = (pw >> 2) * COLS;
         const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)col0;
         float acc[COLS];
         bool ok = true;
@@ -306,13 +342,20 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 }
                 if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[buf], (uint32_t)(n / FEW_BUFS) & 1u));
                 tc5_fence_after();
+                uint32_t v[2][16];  // a chunk is read while the one before it is added up
+                tmem_load16(tbase + buf * NT, v[0]);
 #pragma unroll
-                for (int c = 0; c < COLS; c += 16) {
-                    uint32_t v[16];
-                    tmem_load16(tbase + buf * NT + c, v);
-                    tmem_wait16(v);
+                for (int c = 0; c < COLS / 16; ++c) {
+                    tmem_wait16(v[c & 1]);
+                    if (c + 1 < COLS / 16) tmem_load16(tbase + buf * NT + (c + 1) * 16, v[(c + 1) & 1]);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(__uint_as_float(v[i]), sxs[c + i], acc[c + i]);
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(sxs + c * 16 + i);
+                        acc[c * 16 + i] = fmaf(__uint_as_float(v[c & 1][i]), f.x, acc[c * 16 + i]);
+                        acc[c * 16 + i + 1] = fmaf(__uint_as_float(v[c & 1][i + 1]), f.y, acc[c * 16 + i + 1]);
+                        acc[c * 16 + i + 2] = fmaf(__uint_as_float(v[c & 1][i + 2]), f.z, acc[c * 16 + i + 2]);
+                        acc[c * 16 + i + 3] = fmaf(__uint_as_float(v[c & 1][i + 3]), f.w, acc[c * 16 + i + 3]);
+                    }
                 }
                 tc5_fence_before();
                 mbar_arrive_one(&sh.acc_empty[buf]);
@@ -335,16 +378,30 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 #pragma unroll
             for (int i = 0; i < COLS; ++i)
                 if (tok0 + col0 + i < a.tokens) __stcg(mine + (size_t)(col0 + i) * 128 + quarter * 32 + lane, acc[i]);
-            __threadfence();
-            asm volatile("bar.sync 1, %0;" ::"n"(PW * 32) : "memory");
-            if (tid == 64) {
-                const unsigned before = atomicAdd(&a.done[tile], (unsigned)(kb_b - kb_a));
-                sh.last = before + (unsigned)(kb_b - kb_a) == (unsigned)a.kb_n;
-                if (sh.last) a.done[tile] = 0;  // ready for the next launch
-                __threadfence();
+            // If the other pieces are all there, this one needs no publication (usual for the tile a run ends in: the next
+            // run began with the tile's other end): its threads read what they wrote themselves.
+            const unsigned mine_kb = (unsigned)(kb_b - kb_a);
+            if (tid == 128) {
+                unsigned now;
+                asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(a.done + tile) : "memory");
+                sh.last = now + mine_kb == (unsigned)a.kb_n;
             }
             asm volatile("bar.sync 1, %0;" ::"n"(PW * 32) : "memory");
-            const int is_last = sh.last;
+            const bool alone = sh.last;
+            if (alone && tid == 128) a.done[tile] = 0;  // ready for the next launch
+            int is_last = alone;
+            if (!alone) {
+                __threadfence();
+                asm volatile("bar.sync 1, %0;" ::"n"(PW * 32) : "memory");
+                if (tid == 128) {
+                    const unsigned before = atomicAdd(&a.done[tile], mine_kb);
+                    sh.last = before + mine_kb == (unsigned)a.kb_n;
+                    if (sh.last) a.done[tile] = 0;
+                    __threadfence();
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(PW * 32) : "memory");
+                is_last = sh.last;
+            }
             if (is_last) {
                 const long long t0 = tile * a.kb_n, t1 = t0 + a.kb_n;
                 // the run of CTA c is [units * c / grid, units * (c + 1) / grid)
@@ -382,7 +439,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 // ----------------------------------------------------------- many tokens ----
 constexpr int MANY_M = 128, MANY_N = 256, MANY_STAGES = 4;
 constexpr int MANY_STAGE = (MANY_M + MANY_N) * 128;
-constexpr int MANY_THREADS = 64 + 256;
+constexpr int MANY_THREADS = 128 + 512;  // producer, tensor core, two idle warps (a warp reads the TMEM lanes of its rank of 4), promotion
 
 struct ManySmem {
     uint64_t full[MANY_STAGES], empty[MANY_STAGES];
@@ -416,7 +473,7 @@ fp8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.acc_full[i], 1);
-            mbar_init(&sh.acc_empty[i], 256);
+            mbar_init(&sh.acc_empty[i], 512);
         }
         sh.failed = 0;
         fence_mbar_init();
@@ -478,22 +535,23 @@ fp8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                 __syncwarp();
             }
         if (!ok && lane == 0) sh.failed = 1;
-    } else {
-        // thread = token (TMEM lane), 128 rows of the weight (one row of scale blocks)
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
-        const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+    } else if (warp >= 4) {
+        // thread = token (TMEM lane), 64 rows of the weight (of one row of scale blocks)
+        constexpr int COLS = 64;
+        const int quarter = warp & 3, col0 = ((warp - 4) >> 2) * COLS;
+        const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)col0;
         const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | (size_t)a.out_stride * sizeof(T)) & 15) == 0;
         bool ok = true;
         int n = 0;
         for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
             int mt, nt;
             tile_at(t, mt, nt);
-            const int tok = mt * MANY_M + quarter * 32 + lane, row0 = nt * MANY_N + half * 128;
+            const int tok = mt * MANY_M + quarter * 32 + lane, row0 = nt * MANY_N + col0;
             const float* sxp = a.sx + (size_t)min(tok, a.tokens - 1) * a.kb_n;
             const float* swp = a.sw + (size_t)(min(row0, a.rows - 1) >> 7) * a.kb_n;
-            float acc[128];
+            float acc[COLS];
 #pragma unroll
-            for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
+            for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
             float nx = sxp[0], nw = swp[0];
             for (int kb = 0; kb < a.kb_n; ++kb, ++n) {
                 const int buf = n & 1;
@@ -505,17 +563,14 @@ fp8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                 ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[buf], (uint32_t)(n >> 1) & 1u));
                 if (!ok) break;
                 tc5_fence_after();
+                uint32_t v[2][16];  // a chunk is read while the one before it is added up
+                tmem_load16(tbase + buf * MANY_N, v[0]);
 #pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    uint32_t v[16], w[16];
-                    tmem_load16(tbase + buf * MANY_N + c, v);
-                    tmem_load16(tbase + buf * MANY_N + c + 16, w);
-                    tmem_wait16(v);
-                    tmem_wait16(w);
+                for (int c = 0; c < COLS / 16; ++c) {
+                    tmem_wait16(v[c & 1]);
+                    if (c + 1 < COLS / 16) tmem_load16(tbase + buf * MANY_N + (c + 1) * 16, v[(c + 1) & 1]);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(__uint_as_float(v[i]), f, acc[c + i]);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[c + 16 + i] = fmaf(__uint_as_float(w[i]), f, acc[c + 16 + i]);
+                    for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fmaf(__uint_as_float(v[c & 1][i]), f, acc[c * 16 + i]);
                 }
                 tc5_fence_before();
                 mbar_arrive_one(&sh.acc_empty[buf]);
@@ -524,9 +579,9 @@ fp8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             if (tok < a.tokens) {
                 T* o = static_cast<T*>(a.out) + (size_t)tok * a.out_stride + row0;
                 constexpr int V = 16 / (int)sizeof(T);
-                if (wide && row0 + 128 <= a.rows) {
+                if (wide && row0 + COLS <= a.rows) {
 #pragma unroll
-                    for (int i = 0; i < 128; i += V) {
+                    for (int i = 0; i < COLS; i += V) {
                         alignas(16) T p[V];
 #pragma unroll
                         for (int j = 0; j < V; ++j) p[j] = narrow<T>(acc[i + j]);
@@ -534,7 +589,7 @@ fp8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                     }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 128; ++i)
+                    for (int i = 0; i < COLS; ++i)
                         if (row0 + i < a.rows) o[i] = narrow<T>(acc[i]);
                 }
             }
@@ -598,7 +653,34 @@ cudaError_t launch_many(const Fp8Product& p, const F8Args& a, int grid, bool ove
 
 // Columns of an accumulator of the few-token kernel.
 int few_columns(size_t tokens) { return tokens <= 16 ? 16 : (tokens <= 32 ? 32 : (tokens <= 64 ? 64 : 128)); }
-bool takes_few(size_t tokens) { return tokens <= 128; }
+
+// How a product runs, from estimates in microseconds (fitted to 18 shapes of 1 to 4096 tokens): a k block of a few-token
+// tile takes an SM 0.30 to 0.75 by its columns, or the memory the time of its 16 KB; joining pieces of tiles costs 3.5
+// and 0.11 per column; a k block of a 128 x 256 tile of the other kernel takes 0.55.  Measured: 16 tokens x 28672 ->
+// 8192: spread 53, whole tiles 76, the other kernel 122 us; 1 x 3840 -> 15360: 25, 19, 25; 250 x 2880 -> 2880: 31, 23,
+// 23; 128 x 28672 -> 8192: 102, 177, 135; 1024 x 8192 -> 8192: 200, 213, 92.
+struct Way {
+    bool few, whole;
+    int grid;
+};
+Way way_of(size_t tokens, size_t rows, size_t cols, int sm_count) {
+    const double kb = (double)((cols + 127) / 128), sms = sm_count;
+    const int nt = few_columns(tokens);
+    const double tiles = (double)((tokens + nt - 1) / nt) * (double)((rows + 127) / 128), units = tiles * kb;
+    const double memory = (double)((rows + 127) / 128) * kb * 0.00264;
+    const double unit = nt <= 32 ? 0.30 : (nt == 64 ? 0.38 : 0.75);
+    const double whole = std::max(memory, std::ceil(tiles / sms) * kb * unit);
+    const double spread = std::max(memory, std::ceil(units / sms) * unit) + 3.5 + 0.11 * nt;
+    Way w;
+    w.whole = whole <= spread;
+    w.few = true;
+    w.grid = (int)std::min(w.whole ? tiles : units, sms);
+    if (tokens > 64) {
+        const double t2 = (double)((tokens + MANY_M - 1) / MANY_M) * (double)((rows + MANY_N - 1) / MANY_N);
+        if (std::ceil(t2 / sms) * kb * 0.55 < std::min(whole, spread)) w = Way{false, true, (int)std::min(t2, sms)};
+    }
+    return w;
+}
 
 }  // namespace
 
@@ -607,7 +689,7 @@ cudaError_t launch_fp8_quantize(const void* x, int type, size_t tokens, size_t c
     if (tokens == 0 || cols == 0) return cudaSuccess;
     const int kb_n = (int)((cols + 127) / 128);
     const long long units = (long long)tokens * kb_n;
-    const int grid = (int)std::min<long long>((units + 15) / 16, (long long)sm_count * 64);
+    const int grid = (int)std::min<long long>((units + 16 * QU - 1) / (16 * QU), (long long)sm_count * 32);
     const size_t z = type == LQ_T_F32 ? 4 : 2;
     const bool vec = cols % 8 == 0 && (((uintptr_t)x | x_stride * z) & 15) == 0;
     const int wide = cols % 8 == 0 && (((uintptr_t)codes | code_pitch) & 7) == 0;
@@ -627,22 +709,26 @@ cudaError_t launch_fp8_quantize(const void* x, int type, size_t tokens, size_t c
 }
 
 // Partial tiles and counters of the few-token kernel.
-size_t fp8_part_bytes(size_t tokens, int sm_count) {
-    return takes_few(tokens) ? (size_t)sm_count * 2 * few_columns(tokens) * 128 * 4 : 0;
+size_t fp8_part_bytes(size_t tokens, size_t rows, size_t cols, int sm_count) {
+    const Way w = way_of(tokens, rows, cols, sm_count);
+    return w.few && !w.whole ? (size_t)w.grid * 2 * few_columns(tokens) * 128 * 4 : 0;
 }
-size_t fp8_tile_count(size_t tokens, size_t rows) {
+size_t fp8_tile_count(size_t tokens, size_t rows, size_t cols, int sm_count) {
     const size_t nt = (size_t)few_columns(tokens);
-    return takes_few(tokens) ? ((rows + 127) / 128) * ((tokens + nt - 1) / nt) : 0;
+    const Way w = way_of(tokens, rows, cols, sm_count);
+    return w.few && !w.whole ? ((rows + 127) / 128) * ((tokens + nt - 1) / nt) : 0;
 }
-
 cudaError_t launch_fp8_matmul(const Fp8Product& p, bool overlap, int sm_count, int* err, cudaStream_t st) {
     const int kb_n = (int)((p.cols + 127) / 128);
-    const F8Args a{p.scales, p.w_scales, p.out, (long long)p.out_stride, p.out_type, (int)p.tokens, (int)p.rows, kb_n, p.part,
-                   p.done, err};
-    if (takes_few(p.tokens)) {
+    F8Args a{};
+    a.sx = p.scales, a.sw = p.w_scales, a.out = p.out, a.out_stride = (long long)p.out_stride, a.out_type = p.out_type;
+    a.tokens = (int)p.tokens, a.rows = (int)p.rows, a.kb_n = kb_n;
+    a.part = p.part, a.done = p.done, a.err = err;
+    const Way w = way_of(p.tokens, p.rows, p.cols, sm_count);
+    const int grid = w.grid;
+    a.whole = w.whole;
+    if (w.few) {
         const int nt = few_columns(p.tokens);
-        const long long units = (long long)fp8_tile_count(p.tokens, p.rows) * kb_n;
-        const int grid = (int)std::min<long long>(units, sm_count);
         switch (nt) {
             case 16: return launch_few<16>(p, a, grid, overlap, st);
             case 32: return launch_few<32>(p, a, grid, overlap, st);
@@ -650,8 +736,6 @@ cudaError_t launch_fp8_matmul(const Fp8Product& p, bool overlap, int sm_count, i
         }
         return launch_few<128>(p, a, grid, overlap, st);
     }
-    const long long tiles = (long long)((p.tokens + MANY_M - 1) / MANY_M) * ((p.rows + MANY_N - 1) / MANY_N);
-    const int grid = (int)std::min<long long>(tiles, sm_count);
     if (p.out_type == LQ_T_F32) return launch_many<float>(p, a, grid, overlap, st);
     if (p.out_type == LQ_T_BF16) return launch_many<__nv_bfloat16>(p, a, grid, overlap, st);
     return launch_many<__half>(p, a, grid, overlap, st);

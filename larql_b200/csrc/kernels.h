@@ -215,8 +215,8 @@ struct Fp8Product {
     float* part;             // fp8_part_bytes of workspace
     unsigned* done;          // fp8_tile_count counters, zero between launches
 };
-size_t fp8_part_bytes(size_t tokens, int sm_count);
-size_t fp8_tile_count(size_t tokens, size_t rows);
+size_t fp8_part_bytes(size_t tokens, size_t rows, size_t cols, int sm_count);
+size_t fp8_tile_count(size_t tokens, size_t rows, size_t cols, int sm_count);
 // overlap: the kernel before this one on the stream is this product's own quantisation (it may start while that ends)
 cudaError_t launch_fp8_matmul(const Fp8Product& p, bool overlap, int sm_count, int* err, cudaStream_t st);
 
