@@ -17,6 +17,7 @@
 
 #include "../../include/larql_cuda.h"
 #include "kernels.h"
+#include "tc5.cuh"
 
 namespace lq {
 
@@ -110,6 +111,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_kernel(con
     const float inv_cols = 1.0f / (float)a.cols, eps = (float)a.eps;
     using P = Pack<T, VEC>;
     const int rows_per = WARP ? blockDim.y : 1;
+    pdl_wait();
     for (int row = blockIdx.x * rows_per + (WARP ? threadIdx.y : 0); row < a.rows; row += gridDim.x * rows_per) {
         P h[NV], g[NV];
         float v[NV * VEC];  // y, then z, then h'
@@ -200,6 +202,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_stream_ker
         mbar_init(&full[0], 1);
         mbar_init(&full[1], 1);
         fence_mbar_init();
+    }
+    pdl_wait();
+    if (tid == 0) {
         issue(0, blockIdx.x);  // (the grid is no larger than the rows)
         if (blockIdx.x + gridDim.x < (unsigned)a.rows) issue(1, blockIdx.x + gridDim.x);
     }
@@ -281,8 +286,7 @@ cudaError_t launch_stream(const BlockNorm& a, int threads, int gate_rows, size_t
     auto* fn = block_norm_stream_kernel<T, VEC, NV, SAME, THREADS>;
     cudaError_t e = set_max_dyn_smem((const void*)fn, 224 * 1024 * THREADS / 1024);
     if (e != cudaSuccess) return e;
-    fn<<<std::min(a.rows, sm_count * (1024 / THREADS)), threads, smem, st>>>(a, gate_rows);
-    return cudaGetLastError();
+    return launch_chained(fn, dim3(std::min(a.rows, sm_count * (1024 / THREADS))), dim3(threads), smem, st, a, gate_rows);
 }
 
 template <class T, int VEC, int NV, bool SAME>
@@ -290,8 +294,7 @@ cudaError_t launch_norm(const BlockNorm& a, int sm_count, cudaStream_t st) {
     const int n_pack = a.cols / VEC;
     if (n_pack <= 32 * NV) {
         const int grid = (int)std::min<long long>(((long long)a.rows + 7) / 8, (long long)sm_count * 32);
-        block_norm_kernel<T, VEC, NV, true, SAME, 256><<<grid, dim3(32, 8), 0, st>>>(a);
-        return cudaGetLastError();
+        return launch_chained(block_norm_kernel<T, VEC, NV, true, SAME, 256>, dim3(grid), dim3(32, 8), 0, st, a);
     }
     const int threads = ((n_pack + NV - 1) / NV + 31) / 32 * 32;
     if constexpr (VEC > 1) {
@@ -307,10 +310,9 @@ cudaError_t launch_norm(const BlockNorm& a, int sm_count, cudaStream_t st) {
         }
     }
     const int grid = (int)std::min<long long>(a.rows, (long long)sm_count * 32);
-    if (threads <= 256) block_norm_kernel<T, VEC, NV, false, SAME, 256><<<grid, threads, 0, st>>>(a);
-    else if (threads <= 512) block_norm_kernel<T, VEC, NV, false, SAME, 512><<<grid, threads, 0, st>>>(a);
-    else block_norm_kernel<T, VEC, NV, false, SAME, 1024><<<grid, threads, 0, st>>>(a);
-    return cudaGetLastError();
+    if (threads <= 256) return launch_chained(block_norm_kernel<T, VEC, NV, false, SAME, 256>, dim3(grid), dim3(threads), 0, st, a);
+    if (threads <= 512) return launch_chained(block_norm_kernel<T, VEC, NV, false, SAME, 512>, dim3(grid), dim3(threads), 0, st, a);
+    return launch_chained(block_norm_kernel<T, VEC, NV, false, SAME, 1024>, dim3(grid), dim3(threads), 0, st, a);
 }
 
 template <class T>

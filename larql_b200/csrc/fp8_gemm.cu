@@ -37,30 +37,6 @@ __device__ __forceinline__ float ld_f32(const float* p) { return *p; }
 __device__ __forceinline__ float ld_f32(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float ld_f32(const __half* p) { return __half2float(*p); }
 
-__device__ __forceinline__ void ld8(const float* p, float (&v)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void ld8(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-}
-__device__ __forceinline__ void ld8(const __half* p, float (&v)[8]) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-    }
-}
 __device__ __forceinline__ float max_nan(float a, float b) {  // a NaN wins: it must reach the scale
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -80,67 +56,109 @@ __device__ __forceinline__ float quotient(float x, float s, float r) {
     return copysignf(__fmaf_rn(__fmaf_rn(-q, s, x), r, q), x);  // (s > 0; the correction of a zero would drop its sign)
 }
 
-// 16 threads per (token, block of 128), 8 consecutive elements each; QU such blocks are on their way at a time.  The
-// quotient is the correctly rounded one (and not x times 1 / s): the codes are defined by it, and the tests hold them to
-// the definition bit for bit.
-constexpr int QU = 4;
+// Eight consecutive elements as they lie, their conversion, and the bits of their largest |value| as an f32 (as integers:
+// a NaN's are above every number's).
+template <class T>
+struct Eight {
+    uint4 a, b;
+};
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__ x, long long x_stride, long long units,
-                                                           int kb_n, int cols, uint8_t* __restrict__ codes,
-                                                           long long code_pitch, float* __restrict__ scales, int wide_store) {
+__device__ __forceinline__ Eight<T> load8(const T* p, int n) {
+    Eight<T> r;
+    r.a = r.b = make_uint4(0, 0, 0, 0);
+    if (VEC) {
+        r.a = __ldg(reinterpret_cast<const uint4*>(p));
+        if (sizeof(T) == 4) r.b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+    } else {
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : T(0.0f);
+        memcpy(&r.a, v, 16);
+        if (sizeof(T) == 4) memcpy(&r.b, reinterpret_cast<const uint8_t*>(v) + sizeof(T) * 8 - 16, 16);
+    }
+    return r;
+}
+template <class T>
+__device__ __forceinline__ void values8(const Eight<T>& r, float (&v)[8]) {
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (std::is_same<T, float>::value) v[i] = __uint_as_float(w[i]);
+        else if (std::is_same<T, __nv_bfloat16>::value) v[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        else v[i] = __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> (16 * (i & 1)))));
+    }
+}
+// Largest |value| of a block of 128, 16 threads' eights: 16-bit types two at a time as integers of the same order.
+template <class T>
+__device__ __forceinline__ float block_amax(const Eight<T>& r) {
+    if (std::is_same<T, float>::value) {
+        const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        return __uint_as_float(m);
+    }
+    uint32_t m = __vmaxu2(__vmaxu2(r.a.x & 0x7fff7fffu, r.a.y & 0x7fff7fffu), __vmaxu2(r.a.z & 0x7fff7fffu, r.a.w & 0x7fff7fffu));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = max(m >> 16, m & 0xffffu);
+    return std::is_same<T, __nv_bfloat16>::value ? __uint_as_float(m << 16) : __half2float(__ushort_as_half((unsigned short)m));
+}
+
+// 16 threads per (token, block of 128), 8 consecutive elements each; QU such blocks are on their way at a time (1 where
+// there are few).  The quotients are the correctly rounded ones (and not x times 1 / s): the codes are defined by them,
+// and the tests hold them to the definition bit for bit.  Instructions bound it: 90 for a thread's eight elements.
+template <class T, bool VEC, int QU>
+__global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__ x, long long x_stride, int units, int kb_n,
+                                                           int cols, uint8_t* __restrict__ codes, long long code_pitch,
+                                                           float* __restrict__ scales, int wide_store) {
+    pdl_wait();  // (before the next kernel may start: what it reads early was complete when this one began)
     pdl_launch_next();
     const int sub = threadIdx.x & 15;
-    for (long long u0 = (long long)blockIdx.x * (16 * QU); u0 < units; u0 += (long long)gridDim.x * (16 * QU)) {
-        float v[QU][8];
-        long long t[QU];
-        int k0[QU];
-        bool on[QU];
+    for (int u0 = blockIdx.x * (16 * QU); u0 < units; u0 += gridDim.x * (16 * QU)) {
+        Eight<T> r[QU];
+        int t[QU], kb[QU];
+        const int first = u0 + (threadIdx.x >> 4);
+        t[0] = (int)((unsigned)first / (unsigned)kb_n);
+        kb[0] = first - t[0] * kb_n;
 #pragma unroll
         for (int n = 0; n < QU; ++n) {
-            const long long u = u0 + n * 16 + (threadIdx.x >> 4);
-            on[n] = u < units;
-            t[n] = units <= 0x7fffffff ? (long long)((unsigned)u / (unsigned)kb_n) : u / kb_n;
-            k0[n] = (int)(u - t[n] * kb_n) * 128 + sub * 8;
-            on[n] = on[n] && k0[n] < cols;  // (a block past its last column takes part in its reduction with zeros)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[n][i] = 0.0f;
-            if (on[n]) {
-                const T* p = x + t[n] * x_stride + k0[n];
-                if (VEC) {
-                    ld8(p, v[n]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (k0[n] + i < cols) v[n][i] = ld_f32(p + i);
-                }
+            if (n) {  // 16 blocks on
+                t[n] = t[n - 1], kb[n] = kb[n - 1] + 16;
+                while (kb[n] >= kb_n) kb[n] -= kb_n, ++t[n];
             }
+            const int k0 = kb[n] * 128 + sub * 8;
+            r[n].a = r[n].b = make_uint4(0, 0, 0, 0);
+            if (first + n * 16 < units && k0 < cols) r[n] = load8<T, VEC>(x + t[n] * x_stride + k0, cols - k0);
         }
 #pragma unroll
         for (int n = 0; n < QU; ++n) {
-            float m = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(v[n][i]));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float s = max_nan(__fdiv_rn(m, F8_MAX), F8_MIN_SCALE);
+            const float m = block_amax(r[n]);
+            float v[8], s;
+            values8(r[n], v);
             uint32_t w[4];
-            if (s > 0x1p-100f && s < 0x1p100f) {
-                const float r = __frcp_rn(s);
+            if (m > 0x1p-90f && m < 0x1p100f) {
+                s = quotient(m, F8_MAX, 1.0f / F8_MAX);  // (a constant, correctly rounded)
+                const float inv = __frcp_rn(s);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = e4m3x2(quotient(v[n][2 * i], s, r), quotient(v[n][2 * i + 1], s, r));
-            } else {  // tiny, huge, infinite or NaN
+                for (int i = 0; i < 4; ++i) w[i] = e4m3x2(quotient(v[2 * i], s, inv), quotient(v[2 * i + 1], s, inv));
+            } else {  // zero, tiny, huge, infinite or NaN
+                s = max_nan(__fdiv_rn(m, F8_MAX), F8_MIN_SCALE);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = e4m3x2(__fdiv_rn(v[n][2 * i], s), __fdiv_rn(v[n][2 * i + 1], s));
+                for (int i = 0; i < 4; ++i) w[i] = e4m3x2(__fdiv_rn(v[2 * i], s), __fdiv_rn(v[2 * i + 1], s));
             }
-            if (!on[n]) continue;
-            if (sub == 0) scales[t[n] * kb_n + (k0[n] >> 7)] = s;
-            uint8_t* q = codes + t[n] * code_pitch + k0[n];
+            const int k0 = kb[n] * 128 + sub * 8;
+            if (first + n * 16 >= units || k0 >= cols) continue;
+            if (sub == 0) scales[(size_t)t[n] * kb_n + kb[n]] = s;
+            uint8_t* q = codes + t[n] * code_pitch + k0;
             if (wide_store) {  // cols (and the pitch) are multiples of 8
                 *reinterpret_cast<uint2*>(q) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (k0[n] + i < cols) q[i] = (uint8_t)(w[i >> 1] >> (8 * (i & 1)));
+                    if (k0 + i < cols) q[i] = (uint8_t)(w[i >> 1] >> (8 * (i & 1)));
             }
         }
     }
@@ -170,6 +188,7 @@ struct F8Args {
     int out_type;
     int tokens, rows, kb_n;
     int whole;         // few-token kernel: a CTA's run is whole tiles (nothing to join)
+    int chained;       // the kernel before this one on the stream is the tokens' quantisation
     float* part;       // few-token kernel: [grid][2][NT][128] partial tiles
     unsigned* done;    // few-token kernel: k blocks finished per tile (zero between launches)
     int* err;
@@ -208,6 +227,19 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     const long long tiles = (long long)row_tiles * tok_tiles;
     const long long u0 = a.whole ? tiles * blockIdx.x / gridDim.x * a.kb_n : units * blockIdx.x / gridDim.x;
     const long long u1 = a.whole ? tiles * (blockIdx.x + 1) / gridDim.x * a.kb_n : units * (blockIdx.x + 1) / gridDim.x;
+    // position of a unit, stepped along: row tile, token tile (innermost after k), k block
+    struct Pos {
+        int row, tok, kb;
+    };
+    const long long tile0 = u0 / a.kb_n;
+    const Pos begin{(int)(tile0 / tok_tiles), (int)(tile0 % tok_tiles), (int)(u0 - tile0 * a.kb_n)};
+    auto next = [&](Pos& p) {
+        if (++p.kb == a.kb_n) {
+            p.kb = 0;
+            if (++p.tok == tok_tiles) p.tok = 0, ++p.row;
+        }
+    };
+    const int head = (int)min(u1 - u0, (long long)STAGES);
 
     if (tid == 0) {
         for (int i = 0; i < STAGES; ++i) {
@@ -220,8 +252,15 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         }
         sh.failed = 0;
         fence_mbar_init();
-        tma_prefetch_map(&map_w);
+        // the first weight tiles, before anything else: the weight does not depend on the kernel before this one where that
+        // is the tokens' quantisation (which has waited for all that came before it)
         tma_prefetch_map(&map_x);
+        if (!a.chained) pdl_wait();
+        Pos p = begin;
+        for (int st = 0; st < head; ++st, next(p)) {
+            mbar_expect_tx(&sh.full[st], STAGE);
+            tma_load_2d(ring + st * STAGE, &map_w, p.kb * 128, p.row * 128, &sh.full[st]);
+        }
     }
     if (warp == 1) tmem_alloc(&sh.tmem, TMEM_COLS);
     tc5_fence_before();
@@ -232,29 +271,10 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     if (warp == 0) {
         // ---- producer: weight and token tiles of the run's units ----
         if (lane == 0) {
-            // position of a unit, stepped along: row tile, token tile (innermost after k), k block
-            struct Pos {
-                int row, tok, kb;
-            };
-            const long long tile0 = u0 / a.kb_n;
-            const Pos begin{(int)(tile0 / tok_tiles), (int)(tile0 % tok_tiles), (int)(u0 - tile0 * a.kb_n)};
-            auto next = [&](Pos& p) {
-                if (++p.kb == a.kb_n) {
-                    p.kb = 0;
-                    if (++p.tok == tok_tiles) p.tok = 0, ++p.row;
-                }
-            };
-            // the weight does not depend on the kernel before this one (the quantisation of the tokens)
-            const int head = (int)min(u1 - u0, (long long)STAGES);
             Pos p = begin;
-            for (int st = 0; st < head; ++st, next(p)) {
-                mbar_expect_tx(&sh.full[st], STAGE);
-                tma_load_2d(ring + st * STAGE, &map_w, p.kb * 128, p.row * 128, &sh.full[st]);
-            }
-            Pos px = begin;
             pdl_wait();
-            for (int st = 0; st < head; ++st, next(px))
-                tma_load_2d(ring + st * STAGE + 128 * 128, &map_x, px.kb * 128, px.tok * NT, &sh.full[st]);
+            for (int st = 0; st < head; ++st, next(p))
+                tma_load_2d(ring + st * STAGE + 128 * 128, &map_x, p.kb * 128, p.tok * NT, &sh.full[st]);
             bool ok = true;
             long long u = u0 + head;
             int st = head == STAGES ? 0 : head;
@@ -611,44 +631,28 @@ cudaError_t encode_bytes(CUtensorMap* map, const void* base, size_t rows, size_t
     return encode_tile_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, cols, pitch, box_rows, 128, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <class K>
-cudaError_t launch_after(K kernel, int grid, int threads, size_t smem, cudaStream_t st, bool overlap, const CUtensorMap& w,
-                         const CUtensorMap& x, const F8Args& a) {
-    cudaError_t e = set_max_dyn_smem((const void*)kernel, 227 * 1024);
-    if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = overlap ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, w, x, a);
-}
-
 template <int NT>
-cudaError_t launch_few(const Fp8Product& p, const F8Args& a, int grid, bool overlap, cudaStream_t st) {
+cudaError_t launch_few(const Fp8Product& p, const F8Args& a, int grid, cudaStream_t st) {
     CUtensorMap mw, mx;
     cudaError_t e = encode_bytes(&mw, p.w, p.rows, p.cols, p.cols, 128);
     if (e == cudaSuccess) e = encode_bytes(&mx, p.codes, p.tokens, p.cols, p.code_pitch, NT);
     if (e != cudaSuccess) return e;
     const size_t smem = 1024 + (size_t)few_stages(NT) * few_stage_bytes(NT) + sizeof(FewSmem<NT>);
     static_assert(1024 + few_stages(NT) * few_stage_bytes(NT) + sizeof(FewSmem<NT>) <= 227 * 1024, "shared memory");
-    return launch_after(fp8_few_kernel<NT>, grid, few_threads(NT), smem, st, overlap, mw, mx, a);
+    if ((e = set_max_dyn_smem((const void*)fp8_few_kernel<NT>, 227 * 1024)) != cudaSuccess) return e;
+    return launch_chained(fp8_few_kernel<NT>, dim3(grid), dim3(few_threads(NT)), smem, st, mw, mx, a);
 }
 
 template <class T>
-cudaError_t launch_many(const Fp8Product& p, const F8Args& a, int grid, bool overlap, cudaStream_t st) {
+cudaError_t launch_many(const Fp8Product& p, const F8Args& a, int grid, cudaStream_t st) {
     CUtensorMap mw, mx;
     cudaError_t e = encode_bytes(&mw, p.w, p.rows, p.cols, p.cols, MANY_N);
     if (e == cudaSuccess) e = encode_bytes(&mx, p.codes, p.tokens, p.cols, p.code_pitch, MANY_M);
     if (e != cudaSuccess) return e;
     constexpr size_t smem = 1024 + (size_t)MANY_STAGES * MANY_STAGE + sizeof(ManySmem);
     static_assert(smem <= 227 * 1024, "shared memory");
-    return launch_after(fp8_many_kernel<T>, grid, MANY_THREADS, smem, st, overlap, mw, mx, a);
+    if ((e = set_max_dyn_smem((const void*)fp8_many_kernel<T>, 227 * 1024)) != cudaSuccess) return e;
+    return launch_chained(fp8_many_kernel<T>, dim3(grid), dim3(MANY_THREADS), smem, st, mw, mx, a);
 }
 
 // Columns of an accumulator of the few-token kernel.
@@ -688,24 +692,36 @@ cudaError_t launch_fp8_quantize(const void* x, int type, size_t tokens, size_t c
                                 size_t code_pitch, float* scales, int sm_count, cudaStream_t st) {
     if (tokens == 0 || cols == 0) return cudaSuccess;
     const int kb_n = (int)((cols + 127) / 128);
-    const long long units = (long long)tokens * kb_n;
-    const int grid = (int)std::min<long long>((units + 16 * QU - 1) / (16 * QU), (long long)sm_count * 32);
     const size_t z = type == LQ_T_F32 ? 4 : 2;
     const bool vec = cols % 8 == 0 && (((uintptr_t)x | x_stride * z) & 15) == 0;
     const int wide = cols % 8 == 0 && (((uintptr_t)codes | code_pitch) & 7) == 0;
-    auto go = [&](auto* t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        if (vec)
-            fp8_quantize_kernel<T, true><<<grid, 256, 0, st>>>((const T*)x, (long long)x_stride, units, kb_n, (int)cols, codes,
-                                                               (long long)code_pitch, scales, wide);
-        else
-            fp8_quantize_kernel<T, false><<<grid, 256, 0, st>>>((const T*)x, (long long)x_stride, units, kb_n, (int)cols, codes,
-                                                                (long long)code_pitch, scales, wide);
-    };
-    if (type == LQ_T_F32) go((float*)nullptr);
-    else if (type == LQ_T_BF16) go((__nv_bfloat16*)nullptr);
-    else go((__half*)nullptr);
-    return cudaGetLastError();
+    const size_t most = std::max<size_t>(1, (size_t)(1 << 29) / kb_n);  // tokens whose blocks are counted in 32 bits
+    for (size_t t0 = 0; t0 < tokens; t0 += most) {
+        const int units = (int)(std::min(most, tokens - t0) * kb_n);
+        const void* xt = (const uint8_t*)x + t0 * x_stride * z;
+        uint8_t* ct = codes + t0 * code_pitch;
+        float* sc = scales + t0 * kb_n;
+        auto go = [&](auto* tag, auto vtag, auto qtag) {
+            using T = std::remove_pointer_t<decltype(tag)>;
+            constexpr int Q = decltype(qtag)::value;
+            const int grid = std::min((units + 16 * Q - 1) / (16 * Q), sm_count * 32);
+            return launch_chained(fp8_quantize_kernel<T, decltype(vtag)::value, Q>, dim3(grid), dim3(256), 0, st, (const T*)xt,
+                                  (long long)x_stride, units, kb_n, (int)cols, ct, (long long)code_pitch, sc, wide);
+        };
+        auto by_type = [&](auto vtag, auto qtag) {
+            if (type == LQ_T_F32) return go((float*)nullptr, vtag, qtag);
+            if (type == LQ_T_BF16) return go((__nv_bfloat16*)nullptr, vtag, qtag);
+            return go((__half*)nullptr, vtag, qtag);
+        };
+        using One = std::integral_constant<int, 1>;
+        using Four = std::integral_constant<int, 4>;
+        cudaError_t e;
+        if (!vec) e = by_type(std::false_type{}, One{});
+        else if (units >= sm_count * 64) e = by_type(std::true_type{}, Four{});
+        else e = by_type(std::true_type{}, One{});
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 // Partial tiles and counters of the few-token kernel.
@@ -718,7 +734,7 @@ size_t fp8_tile_count(size_t tokens, size_t rows, size_t cols, int sm_count) {
     const Way w = way_of(tokens, rows, cols, sm_count);
     return w.few && !w.whole ? ((rows + 127) / 128) * ((tokens + nt - 1) / nt) : 0;
 }
-cudaError_t launch_fp8_matmul(const Fp8Product& p, bool overlap, int sm_count, int* err, cudaStream_t st) {
+cudaError_t launch_fp8_matmul(const Fp8Product& p, bool chained, int sm_count, int* err, cudaStream_t st) {
     const int kb_n = (int)((p.cols + 127) / 128);
     F8Args a{};
     a.sx = p.scales, a.sw = p.w_scales, a.out = p.out, a.out_stride = (long long)p.out_stride, a.out_type = p.out_type;
@@ -727,18 +743,19 @@ cudaError_t launch_fp8_matmul(const Fp8Product& p, bool overlap, int sm_count, i
     const Way w = way_of(p.tokens, p.rows, p.cols, sm_count);
     const int grid = w.grid;
     a.whole = w.whole;
+    a.chained = chained;
     if (w.few) {
         const int nt = few_columns(p.tokens);
         switch (nt) {
-            case 16: return launch_few<16>(p, a, grid, overlap, st);
-            case 32: return launch_few<32>(p, a, grid, overlap, st);
-            case 64: return launch_few<64>(p, a, grid, overlap, st);
+            case 16: return launch_few<16>(p, a, grid, st);
+            case 32: return launch_few<32>(p, a, grid, st);
+            case 64: return launch_few<64>(p, a, grid, st);
         }
-        return launch_few<128>(p, a, grid, overlap, st);
+        return launch_few<128>(p, a, grid, st);
     }
-    if (p.out_type == LQ_T_F32) return launch_many<float>(p, a, grid, overlap, st);
-    if (p.out_type == LQ_T_BF16) return launch_many<__nv_bfloat16>(p, a, grid, overlap, st);
-    return launch_many<__half>(p, a, grid, overlap, st);
+    if (p.out_type == LQ_T_F32) return launch_many<float>(p, a, grid, st);
+    if (p.out_type == LQ_T_BF16) return launch_many<__nv_bfloat16>(p, a, grid, st);
+    return launch_many<__half>(p, a, grid, st);
 }
 
 }  // namespace lq

@@ -89,6 +89,22 @@ struct FmtMat {
 
 // launch_util.cu: cudaFuncAttributeMaxDynamicSharedMemorySize, set once per (device, kernel)
 cudaError_t set_max_dyn_smem(const void* func, int bytes);
+// Launch of a kernel that begins with griddepcontrol.wait (pdl_wait): its blocks may be set up while the kernel before it on
+// the stream ends.
+template <class... P, class... A>
+cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A&&... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
 cudaError_t encode_tile_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, size_t rows, size_t cols, size_t pitch,
                             int box_rows, int box_cols, CUtensorMapSwizzle swizzle);
 
@@ -217,8 +233,8 @@ struct Fp8Product {
 };
 size_t fp8_part_bytes(size_t tokens, size_t rows, size_t cols, int sm_count);
 size_t fp8_tile_count(size_t tokens, size_t rows, size_t cols, int sm_count);
-// overlap: the kernel before this one on the stream is this product's own quantisation (it may start while that ends)
-cudaError_t launch_fp8_matmul(const Fp8Product& p, bool overlap, int sm_count, int* err, cudaStream_t st);
+// chained: the kernel before this one on the stream is this product's own quantisation (it may start while that ends)
+cudaError_t launch_fp8_matmul(const Fp8Product& p, bool chained, int sm_count, int* err, cudaStream_t st);
 
 // moe_layer.cu: the whole mixture-of-experts layer for up to MOE_LAYER_MAX_TOKENS tokens, one cooperative launch
 #define MOE_LAYER_MAX_EXPERTS 256
