@@ -264,7 +264,7 @@ struct MoeLayer {
     // group of an expert; bits of the largest |value| per token / pair
     unsigned *exits, *route_done, *down_done, *group_done, *x_max, *act_max;
     int terms;                       // f16 terms per activation (filled in by the launch)
-    int n_stages, stage_bytes, scale_slots[2], finish;  // filled in by the launch
+    int n_stages, stage_bytes, scale_slots[2], finish, chunk[2], n_chunks[2];  // filled in by the launch
     int* err;
 };
 cudaError_t launch_moe_nan_scale(const MoeExpert* table, int experts, int hidden, int inter, int* found, cudaStream_t st);

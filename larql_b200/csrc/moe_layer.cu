@@ -112,11 +112,15 @@ __device__ __forceinline__ void to_f32(const Raw8& r, int type, float (&v)[8]) {
 
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(ML_CONSUMERS) : "memory"); }
 
-// Bounded polls (about a second): an mbarrier phase, and a counter that other CTAs raise to at least `target`.
+// Bounded polls (about a second): an mbarrier phase, and a counter that other CTAs raise to at least `target`.  The producer
+// and the finishers sleep between polls (LAZY): four warps polling flat out took a quarter of the integer pipe's
+// cycles from the conversions of the compute warps.
+template <bool LAZY>
 __device__ __forceinline__ bool ml_wait(uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
     for (uint32_t it = 1;; ++it) {
+        if (LAZY) __nanosleep(100);
         if (mbar_try_wait(bar, parity)) return true;
         if ((it & 255u) == 0 && clock64() - t0 > (1ll << 31)) return false;
     }
@@ -228,6 +232,7 @@ struct Walk {
     int is_down;
     uint8_t* scales;                // [slots] scales of a unit's rows
     int slots;
+    int first, end;                 // this CTA's units
 };
 
 template <int FMT>
@@ -237,17 +242,16 @@ __device__ __forceinline__ Walk walk_of(const MoeLayer& L, bool down, int n_grou
     w.slots = L.scale_slots[down];
     w.is_down = down;
     w.k = down ? L.inter : L.hidden;
-    w.chunk = chunk_cols<FMT>(w.k);
-    w.n_chunks = (w.k + w.chunk - 1) / w.chunk;
-    w.pitch = code_bytes<FMT>(stage_cols<FMT>(w.k));
-    if (!down) {
-        w.tiles = 2;
-        w.units_per_group = L.inter / 16;
-    } else {
-        // 32 rows a unit share the loads of the activations; 16 when there are too few units to even the SMs out
-        w.tiles = (long long)n_groups * (L.hidden / 32) >= 8ll * gridDim.x ? 2 : 1;
-        w.units_per_group = L.hidden / (16 * w.tiles);
-    }
+    w.chunk = L.chunk[down];
+    w.n_chunks = L.n_chunks[down];
+    w.pitch = code_bytes<FMT>(w.chunk + 32);
+    // 32 rows a down unit share the loads of the activations; 16 when there are too few units to even the SMs out
+    w.tiles = !down || n_groups * (L.hidden / 32) >= 8 * (int)gridDim.x ? 2 : 1;
+    w.units_per_group = down ? L.hidden / (16 * w.tiles) : L.inter / 16;
+    // (at most 1024 groups of 512 units, 2^10 CTAs: 32 bits hold the products)
+    const unsigned total = (unsigned)(n_groups * w.units_per_group);
+    w.first = (int)(total * blockIdx.x / gridDim.x);
+    w.end = (int)(total * (blockIdx.x + 1) / gridDim.x);
     return w;
 }
 
@@ -450,8 +454,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
         uint32_t lap = 0;   // parity of the ring's lap (an empty barrier's first wait, for parity 1, passes)
         for (int ph = 0; ph < 2 && ok; ++ph) {
             const Walk w = walk_of<FMT>(L, ph == 1, n_groups, sbuf);
-            const int total = n_groups * w.units_per_group;
-            const int ua = (int)((long long)total * blockIdx.x / gridDim.x), ub = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
+            const int ua = w.first, ub = w.end;
             if (ua >= ub) continue;
             int gi = ua / w.units_per_group, tile = ua - gi * w.units_per_group, a = -1;
             const CUtensorMap *m0 = nullptr, *m1 = nullptr;
@@ -468,7 +471,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                 }
                 const int row0 = (w.is_down ? tile * w.tiles : tile) * 16, row1 = w.is_down ? row0 + 16 : row0;
                 for (int c = 0; c < w.n_chunks; ++c, ++n) {
-                    ok = __all_sync(0xffffffffu, ml_wait(&sh.empty[st], lap ^ 1u));
+                    ok = __all_sync(0xffffffffu, ml_wait<true>(&sh.empty[st], lap ^ 1u));
                     if (!ok) break;
                     if (lane == 0) {  // (columns past the row's end arrive as zeros and count as bytes)
                         const bool with_scales = sbytes16 && c == 0;
@@ -493,7 +496,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
             }
         }
         if (!ok) {  // the copies in flight have to land before the block's shared memory goes away
-            for (int v = max(0, n - L.n_stages); v < n; ++v) ml_wait(&sh.full[v % L.n_stages], (uint32_t)(v / L.n_stages) & 1u);
+            for (int v = max(0, n - L.n_stages); v < n; ++v) ml_wait<true>(&sh.full[v % L.n_stages], (uint32_t)(v / L.n_stages) & 1u);
             sh.failed = 1;
         }
     } else {
@@ -506,8 +509,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
         for (int ph = 0; ph < 2; ++ph) {
             const Walk w = walk_of<FMT>(L, ph == 1, n_groups, sbuf);
             const int xpitch = act_pitch(w.k), srow = row_scale_bytes<FMT>(w.k);
-            const int total = n_groups * w.units_per_group;
-            const int ua = (int)((long long)total * blockIdx.x / gridDim.x), ub = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
+            const int ua = w.first, ub = w.end;
             if (ua >= ub) continue;
             int gi = ua / w.units_per_group, tile = ua - gi * w.units_per_group, a = expert_of(sh, gi, 0);
             if (!computes) {
@@ -537,7 +539,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     const MoeExpert& ex = L.table[sh.active[a]];
                     const int row = lane & 15, half = lane >> 4;
                     const float ts = ex.ts[w.is_down ? 2 : half];
-                    if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.rfull[buf], parity));
+                    if (ok) ok = __all_sync(0xffffffffu, ml_wait<true>(&sh.rfull[buf], parity));
                     const int cnt = sh.cnt;
                     // lane i keeps what belongs to token i of the group
                     float scale = 0.0f;
@@ -597,7 +599,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     cols = (cnt * terms + 7) / 8;
                     // the finishers are done with the previous group's units, the compute warps with its activations
                     for (int v = 0; v < L.finish; ++v)
-                        if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.rempty[v], v < rb ? rlap : rlap ^ 1u));
+                        if (ok) ok = __all_sync(0xffffffffu, ml_wait<false>(&sh.rempty[v], v < rb ? rlap : rlap ^ 1u));
                     consumers_sync();
                     if (tid < cnt) {
                         unsigned long long m = m0;
@@ -684,7 +686,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                 if (++slot == w.slots) slot = 0;
                 for (int c = 0; c < w.n_chunks; ++c) {
                     const int kb0 = c * (w.chunk / 32), blocks = min(w.chunk / 32, w.k / 32 - kb0);
-                    if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.full[st], lap));
+                    if (ok) ok = __all_sync(0xffffffffu, ml_wait<false>(&sh.full[st], lap));
                     // addresses of the warp's first block; the others lie at constant distances
                     const uint32_t ra = frag + (uint32_t)(st * L.stage_bytes + b0 * (F8 ? 32 : 16));
                     const uint32_t sa = s0 + (FMT == LQ_FMT_NVFP4 ? 2 * (kb0 + b0) + (t4 >> 1) : kb0 + b0), sb = sa + 8 * srow;
@@ -778,7 +780,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     if (lane == 0) ml_arrive(&sh.empty[st]);
                     if (++st == L.n_stages) st = 0, lap ^= 1u;
                 }
-                if (ok) ok = __all_sync(0xffffffffu, ml_wait(&sh.rempty[rb], rlap ^ 1u));
+                if (ok) ok = __all_sync(0xffffffffu, ml_wait<false>(&sh.rempty[rb], rlap ^ 1u));
                 float* mine = red + (rb * ML_WARPS + warp) * 2 * RED;
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
@@ -877,6 +879,11 @@ cudaError_t launch_layer(MoeLayer L, int sm_count, cudaStream_t st) {
     if (p.stages == 0) return cudaErrorInvalidConfiguration;
     L.n_stages = p.stages, L.finish = p.finish, L.scale_slots[0] = p.slots[0], L.scale_slots[1] = p.slots[1];
     L.stage_bytes = stage_size<FMT>(L.hidden, L.inter);
+    for (int i = 0; i < 2; ++i) {
+        const int k = i ? L.inter : L.hidden;
+        L.chunk[i] = chunk_cols<FMT>(k);
+        L.n_chunks[i] = (k + L.chunk[i] - 1) / L.chunk[i];
+    }
     const void* fn = (const void*)moe_layer_kernel<FMT, NT>;
     cudaError_t e = set_max_dyn_smem(fn, 227 * 1024);
     if (e != cudaSuccess) return e;
