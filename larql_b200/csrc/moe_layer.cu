@@ -52,6 +52,7 @@ struct MlSmem {
     float unscale[16];          // per token of the group: the power of two its values were divided by
     int gtok[16], gpair[16];    // the group's tokens and (token, slot) pairs
     int n_groups, cnt;
+    unsigned x_bits;            // one token: its largest |value|
     int active[MOE_LAYER_MAX_EXPERTS];
     int gpre[MOE_LAYER_MAX_EXPERTS + 1];     // groups before the active expert
     unsigned mask[MOE_LAYER_MAX_EXPERTS][2]; // tokens that chose the expert
@@ -255,6 +256,43 @@ __device__ __forceinline__ Walk walk_of(const MoeLayer& L, bool down, int n_grou
     return w;
 }
 
+// Eight activations times a power of two, into columns of f16: one term, or a value and its rest.
+template <int FMT>
+__device__ __forceinline__ void put_columns(const float (&v)[8], float scale, int terms, uint8_t* dst, int xpitch, int k) {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const float x0 = v[2 * q] * scale, x1 = v[2 * q + 1] * scale;
+        const __half2 h = __floats2half2_rn(x0, x1);
+        const float2 f = __half22float2(h);
+        const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
+        hi[q] = *reinterpret_cast<const uint32_t*>(&h);
+        lo[q] = *reinterpret_cast<const uint32_t*>(&l);
+    }
+    if (FMT == LQ_FMT_FP8_B128) {
+        // a lane's 8 columns of a block: 4 of either half (what its two code words hold)
+        uint8_t* q = dst + 2 * (k & ~31) + ((k & 15) >> 2) * 16 + ((k >> 4) & 1) * 8;
+        *reinterpret_cast<uint2*>(q) = make_uint2(hi[0], hi[1]);
+        *reinterpret_cast<uint2*>(q + 16) = make_uint2(hi[2], hi[3]);
+        if (terms == 2) {
+            *reinterpret_cast<uint2*>(q + xpitch) = make_uint2(lo[0], lo[1]);
+            *reinterpret_cast<uint2*>(q + xpitch + 16) = make_uint2(lo[2], lo[3]);
+        }
+    } else {
+        *reinterpret_cast<uint4*>(dst + 2 * k) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (terms == 2) *reinterpret_cast<uint4*>(dst + xpitch + 2 * k) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+}
+// The power of two that brings values of at most |bits| to [2^14, 2^15), and the one that takes it back (kept where both
+// are normal numbers).  An infinity makes the whole token NaN, like a NaN.
+__device__ __forceinline__ float down_scale(uint32_t bits) {
+    const int e = min(max((int)(bits >> 23), 15), 254);
+    return bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(127 + 14 + 127 - e) << 23);
+}
+__device__ __forceinline__ float up_scale(uint32_t bits) {
+    return __uint_as_float((uint32_t)(min(max((int)(bits >> 23), 15), 254) - 14) << 23);
+}
+
 // Active expert of group gi (groups are numbered expert by expert).
 __device__ __forceinline__ int expert_of(const MlSmem& sh, int gi, int from) {
     while (gi >= sh.gpre[from + 1]) ++from;
@@ -263,8 +301,8 @@ __device__ __forceinline__ int expert_of(const MlSmem& sh, int gi, int from) {
 
 // The experts of token t, into shared memory: a warp takes top_e rounds of the largest logit left, the lowest index
 // among equals.  Every CTA does it for every token (a publication by one would cost the others a microsecond more).
+template <int PER>
 __device__ void route_token(const MoeLayer& L, MlSmem& sh, int t, int lane) {
-    constexpr int PER = MOE_LAYER_MAX_EXPERTS / 32;
     const int E = L.experts, K = L.top_e;
     uint32_t key[PER];  // logits as integers of the same order; 0: taken (a NaN, 1, comes last: the weights are NaN then)
     float mx = -INFINITY, sum = 0.0f, mine = 0.0f;
@@ -347,9 +385,11 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
             mbar_init(&sh.rempty[i], 1);
         }
         sh.failed = 0;
+        sh.x_bits = 0;
         fence_mbar_init();
     }
     for (int i = tid; i < 2 * E; i += ML_THREADS) sh.mask[i >> 1][i & 1] = 0;
+    __syncthreads();
 
     // ---- route: an item is one token's product with one expert's row, worked on by as many warps as there are to spare ----
     {
@@ -410,6 +450,33 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                 add_release(L.route_done, 1u);
             }
         }
+        if (T == 1) {
+            // one token: every group's activations are the same; make its columns now, while the other CTAs' products arrive
+            Raw8 raw[2];
+            float v[8];
+            uint32_t m = 0;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int k = (tid + q * ML_THREADS) * 8;
+                if (k >= L.hidden) continue;
+                raw[q] = x_wide ? ld8<true>(L.x, L.type, k) : ld8<false>(L.x, L.type, k);
+                to_f32(raw[q], L.type, v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+            }
+            m = __reduce_max_sync(0xffffffffu, m);
+            if (lane == 0) atomicMax(&sh.x_bits, m);
+            __syncthreads();
+            const uint32_t bits = sh.x_bits;
+            if (tid == 0) sh.unscale[0] = up_scale(bits);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int k = (tid + q * ML_THREADS) * 8;
+                if (k >= L.hidden) continue;
+                to_f32(raw[q], L.type, v);
+                put_columns<FMT>(v, down_scale(bits), L.terms, xs, act_pitch(L.hidden), k);
+            }
+        }
         if (tid == 0 && !wait_count(L.route_done, (unsigned)items)) sh.failed = 1;
     }
     __syncthreads();
@@ -417,7 +484,11 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
         if (tid == 0) set_err(L.err, DEV_ERR_TMA_TIMEOUT);
         return;
     }
-    for (int t = warp; t < T; t += ML_THREADS / 32) route_token(L, sh, t, lane);
+    for (int t = warp; t < T; t += ML_THREADS / 32) {
+        if (E <= 32) route_token<1>(L, sh, t, lane);
+        else if (E <= 64) route_token<2>(L, sh, t, lane);
+        else route_token<MOE_LAYER_MAX_EXPERTS / 32>(L, sh, t, lane);
+    }
     __syncthreads();
     if (warp == 0) {  // the chosen experts in order, and their token groups
         int n = 0, groups = 0;
@@ -617,7 +688,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     // the warps share the rows out: `per` warps a token
                     const int per = cnt >= 9 ? 1 : (cnt >= 5 ? 2 : (cnt >= 3 ? 4 : (cnt == 2 ? 8 : 16)));
                     const int i = warp / per, part = (warp % per) * 32 + lane;
-                    if (i < cnt) {
+                    if (i < cnt && !(T == 1 && ph == 0)) {  // (a single token's columns were made while the routing was on its way)
                         const void* src = w.is_down ? L.act : L.x;
                         const int type = w.is_down ? LQ_T_F32 : L.type;
                         const bool wide = w.is_down || x_wide;
@@ -627,41 +698,15 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
 #pragma unroll
                         for (int q = 0; q < 2; ++q)
                             if (part * 8 + q * per * 256 < w.k) next[q] = fetch(part * 8 + q * per * 256);
-                        // exponent of the largest value -> 2^14 (kept where both powers of two are normal numbers)
                         const unsigned bits = __ldcg(w.is_down ? L.act_max + sh.gpair[i] : L.x_max + sh.gtok[i]);
-                        const int ex2 = min(max((int)(bits >> 23), 15), 254);
-                        // (an infinity makes the whole token NaN, like a NaN)
-                        const float down = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(127 + 14 + 127 - ex2) << 23);
-                        if (part == 0) sh.unscale[i] = __uint_as_float((uint32_t)(ex2 - 14) << 23);
-                        uint8_t* dst = xs + (size_t)(i * terms) * xpitch;
+                        const float scale = down_scale(bits);
+                        if (part == 0) sh.unscale[i] = up_scale(bits);
                         for (int k = part * 8; k < w.k; k += per * 256) {
                             float v[8];
                             to_f32(next[0], type, v);
                             next[0] = next[1];
                             if (k + per * 512 < w.k) next[1] = fetch(k + per * 512);
-                            uint32_t hi[4], lo[4];
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                const float x0 = v[2 * q] * down, x1 = v[2 * q + 1] * down;
-                                const __half2 h = __floats2half2_rn(x0, x1);
-                                const float2 f = __half22float2(h);
-                                const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
-                                hi[q] = *reinterpret_cast<const uint32_t*>(&h);
-                                lo[q] = *reinterpret_cast<const uint32_t*>(&l);
-                            }
-                            if (FMT == LQ_FMT_FP8_B128) {
-                                // a lane's 8 columns of a block: 4 of either half (what its two code words hold)
-                                uint8_t* q = dst + 2 * (k & ~31) + ((k & 15) >> 2) * 16 + ((k >> 4) & 1) * 8;
-                                *reinterpret_cast<uint2*>(q) = make_uint2(hi[0], hi[1]);
-                                *reinterpret_cast<uint2*>(q + 16) = make_uint2(hi[2], hi[3]);
-                                if (terms == 2) {
-                                    *reinterpret_cast<uint2*>(q + xpitch) = make_uint2(lo[0], lo[1]);
-                                    *reinterpret_cast<uint2*>(q + xpitch + 16) = make_uint2(lo[2], lo[3]);
-                                }
-                            } else {
-                                *reinterpret_cast<uint4*>(dst + 2 * k) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                                if (terms == 2) *reinterpret_cast<uint4*>(dst + xpitch + 2 * k) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                            }
+                            put_columns<FMT>(v, scale, terms, xs + (size_t)(i * terms) * xpitch, xpitch, k);
                         }
                     }
                     consumers_sync();
