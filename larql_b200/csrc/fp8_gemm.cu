@@ -195,17 +195,15 @@ struct F8Args {
 };
 
 // ------------------------------------------------------------ few tokens ----
-constexpr int FEW_BUFS = 4;  // accumulator buffers in tensor memory
-
 constexpr int few_stage_bytes(int nt) { return 128 * 128 + nt * 128; }
-constexpr int few_stages(int nt) { return nt <= 16 ? 11 : (nt <= 32 ? 10 : (nt <= 64 ? 8 : 6)); }
+constexpr int few_stages(int nt) { return nt <= 16 ? 11 : (nt <= 32 ? 10 : (nt <= 64 ? 8 : 4)); }  // (an accumulator of nt columns each)
 constexpr int few_promo_warps(int nt) { return nt <= 64 ? nt / 4 : 16; }  // 16 columns a warp, 32 at the widest
 constexpr int few_threads(int nt) { return 128 + 32 * few_promo_warps(nt); }  // (two warps idle: a warp reads the TMEM lanes of its rank of 4)
 
 template <int NT>
 struct FewSmem {
-    uint64_t full[few_stages(NT)], empty[few_stages(NT)];
-    uint64_t acc_full[FEW_BUFS], acc_empty[FEW_BUFS];
+    // a stage is its tiles and its accumulator: loaded (full), multiplied (done), added up by every promoting warp (empty)
+    uint64_t full[few_stages(NT)], done[few_stages(NT)], empty[few_stages(NT)];
     alignas(16) float sx[few_promo_warps(NT)][2][NT];  // the scales of a k block's tokens, per warp
     uint32_t tmem;
     int failed;
@@ -217,7 +215,8 @@ __global__ void __launch_bounds__(few_threads(NT), 1)
 fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const F8Args a) {
     constexpr int STAGES = few_stages(NT), STAGE = few_stage_bytes(NT), PW = few_promo_warps(NT);
     constexpr int COLS = NT * 4 / PW;  // columns (tokens) per promoting warp: all of them with one warpgroup
-    constexpr uint32_t TMEM_COLS = NT * FEW_BUFS < 32 ? 32 : NT * FEW_BUFS;
+    constexpr uint32_t TMEM_COLS = NT * STAGES <= 256 ? 256 : 512;
+    static_assert(NT * STAGES <= 512, "tensor memory");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     FewSmem<NT>& sh = *reinterpret_cast<FewSmem<NT>*>(ring + STAGES * STAGE);
@@ -244,11 +243,8 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     if (tid == 0) {
         for (int i = 0; i < STAGES; ++i) {
             mbar_init(&sh.full[i], 1);
-            mbar_init(&sh.empty[i], 1);
-        }
-        for (int i = 0; i < FEW_BUFS; ++i) {
-            mbar_init(&sh.acc_full[i], 1);
-            mbar_init(&sh.acc_empty[i], PW * 32);
+            mbar_init(&sh.done[i], 1);
+            mbar_init(&sh.empty[i], PW);
         }
         sh.failed = 0;
         fence_mbar_init();
@@ -270,7 +266,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 
     if (warp == 0) {
         // ---- producer: weight and token tiles of the run's units ----
-        if (lane == 0) {
+        if (elect_one()) {
             Pos p = begin;
             pdl_wait();
             for (int st = 0; st < head; ++st, next(p))
@@ -299,28 +295,25 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         }
         __syncwarp();
     } else if (warp == 1) {
-        // ---- tensor core: one accumulator buffer per k block ----
-        bool ok = true;
-        int st = 0, buf = 0;
-        uint32_t lap = 0, blap = 0;
-        for (long long u = u0; u < u1; ++u) {
-            ok = mbar_wait(&sh.full[st], lap);
-            if (ok) ok = mbar_wait(&sh.acc_empty[buf], blap ^ 1u);  // (the first lap's wait passes)
-            if (!__all_sync(0xffffffffu, ok)) break;
-            tc5_fence_after();
-            if (elect_one()) {
-                const uint32_t sa = smem_u32(ring + st * STAGE), sb = sa + 128 * 128;
+        // ---- tensor core: one thread, one wait and one commit a block (each costs it a hundred cycles or two) ----
+        if (elect_one()) {
+            const uint64_t da = sw128_desc(smem_u32(ring)), db = sw128_desc(smem_u32(ring) + 128 * 128);
+            int st = 0;
+            uint32_t lap = 0;
+            for (long long u = u0; u < u1; ++u) {
+                if (!mbar_wait(&sh.full[st], lap)) {
+                    sh.failed = 1;
+                    break;
+                }
+                tc5_fence_after();  // (the accumulator's reads: before the arrivals that let the stage be filled again)
+                const uint64_t at = (uint64_t)(st * (STAGE >> 4));
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    umma_f8(tmem + buf * NT, sw128_desc(sa + 32 * j), sw128_desc(sb + 32 * j), f8_idesc(128, NT), j > 0);
-                umma_commit1(&sh.empty[st]);
-                umma_commit1(&sh.acc_full[buf]);
+                for (int j = 0; j < 4; ++j) umma_f8(tmem + st * NT, da + at + 2 * j, db + at + 2 * j, f8_idesc(128, NT), j > 0);
+                umma_commit1(&sh.done[st]);
+                if (++st == STAGES) st = 0, lap ^= 1u;
             }
-            __syncwarp();
-            if (++st == STAGES) st = 0, lap ^= 1u;
-            if (++buf == FEW_BUFS) buf = 0, blap ^= 1u;
         }
-        if (!__all_sync(0xffffffffu, ok) && lane == 0) sh.failed = 1;
+        __syncwarp();
     } else if (warp >= 4) {
         // ---- promotion: thread = row of the weight (TMEM lane); COLS tokens ----
         pdl_wait();  // the tokens' scales
@@ -329,7 +322,10 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         float acc[COLS];
         bool ok = true;
         long long u = u0;
-        int n = 0;
+        int st = 0;
+        uint32_t lap = 0;
+        constexpr int AHEAD = 4;
+        static_assert(COLS <= 32, "a lane's token");
         // (a wait that ran out is not waited for again, but the run is walked to its end: the other warps of the
         // block count on this one at the named barriers, and the tiles' counters have to come out even)
         while (u < u1) {
@@ -338,48 +334,49 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             const int kb_b = (int)min((long long)a.kb_n, kb_a + (u1 - u));
             const int row0 = (int)(tile / tok_tiles) * 128, tok0 = (int)(tile % tok_tiles) * NT;
             const float* swp = a.sw + (size_t)(row0 >> 7) * a.kb_n;
-            float nx[(COLS + 31) / 32], nw = swp[kb_a];
-            auto fetch = [&](int kb) {
-#pragma unroll
-                for (int i = 0; i < (COLS + 31) / 32; ++i) {
-                    const int c = col0 + i * 32 + lane;
-                    nx[i] = (i * 32 + lane < COLS && tok0 + c < a.tokens) ? a.sx[(size_t)(tok0 + c) * a.kb_n + kb] : 0.0f;
-                }
+            // scales are fetched AHEAD blocks before their use: a block passes in less than a load from L2 takes
+            float nx[AHEAD], nw[AHEAD];
+            auto fetch = [&](int kb, float& x, float& w) {
+                w = 0.0f, x = 0.0f;
+                if (kb >= kb_b) return;
+                w = swp[kb];
+                if (lane < COLS && tok0 + col0 + lane < a.tokens) x = a.sx[(size_t)(tok0 + col0 + lane) * a.kb_n + kb];
             };
-            fetch(kb_a);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) fetch(kb_a + i, nx[i], nw[i]);
 #pragma unroll
             for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
-            for (int kb = kb_a; kb < kb_b; ++kb, ++n) {
-                const int buf = n % FEW_BUFS;
-                float* sxs = sh.sx[pw][n & 1];
+            for (int kb0 = kb_a; kb0 < kb_b; kb0 += AHEAD)
 #pragma unroll
-                for (int i = 0; i < (COLS + 31) / 32; ++i)
-                    if (i * 32 + lane < COLS) sxs[i * 32 + lane] = nx[i] * nw;
-                __syncwarp();
-                if (kb + 1 < kb_b) {
-                    nw = swp[kb + 1];
-                    fetch(kb + 1);
-                }
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[buf], (uint32_t)(n / FEW_BUFS) & 1u));
-                tc5_fence_after();
-                uint32_t v[2][16];  // a chunk is read while the one before it is added up
-                tmem_load16(tbase + buf * NT, v[0]);
+                for (int i = 0; i < AHEAD; ++i) {
+                    const int kb = kb0 + i;
+                    if (kb >= kb_b) break;
+                    float* sxs = sh.sx[pw][i & 1];
+                    if (lane < COLS) sxs[lane] = nx[i] * nw[i];
+                    __syncwarp();
+                    fetch(kb + AHEAD, nx[i], nw[i]);
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.done[st], lap));
+                    tc5_fence_after();
+                    uint32_t v[2][16];  // a chunk is read while the one before it is added up
+                    tmem_load16(tbase + st * NT, v[0]);
 #pragma unroll
-                for (int c = 0; c < COLS / 16; ++c) {
-                    tmem_wait16(v[c & 1]);
-                    if (c + 1 < COLS / 16) tmem_load16(tbase + buf * NT + (c + 1) * 16, v[(c + 1) & 1]);
+                    for (int c = 0; c < COLS / 16; ++c) {
+                        tmem_wait16(v[c & 1]);
+                        if (c + 1 < COLS / 16) tmem_load16(tbase + st * NT + (c + 1) * 16, v[(c + 1) & 1]);
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(sxs + c * 16 + i);
-                        acc[c * 16 + i] = fmaf(__uint_as_float(v[c & 1][i]), f.x, acc[c * 16 + i]);
-                        acc[c * 16 + i + 1] = fmaf(__uint_as_float(v[c & 1][i + 1]), f.y, acc[c * 16 + i + 1]);
-                        acc[c * 16 + i + 2] = fmaf(__uint_as_float(v[c & 1][i + 2]), f.z, acc[c * 16 + i + 2]);
-                        acc[c * 16 + i + 3] = fmaf(__uint_as_float(v[c & 1][i + 3]), f.w, acc[c * 16 + i + 3]);
+                        for (int q = 0; q < 16; q += 4) {
+                            const float4 f = *reinterpret_cast<const float4*>(sxs + c * 16 + q);
+                            acc[c * 16 + q] = fmaf(__uint_as_float(v[c & 1][q]), f.x, acc[c * 16 + q]);
+                            acc[c * 16 + q + 1] = fmaf(__uint_as_float(v[c & 1][q + 1]), f.y, acc[c * 16 + q + 1]);
+                            acc[c * 16 + q + 2] = fmaf(__uint_as_float(v[c & 1][q + 2]), f.z, acc[c * 16 + q + 2]);
+                            acc[c * 16 + q + 3] = fmaf(__uint_as_float(v[c & 1][q + 3]), f.w, acc[c * 16 + q + 3]);
+                        }
                     }
+                    tc5_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_one(&sh.empty[st]);
+                    if (++st == STAGES) st = 0, lap ^= 1u;
                 }
-                tc5_fence_before();
-                mbar_arrive_one(&sh.acc_empty[buf]);
-            }
             u += kb_b - kb_a;
             const int row = row0 + quarter * 32 + lane;
             if (kb_a == 0 && kb_b == a.kb_n) {
@@ -508,7 +505,7 @@ fp8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     pdl_wait();
 
     if (warp == 0) {
-        if (lane == 0) {
+        if (elect_one()) {
             bool ok = true;
             int n = 0;
             for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
@@ -533,28 +530,28 @@ fp8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         }
         __syncwarp();
     } else if (warp == 1) {
-        bool ok = true;
-        int n = 0;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
-            for (int kb = 0; kb < a.kb_n; ++kb, ++n) {
-                const int st = n % MANY_STAGES, buf = n & 1;
-                ok = mbar_wait(&sh.full[st], (uint32_t)(n / MANY_STAGES) & 1u);
-                if (ok && n >= 2) ok = mbar_wait(&sh.acc_empty[buf], (uint32_t)(n / 2 - 1) & 1u);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc5_fence_after();
-                if (elect_one()) {
-                    const uint32_t sa = smem_u32(ring + st * MANY_STAGE), sb = sa + MANY_M * 128;
+        if (elect_one()) {
+            const uint64_t da = sw128_desc(smem_u32(ring)), db = sw128_desc(smem_u32(ring) + MANY_M * 128);
+            bool ok = true;
+            int st = 0;
+            uint32_t lap = 0, n = 0;
+            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+                for (int kb = 0; kb < a.kb_n; ++kb, ++n) {
+                    const uint32_t buf = n & 1;
+                    ok = mbar_wait(&sh.acc_empty[buf], ((n >> 1) & 1u) ^ 1u) && mbar_wait(&sh.full[st], lap);  // (the first lap's wait passes)
+                    if (!ok) break;
+                    tc5_fence_after();
+                    const uint64_t at = (uint64_t)(st * (MANY_STAGE >> 4));
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        umma_f8(tmem + buf * MANY_N, sw128_desc(sa + 32 * j), sw128_desc(sb + 32 * j),
-                                f8_idesc(MANY_M, MANY_N), j > 0);
+                        umma_f8(tmem + buf * MANY_N, da + at + 2 * j, db + at + 2 * j, f8_idesc(MANY_M, MANY_N), j > 0);
                     umma_commit1(&sh.empty[st]);
                     umma_commit1(&sh.acc_full[buf]);
+                    if (++st == MANY_STAGES) st = 0, lap ^= 1u;
                 }
-                __syncwarp();
-            }
-        if (!ok && lane == 0) sh.failed = 1;
+            if (!ok) sh.failed = 1;
+        }
+        __syncwarp();
     } else if (warp >= 4) {
         // thread = token (TMEM lane), 64 rows of the weight (of one row of scale blocks)
         constexpr int COLS = 64;
