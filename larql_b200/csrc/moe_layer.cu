@@ -519,32 +519,34 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
     const int n_groups = sh.n_groups;
 
     if (warp == ML_WARPS) {
-        // ---- producer: the rows of both phases' units, in order ----
-        bool ok = true;
-        int n = 0, st = 0;  // stages so far, the ring's next place
-        uint32_t lap = 0;   // parity of the ring's lap (an empty barrier's first wait, for parity 1, passes)
-        for (int ph = 0; ph < 2 && ok; ++ph) {
-            const Walk w = walk_of<FMT>(L, ph == 1, n_groups, sbuf);
-            const int ua = w.first, ub = w.end;
-            if (ua >= ub) continue;
-            int gi = ua / w.units_per_group, tile = ua - gi * w.units_per_group, a = -1;
-            const CUtensorMap *m0 = nullptr, *m1 = nullptr;
-            const uint8_t *sc0 = nullptr, *sc1 = nullptr;
-            int slot = 0;
-            const uint32_t sbytes16 = 16u * row_scale_bytes<FMT>(w.k), code16 = 16u * w.pitch;
-            for (int u = ua; u < ub && ok; ++u) {
-                if (a < 0 || tile == w.units_per_group) {
-                    if (a >= 0) ++gi, tile = 0;
-                    a = expert_of(sh, gi, max(a, 0));
-                    const MoeExpert& ex = L.table[sh.active[a]];
-                    m0 = &ex.map[w.is_down ? 2 : 0], m1 = &ex.map[w.is_down ? 2 : 1];
-                    sc0 = ex.scales[w.is_down ? 2 : 0], sc1 = ex.scales[w.is_down ? 2 : 1];
-                }
-                const int row0 = (w.is_down ? tile * w.tiles : tile) * 16, row1 = w.is_down ? row0 + 16 : row0;
-                for (int c = 0; c < w.n_chunks; ++c, ++n) {
-                    ok = __all_sync(0xffffffffu, ml_wait<true>(&sh.empty[st], lap ^ 1u));
-                    if (!ok) break;
-                    if (lane == 0) {  // (columns past the row's end arrive as zeros and count as bytes)
+        // ---- producer: the rows of both phases' units, in order, by one elected thread (behind a branch on the lane each copy takes
+        // several times as long: its operands have to be the same in the whole warp) ----
+        if (elect_one()) {
+            bool ok = true;
+            int n = 0, st = 0;  // stages so far, the ring's next place
+            uint32_t lap = 0;   // parity of the ring's lap (an empty barrier's first wait, for parity 1, passes)
+            for (int ph = 0; ph < 2 && ok; ++ph) {
+                const Walk w = walk_of<FMT>(L, ph == 1, n_groups, sbuf);
+                const int ua = w.first, ub = w.end;
+                if (ua >= ub) continue;
+                int gi = ua / w.units_per_group, tile = ua - gi * w.units_per_group, a = -1;
+                const CUtensorMap *m0 = nullptr, *m1 = nullptr;
+                const uint8_t *sc0 = nullptr, *sc1 = nullptr;
+                int slot = 0;
+                const uint32_t sbytes16 = 16u * row_scale_bytes<FMT>(w.k), code16 = 16u * w.pitch;
+                for (int u = ua; u < ub && ok; ++u) {
+                    if (a < 0 || tile == w.units_per_group) {
+                        if (a >= 0) ++gi, tile = 0;
+                        a = expert_of(sh, gi, max(a, 0));
+                        const MoeExpert& ex = L.table[sh.active[a]];
+                        m0 = &ex.map[w.is_down ? 2 : 0], m1 = &ex.map[w.is_down ? 2 : 1];
+                        sc0 = ex.scales[w.is_down ? 2 : 0], sc1 = ex.scales[w.is_down ? 2 : 1];
+                    }
+                    const int row0 = (w.is_down ? tile * w.tiles : tile) * 16, row1 = w.is_down ? row0 + 16 : row0;
+                    for (int c = 0; c < w.n_chunks; ++c, ++n) {
+                        ok = ml_wait<true>(&sh.empty[st], lap ^ 1u);
+                        if (!ok) break;
+                        // (columns past the row's end arrive as zeros and count as bytes)
                         const bool with_scales = sbytes16 && c == 0;
                         mbar_expect_tx(&sh.full[st], (code16 + (with_scales ? sbytes16 : 0u)) * w.tiles);
                         uint8_t* dst = ring + (size_t)st * L.stage_bytes;
@@ -558,18 +560,18 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                             tma_bulk_g2s(sd, sc0 + (size_t)(row0 >> 4) * sbytes16, sbytes16, &sh.full[st]);
                             if (w.tiles == 2) tma_bulk_g2s(sd + sbytes16, sc1 + (size_t)(row1 >> 4) * sbytes16, sbytes16, &sh.full[st]);
                         }
+                        if (++st == L.n_stages) st = 0, lap ^= 1u;
                     }
-                    __syncwarp();
-                    if (++st == L.n_stages) st = 0, lap ^= 1u;
+                    ++tile;
+                    if (++slot == w.slots) slot = 0;
                 }
-                ++tile;
-                if (++slot == w.slots) slot = 0;
+            }
+            if (!ok) {  // the copies in flight have to land before the block's shared memory goes away
+                for (int v = max(0, n - L.n_stages); v < n; ++v) ml_wait<true>(&sh.full[v % L.n_stages], (uint32_t)(v / L.n_stages) & 1u);
+                sh.failed = 1;
             }
         }
-        if (!ok) {  // the copies in flight have to land before the block's shared memory goes away
-            for (int v = max(0, n - L.n_stages); v < n; ++v) ml_wait<true>(&sh.full[v % L.n_stages], (uint32_t)(v / L.n_stages) & 1u);
-            sh.failed = 1;
-        }
+        __syncwarp();
     } else {
         // ---- compute warps and finishers walk the same units ----
         const bool computes = warp < ML_WARPS;
