@@ -652,35 +652,40 @@ cudaError_t launch_many(const Fp8Product& p, const F8Args& a, int grid, cudaStre
     return launch_chained(fp8_many_kernel<T>, dim3(grid), dim3(MANY_THREADS), smem, st, mw, mx, a);
 }
 
-// Columns of an accumulator of the few-token kernel.
-int few_columns(size_t tokens) { return tokens <= 16 ? 16 : (tokens <= 32 ? 32 : (tokens <= 64 ? 64 : 128)); }
-
-// How a product runs, from estimates in microseconds (fitted to 18 shapes of 1 to 4096 tokens): a k block of a few-token
-// tile takes an SM 0.30 to 0.75 by its columns, or the memory the time of its 16 KB; joining pieces of tiles costs 3.5
-// and 0.11 per column; a k block of a 128 x 256 tile of the other kernel takes 0.55.  Measured: 16 tokens x 28672 ->
-// 8192: spread 53, whole tiles 76, the other kernel 122 us; 1 x 3840 -> 15360: 25, 19, 25; 250 x 2880 -> 2880: 31, 23,
-// 23; 128 x 28672 -> 8192: 102, 177, 135; 1024 x 8192 -> 8192: 200, 213, 92.
+// How a product runs, from estimates in microseconds (fitted to 23 shapes of 1 to 1024 tokens): a k block of a few-token
+// tile takes an SM 0.235 to 0.68 by its columns, or the memory the time of its 16 KB; joining pieces of tiles costs 3.5,
+// 0.11 per column and 0.45 per piece of a tile; a k block of a 128 x 256 tile of the other kernel takes 0.60.  Measured,
+// quantisation included, whole tiles | tiles spread over the grid | the other kernel:
+//   1 x 3840 -> 15360    16 columns 14.7 | 19.4 | 20.8
+//   16 x 28672 -> 8192   16 columns 51.5 | 49.9 | 105
+//   64 x 2880 -> 2880    16 columns 10.7 | 16.7, 32 columns 11.3 | 16.3, 64 columns 13.1 | 19.7, 16.5
+//   64 x 8192 -> 28672   64 columns 59.8 | 55.9 | 49.7
+//   128 x 28672 -> 8192  64 columns 96.5 | 100, 128 columns 183 | 108 | 144
+//   250 x 2880 -> 2880   32 columns 20.6 | 22.7, 64 columns 14.6 | 21.4, 128 columns 20.3 | 29.3 | 20.7
+//   512 x 8192 -> 8192   64 columns 107 | 104, 128 columns 100 | 102 | 45.5
 struct Way {
-    bool few, whole;
+    int nt;  // columns of the few-token kernel's accumulators, 0: the other kernel
+    bool whole;
     int grid;
+    double us;
 };
 Way way_of(size_t tokens, size_t rows, size_t cols, int sm_count) {
-    const double kb = (double)((cols + 127) / 128), sms = sm_count;
-    const int nt = few_columns(tokens);
-    const double tiles = (double)((tokens + nt - 1) / nt) * (double)((rows + 127) / 128), units = tiles * kb;
-    const double memory = (double)((rows + 127) / 128) * kb * 0.00264;
-    const double unit = nt <= 32 ? 0.30 : (nt == 64 ? 0.38 : 0.75);
-    const double whole = std::max(memory, std::ceil(tiles / sms) * kb * unit);
-    const double spread = std::max(memory, std::ceil(units / sms) * unit) + 3.5 + 0.11 * nt;
-    Way w;
-    w.whole = whole <= spread;
-    w.few = true;
-    w.grid = (int)std::min(w.whole ? tiles : units, sms);
-    if (tokens > 64) {
-        const double t2 = (double)((tokens + MANY_M - 1) / MANY_M) * (double)((rows + MANY_N - 1) / MANY_N);
-        if (std::ceil(t2 / sms) * kb * 0.55 < std::min(whole, spread)) w = Way{false, true, (int)std::min(t2, sms)};
+    const double kb = (double)((cols + 127) / 128), sms = sm_count, row_tiles = (double)((rows + 127) / 128);
+    const double memory = row_tiles * kb * 0.00264;
+    Way best{};
+    auto take = [&](const Way& w) {
+        if (best.grid == 0 || w.us < best.us) best = w;
+    };
+    for (int nt = 16; nt <= 128; nt *= 2) {
+        const double tiles = (double)((tokens + nt - 1) / nt) * row_tiles, units = tiles * kb;
+        const double unit = nt == 16 ? 0.235 : (nt == 32 ? 0.27 : (nt == 64 ? 0.40 : 0.68));
+        take(Way{nt, true, (int)std::min(tiles, sms), std::max(memory, std::ceil(tiles / sms) * kb * unit)});
+        take(Way{nt, false, (int)std::min(units, sms), std::max(memory, std::ceil(units / sms) * unit) + 3.5 + 0.11 * nt + 0.45 * sms / tiles});
+        if ((size_t)nt >= tokens) break;
     }
-    return w;
+    const double tiles = (double)((tokens + MANY_M - 1) / MANY_M) * (double)((rows + MANY_N - 1) / MANY_N);
+    take(Way{0, true, (int)std::min(tiles, sms), std::max(memory, std::ceil(tiles / sms) * kb * 0.60)});
+    return best;
 }
 
 }  // namespace
@@ -724,12 +729,11 @@ cudaError_t launch_fp8_quantize(const void* x, int type, size_t tokens, size_t c
 // Partial tiles and counters of the few-token kernel.
 size_t fp8_part_bytes(size_t tokens, size_t rows, size_t cols, int sm_count) {
     const Way w = way_of(tokens, rows, cols, sm_count);
-    return w.few && !w.whole ? (size_t)w.grid * 2 * few_columns(tokens) * 128 * 4 : 0;
+    return w.whole ? 0 : (size_t)w.grid * 2 * w.nt * 128 * 4;
 }
 size_t fp8_tile_count(size_t tokens, size_t rows, size_t cols, int sm_count) {
-    const size_t nt = (size_t)few_columns(tokens);
     const Way w = way_of(tokens, rows, cols, sm_count);
-    return w.few && !w.whole ? ((rows + 127) / 128) * ((tokens + nt - 1) / nt) : 0;
+    return w.whole ? 0 : ((rows + 127) / 128) * ((tokens + w.nt - 1) / w.nt);
 }
 cudaError_t launch_fp8_matmul(const Fp8Product& p, bool chained, int sm_count, int* err, cudaStream_t st) {
     const int kb_n = (int)((p.cols + 127) / 128);
@@ -741,14 +745,11 @@ cudaError_t launch_fp8_matmul(const Fp8Product& p, bool chained, int sm_count, i
     const int grid = w.grid;
     a.whole = w.whole;
     a.chained = chained;
-    if (w.few) {
-        const int nt = few_columns(p.tokens);
-        switch (nt) {
-            case 16: return launch_few<16>(p, a, grid, st);
-            case 32: return launch_few<32>(p, a, grid, st);
-            case 64: return launch_few<64>(p, a, grid, st);
-        }
-        return launch_few<128>(p, a, grid, st);
+    switch (w.nt) {
+        case 16: return launch_few<16>(p, a, grid, st);
+        case 32: return launch_few<32>(p, a, grid, st);
+        case 64: return launch_few<64>(p, a, grid, st);
+        case 128: return launch_few<128>(p, a, grid, st);
     }
     if (p.out_type == LQ_T_F32) return launch_many<float>(p, a, grid, st);
     if (p.out_type == LQ_T_BF16) return launch_many<__nv_bfloat16>(p, a, grid, st);
