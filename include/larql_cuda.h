@@ -443,7 +443,8 @@ LQ_API int lq_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const float* x, size_t
  *                aligned; hidden and inter multiples of 32, at most 8192 (NVFP4: 6144); 1..256 experts, top_e <= 32.  router
  *                [n_experts, hidden] and router_bias [n_experts] (may be NULL) are device pointers of router_type.
  *                The handle keeps the pointers, not the data, and a workspace for 64 tokens; MXFP4 scales are looked
- *                through once (an e8m0 NaN, 255, is refused).  Weights are immutable while a handle holds them.
+ *                through once (an e8m0 NaN, 255, is refused).  Weights are immutable while a handle holds them.  Not
+ *                during a capture (LQ_ERR_ARGUMENT).
  * lq_dev_moe_ffn x, out [tokens, hidden] of type (LQ_T_F32 / BF16 / F16; out may be x); idx_out, w_out [tokens,
  *                min(top_e, n_experts)] may be NULL.  Calls on one handle run one after another on the stream.
  * lq_moe_ffn     the same with host pointers, f32 (the handle's matrices stay on the device).

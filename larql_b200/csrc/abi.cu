@@ -2438,8 +2438,12 @@ int lq_moe_create(lq_ctx* ctx, const lq_matrix* gates, const lq_matrix* ups, con
     const int fmt = gates[0].fmt & 0xff;
     if (fmt != LQ_FMT_MXFP4 && fmt != LQ_FMT_NVFP4 && fmt != LQ_FMT_FP8_B128)
         return fail(ctx, LQ_REFUSED_UNSUPPORTED, "moe: experts are MXFP4, NVFP4 or FP8_B128");
+    cudaStreamCaptureStatus cs;
+    CK(cudaStreamIsCapturing(ctx->stream, &cs));
+    if (cs != cudaStreamCaptureStatusNone) return fail(ctx, LQ_ERR_ARGUMENT, "moe: create the layer outside a capture");
     const int64_t inter = gates[0].rows, hidden = gates[0].cols;
     std::vector<MoeExpert> table(n_experts);
+    ctx->moes.reserve(ctx->moes.size() + 1);  // (nothing below throws while it holds device memory)
     for (size_t e = 0; e < n_experts; ++e) {
         const lq_matrix* m[3] = {gates + e, ups + e, downs + e};
         for (int i = 0; i < 3; ++i) {

@@ -10,7 +10,8 @@
 // What bounds it is reading h, y, gate and writing h', n once (one token: the two reductions' latency).  Everything is
 // kept in f32 between the loads and the stores, n is taken from the unrounded h'.  A row's squares are summed in f32,
 // pairwise over the threads; when that sum leaves f32's range the row is summed again relative to its largest value
-// (f64 sums, which need no branch, cost 36 us of 159 at 4096 x 8192 bf16: the conversions run at a few lanes a cycle).  Underflow needs no branch: what a square loses is below 2^-149 and eps is at least 2^-126.
+// (f64 sums, which need no branch, cost 36 us of 159 at 4096 x 8192 bf16: the conversions run at a few lanes a cycle).
+// Underflow needs no branch: what a square loses is below 2^-149 and eps is at least 2^-126.
 // rms is at least sqrt(eps) >= 2^-63, so 1 / rms is a normal f32 and one multiply per element replaces a division.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -179,7 +180,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_kernel(con
 }
 
 // Many long rows: a block walks its rows with the next one's operands on their way into shared memory (bulk copies), so
-// that the memory is never idle during a row's two reductions.  4096 x 8192 bf16 with a full gate: 74 us against 98
+// that the memory is never idle during a row's two reductions.  4096 x 8192 bf16 with a full gate: 71 us against 98
 // with loads into registers.
 template <class T, int VEC, int NV, bool SAME, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_stream_kernel(const BlockNorm a, int gate_rows) {

@@ -9,8 +9,8 @@
 // accumulator in registers, while the tensor core works on the next block in another accumulator buffer.  The
 // partial products are exact sums of 8-bit products in f32; every other operation is one f32 fused multiply-add.
 //
-// Two kernels, chosen by the number of tokens (launch_fp8_matmul has the rule and what both measured):
-//   fp8_few_kernel    rows of the weight are the 128 lanes of an accumulator, tokens its 16..128 columns.  What
+// Two kernels, chosen by estimates of their time (way_of has the rule and what both measured):
+//   fp8_few_kernel    rows of the weight are the 128 lanes of an accumulator, tokens its 16, 32 or 64 columns.  What
 //                     bounds it is reading the weight, so the (row tile, k block) units are dealt out evenly over
 //                     the SMs in one contiguous run each, and tiles that end inside a run are joined through a
 //                     workspace by the last CTA to finish its piece, always in the order of k: results do not
@@ -109,7 +109,8 @@ __device__ __forceinline__ float block_amax(const Eight<T>& r) {
 
 // 16 threads per (token, block of 128), 8 consecutive elements each; QU such blocks are on their way at a time (1 where
 // there are few).  The quotients are the correctly rounded ones (and not x times 1 / s): the codes are defined by them,
-// and the tests hold them to the definition bit for bit.  Instructions bound it: 90 for a thread's eight elements.
+// and the tests hold them to the definition bit for bit.  Instructions bound it, 90 for a thread's eight elements: 4096 x 8192
+// bf16 take 26 us, 3.8 TB/s of the 102 MB it reads and writes.
 template <class T, bool VEC, int QU>
 __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__ x, long long x_stride, int units, int kb_n,
                                                            int cols, uint8_t* __restrict__ codes, long long code_pitch,
@@ -195,9 +196,13 @@ struct F8Args {
 };
 
 // ------------------------------------------------------------ few tokens ----
+// What bounds it: with every SM at work the memory (16 tokens x 28672 -> 8192, 237 MB: 50 us with the quantisation, 4.7
+// TB/s); with less than a tile per SM the thread that issues the tensor-core instructions, 0.23 us per block of 16 columns
+// (250 x 2880 -> 2880: 13 us with the quantisation).  That thread and the loading one loop inside elect.sync's branch:
+// behind a branch on the lane every instruction takes several times as long (0.30 us a block).
 constexpr int few_stage_bytes(int nt) { return 128 * 128 + nt * 128; }
-constexpr int few_stages(int nt) { return nt <= 16 ? 11 : (nt <= 32 ? 10 : (nt <= 64 ? 8 : 4)); }  // (an accumulator of nt columns each)
-constexpr int few_promo_warps(int nt) { return nt <= 64 ? nt / 4 : 16; }  // 16 columns a warp, 32 at the widest
+constexpr int few_stages(int nt) { return nt == 16 ? 11 : (nt == 32 ? 10 : 8); }  // (an accumulator of nt columns each)
+constexpr int few_promo_warps(int nt) { return nt / 4; }  // 16 columns a warp
 constexpr int few_threads(int nt) { return 128 + 32 * few_promo_warps(nt); }  // (two warps idle: a warp reads the TMEM lanes of its rank of 4)
 
 template <int NT>
@@ -454,6 +459,10 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 }
 
 // ----------------------------------------------------------- many tokens ----
+// What bounds it is tensor memory, which the product's accumulation and the promotion's reads share: a block (128 x 256 x
+// 128) takes 0.31 us of multiplication alone, 0.60 with its 128 KB read back.  4096 x 8192 -> 28672 in 1.02 ms, 1.9 PFLOP/s,
+// in a burst, 1.2 ms at the power limit.  Measured and not kept: pairs of CTAs on one tile (a third less to load: 1.06 ms),
+// accumulators handed over by halves (1.05), two multiply-adds an instruction (1.09), one arrival a warp (1.05).
 constexpr int MANY_M = 128, MANY_N = 256, MANY_STAGES = 4;
 constexpr int MANY_STAGE = (MANY_M + MANY_N) * 128;
 constexpr int MANY_THREADS = 128 + 512;  // producer, tensor core, two idle warps (a warp reads the TMEM lanes of its rank of 4), promotion
@@ -653,16 +662,17 @@ cudaError_t launch_many(const Fp8Product& p, const F8Args& a, int grid, cudaStre
 }
 
 // How a product runs, from estimates in microseconds (fitted to 23 shapes of 1 to 1024 tokens): a k block of a few-token
-// tile takes an SM 0.235 to 0.68 by its columns, or the memory the time of its 16 KB; joining pieces of tiles costs 3.5,
+// tile takes an SM 0.235 to 0.40 by its columns, or the memory the time of its 16 KB; joining pieces of tiles costs 3.5,
 // 0.11 per column and 0.45 per piece of a tile; a k block of a 128 x 256 tile of the other kernel takes 0.60.  Measured,
 // quantisation included, whole tiles | tiles spread over the grid | the other kernel:
 //   1 x 3840 -> 15360    16 columns 14.7 | 19.4 | 20.8
 //   16 x 28672 -> 8192   16 columns 51.5 | 49.9 | 105
 //   64 x 2880 -> 2880    16 columns 10.7 | 16.7, 32 columns 11.3 | 16.3, 64 columns 13.1 | 19.7, 16.5
 //   64 x 8192 -> 28672   64 columns 59.8 | 55.9 | 49.7
-//   128 x 28672 -> 8192  64 columns 96.5 | 100, 128 columns 183 | 108 | 144
-//   250 x 2880 -> 2880   32 columns 20.6 | 22.7, 64 columns 14.6 | 21.4, 128 columns 20.3 | 29.3 | 20.7
-//   512 x 8192 -> 8192   64 columns 107 | 104, 128 columns 100 | 102 | 45.5
+//   128 x 28672 -> 8192  32 columns 122 | 155, 64 columns 96.8 | 95.9 | 134
+//   250 x 2880 -> 2880   32 columns 20.6 | 22.7, 64 columns 14.6 | 21.4 | 20.7
+//   512 x 8192 -> 8192   64 columns 107 | 104 | 45.5
+// (128 columns were never the fastest: 171 | 108 us at 128 x 28672 -> 8192, 20.3 | 29.3 at 250 x 2880 -> 2880.)
 struct Way {
     int nt;  // columns of the few-token kernel's accumulators, 0: the other kernel
     bool whole;
@@ -676,9 +686,9 @@ Way way_of(size_t tokens, size_t rows, size_t cols, int sm_count) {
     auto take = [&](const Way& w) {
         if (best.grid == 0 || w.us < best.us) best = w;
     };
-    for (int nt = 16; nt <= 128; nt *= 2) {
+    for (int nt = 16; nt <= 64; nt *= 2) {
         const double tiles = (double)((tokens + nt - 1) / nt) * row_tiles, units = tiles * kb;
-        const double unit = nt == 16 ? 0.235 : (nt == 32 ? 0.27 : (nt == 64 ? 0.40 : 0.68));
+        const double unit = nt == 16 ? 0.235 : (nt == 32 ? 0.27 : 0.40);
         take(Way{nt, true, (int)std::min(tiles, sms), std::max(memory, std::ceil(tiles / sms) * kb * unit)});
         take(Way{nt, false, (int)std::min(units, sms), std::max(memory, std::ceil(units / sms) * unit) + 3.5 + 0.11 * nt + 0.45 * sms / tiles});
         if ((size_t)nt >= tokens) break;
@@ -749,7 +759,6 @@ cudaError_t launch_fp8_matmul(const Fp8Product& p, bool chained, int sm_count, i
         case 16: return launch_few<16>(p, a, grid, st);
         case 32: return launch_few<32>(p, a, grid, st);
         case 64: return launch_few<64>(p, a, grid, st);
-        case 128: return launch_few<128>(p, a, grid, st);
     }
     if (p.out_type == LQ_T_F32) return launch_many<float>(p, a, grid, st);
     if (p.out_type == LQ_T_BF16) return launch_many<__nv_bfloat16>(p, a, grid, st);
