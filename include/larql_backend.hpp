@@ -25,7 +25,7 @@ struct BackendError : std::runtime_error {
     BackendError(int st, const std::string& what) : std::runtime_error(what), status(st) {}
 };
 
-enum class QuantFormat : int { Q4_K = LQ_FMT_Q4_K, Q8_0 = LQ_FMT_Q8_0, MXFP4 = LQ_FMT_MXFP4, NVFP4 = LQ_FMT_NVFP4 };
+enum class QuantFormat : int { Q4_K = LQ_FMT_Q4_K, Q8_0 = LQ_FMT_Q8_0, MXFP4 = LQ_FMT_MXFP4, NVFP4 = LQ_FMT_NVFP4, FP8_B128 = LQ_FMT_FP8_B128 };
 
 // A quantised [rows, cols] matrix in host memory (the reference's mmap slices) or, with
 // `on_device`, raw device pointers.
@@ -33,7 +33,7 @@ struct QuantMatrix {
     QuantFormat fmt = QuantFormat::Q4_K;
     const uint8_t* data = nullptr;
     size_t data_len = 0;
-    const uint8_t* scales = nullptr;  // MXFP4 e8m0 / NVFP4 e4m3 stream
+    const uint8_t* scales = nullptr;  // MXFP4 e8m0 / NVFP4 e4m3 stream / FP8_B128 f32, one per 128 x 128
     size_t scales_len = 0;
     float tensor_scale = 1.0f;        // NVFP4
     int64_t rows = 0, cols = 0;
@@ -51,6 +51,30 @@ struct QuantMatrix {
         m.cols = cols;
         return m;
     }
+};
+
+// A mixture-of-experts layer (CudaBackend::moe_create): destroy it before its weights.
+class MoeLayer {
+public:
+    MoeLayer(lq_ctx* ctx, lq_moe* h, size_t hidden, size_t per_token) : ctx_(ctx), h_(h), hidden_(hidden), per_token_(per_token) {}
+    MoeLayer(MoeLayer&& o) noexcept : ctx_(o.ctx_), h_(std::exchange(o.h_, nullptr)), hidden_(o.hidden_), per_token_(o.per_token_) {}
+    MoeLayer(const MoeLayer&) = delete;
+    MoeLayer& operator=(const MoeLayer&) = delete;
+    MoeLayer& operator=(MoeLayer&&) = delete;
+    ~MoeLayer() { lq_moe_destroy(ctx_, h_); }
+    lq_moe* raw() const { return h_; }
+    size_t hidden() const { return hidden_; }
+    size_t per_token() const { return per_token_; }  // experts a token goes to
+
+private:
+    lq_ctx* ctx_;
+    lq_moe* h_;
+    size_t hidden_, per_token_;
+};
+struct MoeResult {
+    std::vector<float> out;      // [tokens, hidden]
+    std::vector<uint32_t> idx;   // [tokens, per_token]
+    std::vector<float> weights;  // [tokens, per_token]
 };
 
 struct WalkResult {
@@ -202,6 +226,47 @@ public:
         if (!ok(lq_walk_ffn(ctx_, &g, &u, &d, x, batch, top_k, flags, r.out.data(), idx.data(), cnt.data()))) return std::nullopt;
         r.hits.resize(batch);
         for (size_t t = 0; t < batch; ++t) r.hits[t].assign(idx.begin() + t * stride, idx.begin() + t * stride + cnt[t]);
+        return r;
+    }
+
+    // ---- layer operators (no trait method; larql_cuda.h has their formulas).  dev_* take device pointers, enqueue on the
+    // context's stream and return false where the library refuses the call.
+    bool dev_block_norm(const lq_block_norm_args& args) { return ok(lq_dev_block_norm(ctx_, &args)); }
+    bool dev_fp8_quantize(const void* x, int type, size_t tokens, size_t cols, size_t x_stride, uint8_t* codes, float* scales) {
+        return ok(lq_dev_fp8_quantize(ctx_, x, type, tokens, cols, x_stride, codes, scales));
+    }
+    bool dev_fp8_matmul(const QuantMatrix& w, const void* x, int x_type, const float* x_scales, size_t tokens, size_t x_stride,
+                        void* out, int out_type, size_t out_stride) {
+        const lq_matrix m = w.c();
+        return ok(lq_dev_fp8_matmul(ctx_, &m, x, x_type, x_scales, tokens, x_stride, out, out_type, out_stride));
+    }
+    // x [tokens, cols] on the host -> [tokens, rows], activations quantised on the way
+    std::optional<std::vector<float>> fp8_matmul(const QuantMatrix& w, const float* x, size_t x_len, size_t tokens) {
+        const lq_matrix m = w.c();
+        std::vector<float> out(tokens * static_cast<size_t>(w.rows));
+        return ok(lq_fp8_matmul(ctx_, &m, x, x_len, tokens, out.data(), out.size())) ? std::optional(std::move(out)) : std::nullopt;
+    }
+    // The experts' matrices are on the device, as router [experts, hidden] and bias [experts] (may be null) of router_type.
+    std::optional<MoeLayer> moe_create(const std::vector<QuantMatrix>& gates, const std::vector<QuantMatrix>& ups,
+                                       const std::vector<QuantMatrix>& downs, const void* router, int router_type, const void* bias,
+                                       size_t top_e, bool renormalise) {
+        if (gates.size() != ups.size() || gates.size() != downs.size() || gates.empty()) return std::nullopt;
+        std::vector<lq_matrix> g, u, d;
+        for (size_t e = 0; e < gates.size(); ++e) g.push_back(gates[e].c()), u.push_back(ups[e].c()), d.push_back(downs[e].c());
+        lq_moe* h = nullptr;
+        if (!ok(lq_moe_create(ctx_, g.data(), u.data(), d.data(), g.size(), router, router_type, bias, top_e, renormalise, &h)))
+            return std::nullopt;
+        return std::optional<MoeLayer>(std::in_place, ctx_, h, static_cast<size_t>(gates[0].cols), top_e < g.size() ? top_e : g.size());
+    }
+    bool dev_moe_ffn(const MoeLayer& layer, const void* x, int type, size_t tokens, void* out, uint32_t* idx, float* weights) {
+        return ok(lq_dev_moe_ffn(ctx_, layer.raw(), x, type, tokens, out, idx, weights));
+    }
+    std::optional<MoeResult> moe_ffn(const MoeLayer& layer, const float* x, size_t x_len, size_t tokens) {
+        MoeResult r;
+        r.out.resize(tokens * layer.hidden());
+        r.idx.resize(tokens * layer.per_token());
+        r.weights.resize(tokens * layer.per_token());
+        if (!ok(lq_moe_ffn(ctx_, layer.raw(), x, x_len, tokens, r.out.data(), r.idx.data(), r.weights.data()))) return std::nullopt;
         return r;
     }
 

@@ -46,6 +46,13 @@ pub const LQ_FMT_Q4_K: i32 = 0;
 pub const LQ_FMT_Q8_0: i32 = 1;
 pub const LQ_FMT_MXFP4: i32 = 2;
 pub const LQ_FMT_NVFP4: i32 = 3;
+pub const LQ_FMT_FP8_B128: i32 = 5;
+pub const LQ_MAT_DEVICE: i32 = 0x100;
+/// Element types of the layer operators (`enum lq_type`).
+pub const LQ_T_F32: i32 = 0;
+pub const LQ_T_BF16: i32 = 1;
+pub const LQ_T_F16: i32 = 2;
+pub const LQ_T_E4M3: i32 = 3;
 pub const LQ_WALK_RMSNORM: u32 = 1;
 pub const LQ_WALK_RESIDUAL: u32 = 2;
 pub const LQ_WALK_FORCE_SPARSE: u32 = 4;
@@ -58,6 +65,39 @@ pub struct LqCtx {
 #[repr(C)]
 pub struct LqStack {
     _opaque: [u8; 0],
+}
+
+#[repr(C)]
+pub struct LqMoe {
+    _opaque: [u8; 0],
+}
+
+/// Mirrors `lq_block_norm_args`.
+#[repr(C)]
+pub struct LqBlockNormArgs {
+    pub ty: i32,
+    pub w_type: i32,
+    pub post_norm: i32,
+    pub w_offset: f32,
+    pub h_scale: f32,
+    pub y_scale: f32,
+    pub eps: f64,
+    pub rows: usize,
+    pub cols: usize,
+    pub h: *const c_void,
+    pub h_stride: usize,
+    pub y: *const c_void,
+    pub y_stride: usize,
+    pub post_w: *const c_void,
+    pub pre_w: *const c_void,
+    pub gate: *const c_void,
+    pub gate_cols: usize,
+    pub gate_stride: usize,
+    pub gate_group: usize,
+    pub h_out: *mut c_void,
+    pub h_out_stride: usize,
+    pub n_out: *mut c_void,
+    pub n_out_stride: usize,
 }
 
 extern "C" {
@@ -100,6 +140,21 @@ extern "C" {
                        n_layers: usize, batch: usize, top_k: usize, flags: u32, out: *mut *mut LqStack) -> c_int;
     fn lq_stack_run_host(ctx: *mut LqCtx, stack: *mut LqStack, h_in: *const f32, h_out: *mut f32) -> c_int;
     fn lq_stack_destroy(ctx: *mut LqCtx, stack: *mut LqStack);
+    fn lq_dev_block_norm(ctx: *mut LqCtx, args: *const LqBlockNormArgs) -> c_int;
+    fn lq_dev_fp8_quantize(ctx: *mut LqCtx, x: *const c_void, x_type: c_int, tokens: usize, cols: usize, x_stride: usize,
+                           codes: *mut u8, scales: *mut f32) -> c_int;
+    fn lq_dev_fp8_matmul(ctx: *mut LqCtx, w: *const LqMatrix, x: *const c_void, x_type: c_int, x_scales: *const f32,
+                         tokens: usize, x_stride: usize, out: *mut c_void, out_type: c_int, out_stride: usize) -> c_int;
+    fn lq_fp8_matmul(ctx: *mut LqCtx, w: *const LqMatrix, x: *const f32, x_len: usize, tokens: usize, out: *mut f32,
+                     out_len: usize) -> c_int;
+    fn lq_moe_create(ctx: *mut LqCtx, gates: *const LqMatrix, ups: *const LqMatrix, downs: *const LqMatrix,
+                     n_experts: usize, router: *const c_void, router_type: c_int, router_bias: *const c_void,
+                     top_e: usize, renormalise: c_int, out: *mut *mut LqMoe) -> c_int;
+    fn lq_dev_moe_ffn(ctx: *mut LqCtx, moe: *mut LqMoe, x: *const c_void, ty: c_int, tokens: usize, out: *mut c_void,
+                      idx_out: *mut u32, w_out: *mut f32) -> c_int;
+    fn lq_moe_ffn(ctx: *mut LqCtx, moe: *mut LqMoe, x: *const f32, x_len: usize, tokens: usize, out: *mut f32,
+                  idx_out: *mut u32, w_out: *mut f32) -> c_int;
+    fn lq_moe_destroy(ctx: *mut LqCtx, moe: *mut LqMoe);
 }
 
 struct Ctx(*mut LqCtx);
@@ -220,6 +275,95 @@ impl Drop for WalkStack<'_> {
     fn drop(&mut self) {
         let guard = self.backend.ctx.lock().unwrap_or_else(|e| e.into_inner());
         unsafe { lq_stack_destroy(guard.0, self.raw) };
+    }
+}
+
+/// The layer operators beside the walk (include/larql_cuda.h): no trait method carries them.
+impl CudaBackend {
+    /// `x` `[tokens, cols]` by an FP8_B128 matrix in host memory, activations quantised on the way.
+    pub fn fp8_matmul(&self, w: &LqMatrix, x: &[f32], tokens: usize) -> Option<Vec<f32>> {
+        let mut out = vec![0f32; tokens * w.rows as usize];
+        self.call(|c| (unsafe { lq_fp8_matmul(c, w, x.as_ptr(), x.len(), tokens, out.as_mut_ptr(), out.len()) }, ()))
+            .map(|_| out)
+    }
+
+    /// # Safety
+    /// Every pointer of `args` is null where that is allowed, or device memory of its rows.
+    pub unsafe fn dev_block_norm(&self, args: &LqBlockNormArgs) -> Option<()> {
+        self.call(|c| (lq_dev_block_norm(c, args), ()))
+    }
+
+    /// # Safety
+    /// `x`, `codes` and `scales` are device memory of their sizes.
+    pub unsafe fn dev_fp8_quantize(&self, x: *const c_void, x_type: i32, tokens: usize, cols: usize, x_stride: usize,
+                                   codes: *mut u8, scales: *mut f32) -> Option<()> {
+        self.call(|c| (lq_dev_fp8_quantize(c, x, x_type, tokens, cols, x_stride, codes, scales), ()))
+    }
+
+    /// # Safety
+    /// `w` (with `LQ_MAT_DEVICE`), `x`, `x_scales` and `out` are device memory of their sizes.
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn dev_fp8_matmul(&self, w: &LqMatrix, x: *const c_void, x_type: i32, x_scales: *const f32, tokens: usize,
+                                 x_stride: usize, out: *mut c_void, out_type: i32, out_stride: usize) -> Option<()> {
+        self.call(|c| (lq_dev_fp8_matmul(c, w, x, x_type, x_scales, tokens, x_stride, out, out_type, out_stride), ()))
+    }
+
+    /// A mixture-of-experts layer over matrices on the device (`gates`, `ups` `[inter, hidden]`, `downs`
+    /// `[hidden, inter]`).
+    ///
+    /// # Safety
+    /// The matrices (with `LQ_MAT_DEVICE`), `router` and `router_bias` (may be null) are device memory that outlives the
+    /// layer.
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn moe_layer(&self, gates: &[LqMatrix], ups: &[LqMatrix], downs: &[LqMatrix], router: *const c_void,
+                            router_type: i32, router_bias: *const c_void, top_e: usize, renormalise: bool)
+                            -> Option<MoeLayer<'_>> {
+        if gates.len() != ups.len() || gates.len() != downs.len() || gates.is_empty() {
+            return None;
+        }
+        let mut raw: *mut LqMoe = std::ptr::null_mut();
+        self.call(|c| {
+            let rc = lq_moe_create(c, gates.as_ptr(), ups.as_ptr(), downs.as_ptr(), gates.len(), router, router_type,
+                                   router_bias, top_e, renormalise as c_int, &mut raw);
+            (rc, ())
+        })?;
+        Some(MoeLayer { backend: self, raw, hidden: gates[0].cols as usize, per_token: top_e.min(gates.len()) })
+    }
+}
+
+pub struct MoeLayer<'a> {
+    backend: &'a CudaBackend,
+    raw: *mut LqMoe,
+    hidden: usize,
+    per_token: usize,
+}
+
+impl MoeLayer<'_> {
+    /// `x` `[tokens, hidden]` → the layer's output, each token's experts and their weights.
+    pub fn ffn(&self, x: &[f32], tokens: usize) -> Option<(Vec<f32>, Vec<u32>, Vec<f32>)> {
+        let mut out = vec![0f32; tokens * self.hidden];
+        let (mut idx, mut w) = (vec![0u32; tokens * self.per_token], vec![0f32; tokens * self.per_token]);
+        self.backend.call(|c| {
+            let rc = unsafe {
+                lq_moe_ffn(c, self.raw, x.as_ptr(), x.len(), tokens, out.as_mut_ptr(), idx.as_mut_ptr(), w.as_mut_ptr())
+            };
+            (rc, ())
+        })?;
+        Some((out, idx, w))
+    }
+
+    /// # Safety
+    /// `x` and `out` are device memory of `[tokens, hidden]`, `idx` and `w` null or of `[tokens, per_token]`.
+    pub unsafe fn dev_ffn(&self, x: *const c_void, ty: i32, tokens: usize, out: *mut c_void, idx: *mut u32, w: *mut f32)
+                          -> Option<()> {
+        self.backend.call(|c| (lq_dev_moe_ffn(c, self.raw, x, ty, tokens, out, idx, w), ()))
+    }
+}
+
+impl Drop for MoeLayer<'_> {
+    fn drop(&mut self) {
+        let guard = self.backend.ctx.lock().unwrap_or_else(|e| e.into_inner());
+        unsafe { lq_moe_destroy(guard.0, self.raw) };
     }
 }
 
