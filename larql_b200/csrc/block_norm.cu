@@ -100,7 +100,7 @@ __device__ __forceinline__ float inverse_rms(const float (&v)[N], float inv_cols
 #pragma unroll
     for (int i = 0; i < N; ++i) t = fmaf(v[i] / m, v[i] / m, t);
     t = row_reduce<WARP, false>(t, red);
-    return 1.0f / m / sqrtf(t * inv_cols);  // (eps is nothing beside such values)
+    return 1.0f / m / sqrtf(fmaf(t, inv_cols, eps / m / m));
 }
 
 // One row per warp (WARP: blockDim = 32 x rows) or per block; a thread holds NV packs of VEC elements.
@@ -113,12 +113,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_kernel(con
     using P = Pack<T, VEC>;
     const int rows_per = WARP ? blockDim.y : 1;
     pdl_wait();
-    for (int row = blockIdx.x * rows_per + (WARP ? threadIdx.y : 0); row < a.rows; row += gridDim.x * rows_per) {
+    // (unsigned: a step past the last row may leave int's range)
+    for (unsigned row = blockIdx.x * rows_per + (WARP ? threadIdx.y : 0); row < (unsigned)a.rows; row += gridDim.x * rows_per) {
         P h[NV], g[NV];
         float v[NV * VEC];  // y, then z, then h'
         const T* hp = static_cast<const T*>(a.h) + (size_t)row * a.h_stride;
         const T* yp = static_cast<const T*>(a.y) + (a.y ? (size_t)row * a.y_stride : 0);
-        const T* gp = static_cast<const T*>(a.gate) + (a.gate ? (size_t)(row / (int)a.gate_group) * a.gate_stride : 0);
+        const T* gp = static_cast<const T*>(a.gate) + (a.gate ? (size_t)(row / (unsigned)a.gate_group) * a.gate_stride : 0);
         const bool gate_vec = a.gate && a.gate_cols != 1;
         float gs = a.y_scale;
         if (a.gate && a.gate_cols == 1) gs *= to_f32(gp[0]);

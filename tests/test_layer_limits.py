@@ -92,6 +92,35 @@ def test_block_norm_offsets_past_32_bits(be):
     check_norm(c, rows["h_out"], rows["n_out"])
 
 
+@gpu
+@pytest.mark.parametrize("rows", [3, 1300])
+def test_block_norm_eps_beside_values_beyond_f32(be, rows):
+    """Rows whose squares leave f32's range, and an eps of their size."""
+    c = norm_case(rows, 4096, "f32", "f32", True, "none", 0, 5, y_scale=1.0)
+    c["h"].zero_()
+    c["y"].mul_(1e18)  # sum of squares 4e39, mean 1e36
+    c["eps"] = 1e36
+    h_out, n_out = torch.empty(rows, 4096, device="cuda"), torch.empty(rows, 4096, device="cuda")
+    torch.cuda.synchronize()
+    assert be.dev_block_norm(norm_args(c, h_out, n_out))
+    be.synchronize()
+    check_norm(c, h_out, None)
+    assert (n_out.abs().amax() < 1e-17) and (n_out != 0).any()  # h' is near 1, eps far above its square
+
+
+@gpu
+def test_block_norm_of_the_most_rows(be):
+    """2^31 - 1 rows of one element: the last step of the walk over the rows leaves int's range."""
+    rows = 2 ** 31 - 1
+    h = torch.ones(rows, dtype=torch.float16, device="cuda")
+    out = torch.zeros(rows, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    assert be.dev_block_norm(larql_b200.BlockNormArgs(type=larql_b200.T_F16, w_type=larql_b200.T_F16, h_scale=3.0, y_scale=1.0, eps=1e-6, rows=rows,
+                                                      cols=1, h=h.data_ptr(), h_stride=1, gate_group=1, h_out=out.data_ptr(), h_out_stride=1))
+    be.synchronize()
+    assert bool((out == 3).all())
+
+
 # ------------------------------------------------------------------ FP8 ----
 @gpu
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
