@@ -615,38 +615,45 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     ++units;
                     const MoeExpert& ex = L.table[sh.active[a]];
                     const int row = lane & 15, half = lane >> 4;
-                    const float ts = ex.ts[w.is_down ? 2 : half];
+                    const float ts0 = ex.ts[w.is_down ? 2 : 0], ts1 = ex.ts[w.is_down ? 2 : 1];
                     if (ok) ok = __all_sync(0xffffffffu, ml_wait<true>(&sh.rfull[buf], parity));
                     const int cnt = sh.cnt;
-                    // lane i keeps what belongs to token i of the group
-                    float scale = 0.0f;
-                    if (lane < cnt) {
-                        pair = sh.gpair[lane];
-                        // (the routing weight goes into the power of two, so that only the weighted output has to be in range)
-                        scale = sh.unscale[lane] * (w.is_down ? sh.w[pair] : 1.0f);
-                    }
+                    if (lane < cnt) pair = sh.gpair[lane];  // (lane i publishes what belongs to token i of the group)
                     const float* all = red + buf * ML_WARPS * 2 * RED;
-                    // two tiles: a half of the lanes each; one tile: the halves take half of the warps' parts each (an even
-                    // and an odd part at a time, in the order of the warps)
-                    const float* part = all + (w.tiles == 2 ? half * RED : half * (ML_WARPS / 2) * 2 * RED);
-                    const int parts = w.tiles == 2 ? ML_WARPS : ML_WARPS / 2;
-                    for (int i = 0; i < cnt; ++i) {
-                        float v = 0.0f;
-                        const int c0 = red_at(terms * i, row), c1 = red_at(terms * i + terms - 1, row);
-#pragma unroll 8
-                        for (int q = 0; q < parts; ++q) v += terms == 2 ? part[q * 2 * RED + c0] + part[q * 2 * RED + c1] : part[q * 2 * RED + c0];
-                        if (w.tiles == 1) v += __shfl_xor_sync(0xffffffffu, v, 16);
-                        v = v * __shfl_sync(0xffffffffu, scale, i) * ts;
-                        const size_t at = (size_t)__shfl_sync(0xffffffffu, pair, i);
-                        if (!w.is_down) {
-                            const float up = __shfl_down_sync(0xffffffffu, v, 16);
-                            const float act = v / (1.0f + expf(-v)) * up;
-                            if (half == 0) __stcg(L.act + at * L.inter + tile * 16 + row, act);
-                            // the pair's largest |value| (a NaN's bits are above every number's)
-                            const unsigned m = __reduce_max_sync(0xffffffffu, half == 0 ? __float_as_uint(act) & 0x7fffffffu : 0u);
-                            if (lane == i) top = max(top, m);
-                        } else if (w.tiles == 2 || half == 0) {
-                            __stcg(L.pair_out + at * L.hidden + (tile * w.tiles + (w.tiles == 2 ? half : 0)) * 16 + row, v);
+                    // a half of the lanes takes a token, a lane one row of either tile
+                    for (int i0 = 0; i0 < cnt; i0 += 2) {
+                        const bool live = i0 + half < cnt;
+                        const int i = live ? i0 + half : i0, at = sh.gpair[i];
+                        // (the routing weight goes into the power of two, so that only the weighted output has to be in range)
+                        const float scale = sh.unscale[i] * (w.is_down ? sh.w[at] : 1.0f);
+                        // (the second half adds a value's two columns the other way round: different banks)
+                        const int swap = half & (terms - 1);
+                        const int c0 = red_at(terms * i + swap, row), c1 = red_at(terms * i + terms - 1 - swap, row);
+                        auto parts = [&](const float* part, int from, int to) {
+                            float v = 0.0f;
+#pragma unroll
+                            for (int q = from; q < to; ++q) v += terms == 2 ? part[q * 2 * RED + c0] + part[q * 2 * RED + c1] : part[q * 2 * RED + c0];
+                            return v;
+                        };
+                        if (w.tiles == 2) {
+                            const float v0 = parts(all, 0, ML_WARPS) * scale * ts0, v1 = parts(all + RED, 0, ML_WARPS) * scale * ts1;
+                            if (!w.is_down) {
+                                const float act = v0 / (1.0f + expf(-v0)) * v1;
+                                if (live) __stcg(L.act + (size_t)at * L.inter + tile * 16 + row, act);
+                                // the pairs' largest |value| (a NaN's bits are above every number's)
+                                const unsigned m = live ? __float_as_uint(act) & 0x7fffffffu : 0u;
+                                const unsigned m0 = __reduce_max_sync(0xffffffffu, half ? 0u : m), m1 = __reduce_max_sync(0xffffffffu, half ? m : 0u);
+                                if (lane == i0) top = max(top, m0);
+                                if (lane == i0 + 1) top = max(top, m1);
+                            } else if (live) {
+                                float* o = L.pair_out + (size_t)at * L.hidden + tile * 32 + row;
+                                __stcg(o, v0);
+                                __stcg(o + 16, v1);
+                            }
+                        } else {
+                            // (two sums of eight)
+                            const float v = parts(all, 0, ML_WARPS / 2) + parts(all, ML_WARPS / 2, ML_WARPS);
+                            if (live) __stcg(L.pair_out + (size_t)at * L.hidden + tile * 16 + row, v * scale * ts0);
                         }
                     }
                     __syncwarp();
