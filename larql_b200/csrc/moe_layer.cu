@@ -614,46 +614,55 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     if (!mine) continue;
                     ++units;
                     const MoeExpert& ex = L.table[sh.active[a]];
-                    const int row = lane & 15, half = lane >> 4;
                     const float ts0 = ex.ts[w.is_down ? 2 : 0], ts1 = ex.ts[w.is_down ? 2 : 1];
                     if (ok) ok = __all_sync(0xffffffffu, ml_wait<true>(&sh.rfull[buf], parity));
                     const int cnt = sh.cnt;
                     if (lane < cnt) pair = sh.gpair[lane];  // (lane i publishes what belongs to token i of the group)
                     const float* all = red + buf * ML_WARPS * 2 * RED;
-                    // a half of the lanes takes a token, a lane one row of either tile
-                    for (int i0 = 0; i0 < cnt; i0 += 2) {
-                        const bool live = i0 + half < cnt;
-                        const int i = live ? i0 + half : i0, at = sh.gpair[i];
-                        // (the routing weight goes into the power of two, so that only the weighted output has to be in range)
-                        const float scale = sh.unscale[i] * (w.is_down ? sh.w[at] : 1.0f);
-                        // (the second half adds a value's two columns the other way round: different banks)
-                        const int swap = half & (terms - 1);
-                        const int c0 = red_at(terms * i + swap, row), c1 = red_at(terms * i + terms - 1 - swap, row);
-                        auto parts = [&](const float* part, int from, int to) {
-                            float v = 0.0f;
+                    // eight columns at a time, a lane four rows of one column in both tiles; a token's two terms lie in two columns
+                    const int col = lane >> 2, quad = lane & 3, per_tile = 8 / terms;
 #pragma unroll
-                            for (int q = from; q < to; ++q) v += terms == 2 ? part[q * 2 * RED + c0] + part[q * 2 * RED + c1] : part[q * 2 * RED + c0];
-                            return v;
-                        };
-                        if (w.tiles == 2) {
-                            const float v0 = parts(all, 0, ML_WARPS) * scale * ts0, v1 = parts(all + RED, 0, ML_WARPS) * scale * ts1;
-                            if (!w.is_down) {
-                                const float act = v0 / (1.0f + expf(-v0)) * v1;
-                                if (live) __stcg(L.act + (size_t)at * L.inter + tile * 16 + row, act);
-                                // the pairs' largest |value| (a NaN's bits are above every number's)
-                                const unsigned m = live ? __float_as_uint(act) & 0x7fffffffu : 0u;
-                                const unsigned m0 = __reduce_max_sync(0xffffffffu, half ? 0u : m), m1 = __reduce_max_sync(0xffffffffu, half ? m : 0u);
-                                if (lane == i0) top = max(top, m0);
-                                if (lane == i0 + 1) top = max(top, m1);
-                            } else if (live) {
-                                float* o = L.pair_out + (size_t)at * L.hidden + tile * 32 + row;
-                                __stcg(o, v0);
-                                __stcg(o + 16, v1);
+                    for (int j = 0; j < NT; ++j) {
+                        if (j * per_tile >= cnt) break;
+                        const int i = j * per_tile + col / terms;
+                        const bool live = i < cnt && (terms == 1 || (col & 1) == 0);
+                        const int at = sh.gpair[i < cnt ? i : 0];
+                        // (the routing weight goes into the power of two, so that only the weighted output has to be in range)
+                        const float scale = sh.unscale[i < cnt ? i : 0] * (w.is_down ? sh.w[at] : 1.0f);
+                        auto sums = [&](const float* part, float f) {  // the warps' parts in order
+                            const float* from = part + red_at(j * 8 + col, 4 * quad);
+                            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                            for (int q = 0; q < ML_WARPS; ++q) {
+                                const float4 u = *reinterpret_cast<const float4*>(from + q * 2 * RED);
+                                v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
                             }
+                            if (terms == 2) {
+                                v.x += __shfl_xor_sync(0xffffffffu, v.x, 4), v.y += __shfl_xor_sync(0xffffffffu, v.y, 4);
+                                v.z += __shfl_xor_sync(0xffffffffu, v.z, 4), v.w += __shfl_xor_sync(0xffffffffu, v.w, 4);
+                            }
+                            return make_float4(v.x * scale * f, v.y * scale * f, v.z * scale * f, v.w * scale * f);
+                        };
+                        const float4 a0 = sums(all, ts0);
+                        if (!w.is_down) {
+                            const float4 a1 = sums(all + RED, ts1);
+                            auto silu = [](float g, float u) { return g / (1.0f + expf(-g)) * u; };
+                            const float4 act = make_float4(silu(a0.x, a1.x), silu(a0.y, a1.y), silu(a0.z, a1.z), silu(a0.w, a1.w));
+                            if (live) __stcg(reinterpret_cast<float4*>(L.act + (size_t)at * L.inter + tile * 16 + 4 * quad), act);
+                            // the pairs' largest |value| (a NaN's bits are above every number's)
+                            auto bits = [](float v) { return __float_as_uint(v) & 0x7fffffffu; };
+                            unsigned m = max(max(bits(act.x), bits(act.y)), max(bits(act.z), bits(act.w)));
+                            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                            const unsigned mine = __shfl_sync(0xffffffffu, m, (lane - j * per_tile) * terms * 4 & 31);
+                            if (lane >= j * per_tile && lane < min(cnt, (j + 1) * per_tile)) top = max(top, mine);  // (columns past the group hold anything)
                         } else {
-                            // (two sums of eight)
-                            const float v = parts(all, 0, ML_WARPS / 2) + parts(all, ML_WARPS / 2, ML_WARPS);
-                            if (live) __stcg(L.pair_out + (size_t)at * L.hidden + tile * 16 + row, v * scale * ts0);
+                            float* o = L.pair_out + (size_t)at * L.hidden + tile * w.tiles * 16 + 4 * quad;
+                            if (live) __stcg(reinterpret_cast<float4*>(o), a0);
+                            if (w.tiles == 2) {
+                                const float4 a1 = sums(all + RED, ts1);
+                                if (live) __stcg(reinterpret_cast<float4*>(o + 16), a1);
+                            }
                         }
                     }
                     __syncwarp();
