@@ -25,9 +25,9 @@
 // power of two per token; bf16 layers take one f16 term (all of a bf16's bits; activations between the products
 // rounded to f16's 11), f32 and f16 layers two (22 bits, a column each).  Scales: e8m0 (per row and 32) and
 // FP8 blocks multiply the f32 sums of 32 products, e4m3 (per row and 16) the f16 codes, which is exact (2 + 4 bits).
-// Measured: 32 MXFP4 experts of 2880 x 2880, 4 a token: 16 bf16 tokens 108 us for 373 MB, 3.4 TB/s; one f32 token 35 us for
-// 53 MB.  64 FP8 experts of 3840 x 800, 6 a token: 37 bf16 tokens 173 us for 576 MB, 3.3 TB/s.  The copies alone take 55, 9
-// and 93 us: the compute warps' conversions and latencies bound it (integer pipe 47 %, an instruction in 57 % of the
+// Measured: 32 MXFP4 experts of 2880 x 2880, 4 a token: 16 bf16 tokens 107 us for 373 MB, 3.5 TB/s; one f32 token 35 us for
+// 53 MB.  64 FP8 experts of 3840 x 800, 6 a token: 37 bf16 tokens 169 us for 576 MB, 3.4 TB/s.  The copies alone take 55, 9
+// and 93 us: the compute warps' conversions and latencies bound it (integer pipe 51 %, an instruction in 58 % of the
 // cycles, tensor pipe 19 %), and for one token the routing's exchange between the CTAs and the two phases' starts.
 // (Tried: e4m3 terms and m16n8k32 e4m3 products, which need no conversion of FP8 codes: that form is converted to f16
 // behind the instruction, 32 cycles of a scheduler against 2 x 8.)
