@@ -20,6 +20,8 @@
 #include "kernels.h"
 #include "tc5.cuh"
 
+#include <type_traits>
+
 namespace lq {
 
 namespace {
@@ -78,6 +80,21 @@ __device__ __forceinline__ float row_reduce(float s, float* red) {
     return s;
 }
 
+// inverse_rms for a row whose squares' sum s left f32's range (or is NaN).
+template <bool WARP, int N>
+__device__ __forceinline__ float inverse_rms_beyond(const float (&v)[N], float s, float inv_cols, float eps, float* red) {
+    if (s != s) return s;
+    float m = 0.0f;  // (the same for every thread of the row)
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(v[i]));
+    m = row_reduce<WARP, true>(m, red);
+    if (m > 3.4e38f) return 0.0f;  // an infinity: finite / inf, and inf * 0 = NaN where it stands
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t = fmaf(v[i] / m, v[i] / m, t);
+    t = row_reduce<WARP, false>(t, red);
+    return 1.0f / m / sqrtf(fmaf(t, inv_cols, eps / m / m));
+}
 // 1 / rms of the row whose elements the threads hold N each (zero past the end).
 template <bool WARP, int N>
 __device__ __forceinline__ float inverse_rms(const float (&v)[N], float inv_cols, float eps, float* red) {
@@ -90,17 +107,7 @@ __device__ __forceinline__ float inverse_rms(const float (&v)[N], float inv_cols
         for (int i = 0; i < n; ++i) q[i] += q[i + n];
     const float s = row_reduce<WARP, false>(q[0], red);
     if (s <= 1e38f) return 1.0f / sqrtf(s * inv_cols + eps);
-    if (s != s) return s;
-    float m = 0.0f;  // beyond f32 (the same for every thread of the row)
-#pragma unroll
-    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(v[i]));
-    m = row_reduce<WARP, true>(m, red);
-    if (m > 3.4e38f) return 0.0f;  // an infinity: finite / inf, and inf * 0 = NaN where it stands
-    float t = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) t = fmaf(v[i] / m, v[i] / m, t);
-    t = row_reduce<WARP, false>(t, red);
-    return 1.0f / m / sqrtf(fmaf(t, inv_cols, eps / m / m));
+    return inverse_rms_beyond<WARP>(v, s, inv_cols, eps, red);
 }
 
 // One row per warp (WARP: blockDim = 32 x rows) or per block; a thread holds NV packs of VEC elements.
@@ -180,8 +187,80 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_kernel(con
     }
 }
 
+// Two f32 in one register pair, worked on by one instruction (each lane of it correctly rounded).
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pair(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 halves(F2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+// A pack's elements in pairs, and back.
+template <class T, int VEC>
+__device__ __forceinline__ void pairs_of(const Pack<T, VEC>& p, F2 (&out)[VEC / 2]) {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            out[i] = pair(p.v[2 * i], p.v[2 * i + 1]);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const uint32_t w = reinterpret_cast<const uint32_t*>(&p)[i];
+            out[i] = pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+        } else {
+            const float2 f = __half22float2(reinterpret_cast<const __half2*>(&p)[i]);
+            out[i] = pair(f.x, f.y);
+        }
+    }
+}
+template <class T>
+__device__ __forceinline__ void put_pair(T* at, F2 v) {
+    const float2 f = halves(v);
+    if constexpr (sizeof(T) == 4) at[0] = f.x, at[1] = f.y;
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<__nv_bfloat162*>(at) = __floats2bfloat162_rn(f.x, f.y);
+    else *reinterpret_cast<__half2*>(at) = __floats2half2_rn(f.x, f.y);
+}
+// inverse_rms of elements held in pairs, by the whole block.
+template <int N>
+__device__ __forceinline__ float inverse_rms_pairs(const F2 (&v)[N], float inv_cols, float eps, float* red) {
+    F2 q[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i] = mul2(v[i], v[i]);
+#pragma unroll
+    for (int n = N / 2; n > 0; n >>= 1)
+#pragma unroll
+        for (int i = 0; i < n; ++i) q[i] = add2(q[i], q[i + n]);
+    const float2 f = halves(q[0]);
+    const float s = row_reduce<false, false>(f.x + f.y, red);
+    if (s <= 1e38f) return 1.0f / sqrtf(s * inv_cols + eps);
+    float e[2 * N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float2 h = halves(v[i]);
+        e[2 * i] = h.x, e[2 * i + 1] = h.y;
+    }
+    return inverse_rms_beyond<false>(e, s, inv_cols, eps, red);
+}
+
 // Many long rows: a block walks its rows with the next one's operands on their way into shared memory (bulk copies), so
-// that the memory is never idle during a row's two reductions.  4096 x 8192 bf16 with a full gate: 71 us against 98
+// that the memory is never idle during a row's two reductions.  4096 x 8192 bf16 with a full gate: 64 us (5.2 TB/s) against 98
 // with loads into registers.
 template <class T, int VEC, int NV, bool SAME, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_stream_kernel(const BlockNorm a, int gate_rows) {
@@ -222,41 +301,84 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_stream_ker
         const bool gate_vec = a.gate && a.gate_cols != 1;
         float gs = a.y_scale;
         if (a.gate && a.gate_cols == 1) gs *= to_f32(gp[0]);
-        float v[NV * VEC];
+        constexpr int H = VEC / 2;
+        F2 v[NV * H];  // y, then z, then h'
+        const F2 gs2 = pair(gs, gs), hs2 = pair(a.h_scale, a.h_scale), off2 = pair(a.w_offset, a.w_offset);
+        // weights of the activation's type are on their way during the reduction before their use
+        P raw[NV];
+        auto fetch = [&](const void* w) {
+            if (!SAME || !w) return;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (tid + i * step < n_pack) raw[i] = *reinterpret_cast<const P*>(static_cast<const T*>(w) + (size_t)(tid + i * step) * VEC);
+        };
+        auto weights = [&](const void* w, int i, float inv, F2 (&out)[H]) {  // inv * (offset + weight)
+            const F2 inv2 = pair(inv, inv);
+            const int p = tid + i * step;
+            if (SAME) {
+                pairs_of<T, VEC>(raw[i], out);
+            } else {
+                float e[VEC];
+                load_w<T, VEC, false>(w, a.w_type, (size_t)p * VEC, e);
+#pragma unroll
+                for (int j = 0; j < H; ++j) out[j] = pair(e[2 * j], e[2 * j + 1]);
+            }
+#pragma unroll
+            for (int j = 0; j < H; ++j) out[j] = mul2(inv2, add2(off2, out[j]));
+        };
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int p = tid + i * step;
-            P y = {};
-            if (p < n_pack) y = *reinterpret_cast<const P*>(ys + p * VEC);
+            F2 y[H] = {};
+            if (p < n_pack) pairs_of<T, VEC>(*reinterpret_cast<const P*>(ys + p * VEC), y);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[i * VEC + j] = to_f32(y.v[j]);
+            for (int j = 0; j < H; ++j) v[i * H + j] = y[j];
         }
         float inv = 1.0f;
-        if (a.post_norm) inv = inverse_rms<false>(v, inv_cols, eps, red);
+        if (a.post_norm) {
+            fetch(a.post_w);
+            inv = inverse_rms_pairs(v, inv_cols, eps, red);
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int p = tid + i * step;
             if (p < n_pack) {
                 if (a.post_norm) {
-                    float w[VEC];
-                    if (a.post_w) load_w<T, VEC, SAME>(a.post_w, a.w_type, (size_t)p * VEC, w);
+                    F2 w[H];
+                    if (a.post_w) {
+                        weights(a.post_w, i, inv, w);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[i * VEC + j] *= a.post_w ? inv * (a.w_offset + w[j]) : inv;
+                        for (int j = 0; j < H; ++j) w[j] = pair(inv, inv);
+                    }
+#pragma unroll
+                    for (int j = 0; j < H; ++j) v[i * H + j] = mul2(v[i * H + j], w[j]);
                 }
-                const P h = *reinterpret_cast<const P*>(hs + p * VEC);
-                P g = {}, o;
-                if (gate_vec) g = *reinterpret_cast<const P*>(gp + p * VEC);
+                F2 h[H], g[H];
+                pairs_of<T, VEC>(*reinterpret_cast<const P*>(hs + p * VEC), h);
+                if (gate_vec) {
+                    pairs_of<T, VEC>(*reinterpret_cast<const P*>(gp + p * VEC), g);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float x = fmaf(gate_vec ? gs * to_f32(g.v[j]) : gs, v[i * VEC + j], a.h_scale * to_f32(h.v[j]));
-                    v[i * VEC + j] = x;
-                    o.v[j] = from_f32<T>(x);
+                    for (int j = 0; j < H; ++j) g[j] = mul2(gs2, g[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < H; ++j) g[j] = gs2;
+                }
+                P o;
+#pragma unroll
+                for (int j = 0; j < H; ++j) {
+                    v[i * H + j] = fma2(g[j], v[i * H + j], mul2(hs2, h[j]));
+                    put_pair(o.v + 2 * j, v[i * H + j]);
                 }
                 if (a.h_out) *reinterpret_cast<P*>(static_cast<T*>(a.h_out) + (size_t)row * a.h_out_stride + (size_t)p * VEC) = o;
             }
         }
-        if (a.n_out) inv = inverse_rms<false>(v, inv_cols, eps, red);
-        else __syncthreads();
+        if (a.n_out) {
+            fetch(a.pre_w);
+            inv = inverse_rms_pairs(v, inv_cols, eps, red);
+        } else {
+            __syncthreads();
+        }
         // (everyone has read the stage: the reduction above was a barrier)
         if (tid == 0 && ok && row + 2ll * gridDim.x < a.rows) issue(s, (int)(row + 2ll * gridDim.x));
         if (a.n_out) {
@@ -264,15 +386,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_stream_ker
             for (int i = 0; i < NV; ++i) {
                 const int p = tid + i * step;
                 if (p < n_pack) {
-                    float w[VEC];
-                    if (a.pre_w) load_w<T, VEC, SAME>(a.pre_w, a.w_type, (size_t)p * VEC, w);
                     P o;
+                    F2 w[H];
+                    if (a.pre_w) {
+                        weights(a.pre_w, i, inv, w);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        float x = v[i * VEC + j] * inv;
-                        if (a.pre_w) x *= a.w_offset + w[j];
-                        o.v[j] = from_f32<T>(x);
+                        for (int j = 0; j < H; ++j) w[j] = pair(inv, inv);
                     }
+#pragma unroll
+                    for (int j = 0; j < H; ++j) put_pair(o.v + 2 * j, mul2(v[i * H + j], w[j]));
                     *reinterpret_cast<P*>(static_cast<T*>(a.n_out) + (size_t)row * a.n_out_stride + (size_t)p * VEC) = o;
                 }
             }
