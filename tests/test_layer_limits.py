@@ -6,7 +6,7 @@ import torch
 
 import larql_b200
 from test_layer_moe import Layer, check, tokens
-from test_layer_ops import TYPES, U, check_norm, dev, fp8_matrix, fp8_weight, gen, norm_args, norm_case, quantized
+from test_layer_ops import TYPES, U, check_norm, dev, fp8_matrix, fp8_weight, gen, norm_args, norm_case, quantized, run_fp8
 
 gpu = pytest.mark.gpu
 
@@ -192,6 +192,15 @@ def test_fp8_matmul_every_way_of_cutting_it_up(be, case):
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,pad", [(1221, 0), (1216, 3), (1216, 0), (1093, 8)])
+def test_fp8_matmul_of_many_tokens_into_ragged_rows(be, kind, rows, pad):
+    """The kernel for many tokens where a row of the output ends inside a tile or starts at any element: nothing beside the
+    row is written (run_fp8 checks that too)."""
+    run_fp8(be, kind, 1999, 528, rows, seed=rows + pad, out_pad=pad)
+
+
+@gpu
 @pytest.mark.parametrize("tokens_", [3, 140])
 def test_fp8_matmul_offsets_past_32_bits(be, tokens_):
     """Strides that put the last token's activations and outputs past 2^32 bytes."""
@@ -324,3 +333,47 @@ def test_moe_handle_and_its_context():
     b.close()
     layer.layer.close()
     layer.layer.close()
+
+
+@gpu
+@pytest.mark.parametrize("t", [1, 40, 1400])
+def test_a_captured_tail_of_a_decoder_replays_with_new_inputs(be, t):
+    """norm -> layer -> norm -> quantisation -> coded product -> quantising product, captured once and replayed: the bits of
+    the eager calls on the same inputs."""
+    hidden, kind = 1024, "bf16"
+    layer = Layer(be, "mxfp4", hidden, 96, 4, 2, kind, True, True, 3)
+    before = norm_case(t, hidden, kind, kind, False, "none", 0, 4)
+    new = lambda *s, dt=torch.bfloat16: torch.empty(*s, dtype=dt, device="cuda")
+    n1, y, h2, n2, out1, out2 = (new(t, hidden) for _ in range(6))
+    q, s = new(t, hidden, dt=torch.uint8), new(t, hidden // 128, dt=torch.float32)
+    after = dict(norm_case(t, hidden, kind, kind, True, "channel", 0, 7, y_scale=0.8), h=before["h"], y=y)
+    wq, ws = (v.cuda() for v in fp8_weight(gen(6), hidden, hidden))
+    m = fp8_matrix(wq, ws)
+    bf16, e4m3 = larql_b200.T_BF16, larql_b200.T_E4M3
+
+    def calls():
+        assert be.dev_block_norm(norm_args(before, None, n1, use_y=False))
+        assert be.dev_moe_ffn(layer.layer, n1.data_ptr(), bf16, t, y.data_ptr())
+        assert be.dev_block_norm(norm_args(after, h2, n2))
+        assert be.dev_fp8_quantize(n2.data_ptr(), bf16, t, hidden, hidden, q.data_ptr(), s.data_ptr())
+        assert be.dev_fp8_matmul(m, q.data_ptr(), e4m3, t, hidden, out1.data_ptr(), bf16, hidden, s.data_ptr())
+        assert be.dev_fp8_matmul(m, out1.data_ptr(), bf16, t, hidden, out2.data_ptr(), bf16, hidden)
+
+    torch.cuda.synchronize()
+    calls()
+    be.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.ExternalStream(be.stream()), capture_error_mode="thread_local"):
+        calls()
+    for i in range(3):
+        before["h"].copy_(torch.randn(t, hidden, generator=gen(60 + i)))
+        torch.cuda.synchronize()
+        graph.replay()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [v.clone() for v in (n1, y, h2, n2, q, s, out1, out2)]
+        torch.cuda.synchronize()
+        calls()
+        be.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, (n1, y, h2, n2, q, s, out1, out2)))
+        assert out2.isfinite().all() and (out2 != 0).any()
