@@ -53,7 +53,19 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 // either way.
 __device__ __forceinline__ float quotient(float x, float s, float r) {
     const float q = __fmul_rn(x, r);
-    return copysignf(__fmaf_rn(__fmaf_rn(-q, s, x), r, q), x);  // (s > 0; the correction of a zero would drop its sign)
+    return __fmaf_rn(__fmaf_rn(-q, s, x), r, q);
+}
+// Minus the quotients of two elements, two f32 an instruction: with the signs this way round the correction keeps a zero's
+// (x = -0: +0; q itself would lose it).
+__device__ __forceinline__ float2 minus_quotients(float x0, float x1, float s, float r) {
+    float2 n;
+    asm("{\n\t.reg .b64 x, s, r, q, e;\n\t"
+        "mov.b64 x, {%2, %3};\n\tmov.b64 s, {%4, %4};\n\tmov.b64 r, {%5, %5};\n\t"
+        "mul.rn.f32x2 q, x, r;\n\tfma.rn.f32x2 e, q, s, x;\n\tfma.rn.f32x2 q, e, r, q;\n\t"
+        "mov.b64 {%0, %1}, q;\n\t}"
+        : "=f"(n.x), "=f"(n.y)
+        : "f"(x0), "f"(x1), "f"(s), "f"(-r));
+    return n;
 }
 
 // Eight consecutive elements as they lie, their conversion, and the bits of their largest |value| as an f32 (as integers:
@@ -139,12 +151,16 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__
             const float m = block_amax(r[n]);
             float v[8], s;
             values8(r[n], v);
-            uint32_t w[4];
+            uint32_t w[4], flip = 0;
             if (m > 0x1p-90f && m < 0x1p100f) {
                 s = quotient(m, F8_MAX, 1.0f / F8_MAX);  // (a constant, correctly rounded)
                 const float inv = __frcp_rn(s);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = e4m3x2(quotient(v[2 * i], s, inv), quotient(v[2 * i + 1], s, inv));
+                for (int i = 0; i < 4; ++i) {
+                    const float2 n = minus_quotients(v[2 * i], v[2 * i + 1], s, inv);
+                    w[i] = e4m3x2(n.x, n.y);
+                }
+                flip = 0x80808080u;
             } else {  // zero, tiny, huge, infinite or NaN
                 s = max_nan(__fdiv_rn(m, F8_MAX), F8_MIN_SCALE);
 #pragma unroll
@@ -155,11 +171,11 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__
             if (sub == 0) scales[(size_t)t[n] * kb_n + kb[n]] = s;
             uint8_t* q = codes + t[n] * code_pitch + k0;
             if (wide_store) {  // cols (and the pitch) are multiples of 8
-                *reinterpret_cast<uint2*>(q) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+                *reinterpret_cast<uint2*>(q) = make_uint2((w[0] | (w[1] << 16)) ^ flip, (w[2] | (w[3] << 16)) ^ flip);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (k0 + i < cols) q[i] = (uint8_t)(w[i >> 1] >> (8 * (i & 1)));
+                    if (k0 + i < cols) q[i] = (uint8_t)((w[i >> 1] ^ flip) >> (8 * (i & 1)));
             }
         }
     }
