@@ -120,9 +120,9 @@ __device__ __forceinline__ float block_amax(const Eight<T>& r) {
 }
 
 // 16 threads per (token, block of 128), 8 consecutive elements each; QU such blocks are on their way at a time (1 where
-// there are few).  The quotients are the correctly rounded ones (and not x times 1 / s): the codes are defined by them,
-// and the tests hold them to the definition bit for bit.  Instructions bound it, 90 for a thread's eight elements: 4096 x 8192
-// bf16 take 26 us, 3.8 TB/s of the 102 MB it reads and writes.
+// there are few, else 2: 4096 x 8192 bf16 24.1 us, with 4 25.5, with 8 33.3).  The quotients are the correctly rounded ones
+// (and not x times 1 / s): the codes are defined by them, and the tests hold them to the definition bit for bit.
+// Instructions bound it, about 80 for a thread's eight elements: 4.2 TB/s of the 102 MB it reads and writes.
 template <class T, bool VEC, int QU>
 __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__ x, long long x_stride, int units, int kb_n,
                                                            int cols, uint8_t* __restrict__ codes, long long code_pitch,
@@ -763,10 +763,10 @@ cudaError_t launch_fp8_quantize(const void* x, int type, size_t tokens, size_t c
             return go((__half*)nullptr, vtag, qtag);
         };
         using One = std::integral_constant<int, 1>;
-        using Four = std::integral_constant<int, 4>;
+        using Two = std::integral_constant<int, 2>;
         cudaError_t e;
         if (!vec) e = by_type(std::false_type{}, One{});
-        else if (units >= sm_count * 64) e = by_type(std::true_type{}, Four{});
+        else if (units >= sm_count * 64) e = by_type(std::true_type{}, Two{});
         else e = by_type(std::true_type{}, One{});
         if (e != cudaSuccess) return e;
     }
