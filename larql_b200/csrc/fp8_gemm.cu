@@ -122,7 +122,7 @@ __device__ __forceinline__ float block_amax(const Eight<T>& r) {
 // 16 threads per (token, block of 128), 8 consecutive elements each; QU such blocks are on their way at a time (1 where
 // there are few, else 2: 4096 x 8192 bf16 24.1 us, with 4 25.5, with 8 33.3).  The quotients are the correctly rounded ones
 // (and not x times 1 / s): the codes are defined by them, and the tests hold them to the definition bit for bit.
-// Instructions bound it, about 80 for a thread's eight elements: 4.2 TB/s of the 102 MB it reads and writes.
+// Instructions bound it, 142 for a thread's eight elements: 4.2 TB/s of the 102 MB it reads and writes.
 template <class T, bool VEC, int QU>
 __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__ x, long long x_stride, int units, int kb_n,
                                                            int cols, uint8_t* __restrict__ codes, long long code_pitch,
