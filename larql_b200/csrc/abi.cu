@@ -2365,7 +2365,7 @@ int lq_dev_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const void* x, int x_type
     if (coded && (((uintptr_t)x & 15) || (tokens > 1 && (x_stride & 15))))
         return fail(ctx, LQ_ERR_ARGUMENT, "fp8_matmul: e4m3 activations need 16-byte aligned rows");
     if (cols == 0) {
-        CK(cudaMemset2DAsync(out, out_stride * oz, 0, rows * oz, tokens, ctx->stream));
+        CK(cudaMemset2DAsync(out, std::max(out_stride, rows) * oz, 0, rows * oz, tokens, ctx->stream));  // (one token: any stride)
         return LQ_OK;
     }
     const size_t kb = (cols + 127) / 128, chunk = 32768;  // (bounds the codes' workspace)

@@ -201,6 +201,20 @@ def test_fp8_matmul_of_many_tokens_into_ragged_rows(be, kind, rows, pad):
 
 
 @gpu
+def test_fp8_matmul_of_nothing(be):
+    """No columns: zeros, for one token whatever its strides; no tokens, no rows: nothing."""
+    for t, stride in ((1, 0), (1, 7), (3, 6)):
+        out = torch.full((t, 6), 9.0, dtype=torch.bfloat16, device="cuda")
+        torch.cuda.synchronize()
+        m = larql_b200.DeviceMatrix(larql_b200.FMT_FP8_B128, 5, 0, 0, 0)
+        assert be.dev_fp8_matmul(m, 0, larql_b200.T_BF16, t, 0, out.data_ptr(), larql_b200.T_BF16, stride)
+        be.synchronize()
+        assert (out[:, :5] == 0).all() and (out[:, 5] == 9).all()
+        assert be.dev_fp8_matmul(m, 0, larql_b200.T_BF16, 0, 0, 0, larql_b200.T_BF16, 0)
+        assert be.dev_fp8_matmul(larql_b200.DeviceMatrix(larql_b200.FMT_FP8_B128, 0, 16, 0, 0), 0, larql_b200.T_BF16, t, 16, 0, larql_b200.T_BF16, 0)
+
+
+@gpu
 @pytest.mark.parametrize("tokens_", [3, 140])
 def test_fp8_matmul_offsets_past_32_bits(be, tokens_):
     """Strides that put the last token's activations and outputs past 2^32 bytes."""
