@@ -448,6 +448,8 @@ LQ_API int lq_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const float* x, size_t
  * lq_dev_moe_ffn x, out [tokens, hidden] of type (LQ_T_F32 / BF16 / F16; out may be x); idx_out, w_out [tokens,
  *                min(top_e, n_experts)] may be NULL.  Calls on one handle run one after another on the stream.
  * lq_moe_ffn     the same with host pointers, f32 (the handle's matrices stay on the device).
+ * Both products take their activations in two f16 terms, off by at most 2^-23 of the value plus 2^-39 of the token's largest
+ * (a bf16 x in one: 2^-39 alone); nothing between them is rounded to the layer's type.
  * A token with a NaN or infinity gets NaN outputs and weights; the other tokens are not touched by it. */
 typedef struct lq_moe lq_moe;
 LQ_API int lq_moe_create(lq_ctx* ctx, const lq_matrix* gates, const lq_matrix* ups, const lq_matrix* downs, size_t n_experts,

@@ -263,7 +263,7 @@ struct MoeLayer {
     // counters, zero between launches: CTAs gone, router products done, down units done, gate/up units done per token
     // group of an expert; bits of the largest |value| per token / pair
     unsigned *exits, *route_done, *down_done, *group_done, *x_max, *act_max;
-    int terms;                       // f16 terms per activation (filled in by the launch)
+    int x_terms, group;              // f16 terms per element of x, tokens per group (filled in by the launch)
     int n_stages, stage_bytes, scale_slots[2], finish, chunk[2], n_chunks[2];  // filled in by the launch
     int* err;
 };

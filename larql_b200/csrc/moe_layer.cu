@@ -22,11 +22,14 @@
 //
 // The products run on the tensor cores (mma.sync m16n8k16, f16 x f16 -> f32): weights are the 16 rows of A, tokens the 8
 // columns of B.  The codes of all three formats are exact in f16.  An activation is brought to [2^14, 2^15) by a
-// power of two per token; bf16 layers take one f16 term (all of a bf16's bits; activations between the products
-// rounded to f16's 11), f32 and f16 layers two (22 bits, a column each).  Scales: e8m0 (per row and 32) and
-// FP8 blocks multiply the f32 sums of 32 products, e4m3 (per row and 16) the f16 codes, which is exact (2 + 4 bits).
-// Measured: 32 MXFP4 experts of 2880 x 2880, 4 a token: 16 bf16 tokens 107 us for 373 MB, 3.5 TB/s; one f32 token 35 us for
-// 53 MB.  64 FP8 experts of 3840 x 800, 6 a token: 37 bf16 tokens 169 us for 576 MB, 3.4 TB/s.  The copies alone take 55, 9
+// power of two per token and held as two f16 terms (22 bits), in both products and for every type; only a bf16 x takes a
+// single one, which has all of its bits.  The terms are a column each, or, where a bf16 layer's group has too many tokens
+// for that behind gate/up, two sets of columns multiplied one after the other into the same sums.  Scales: e8m0 (per row
+// and 32) and FP8 blocks multiply the f32 sums of 32 products, e4m3 (per row and 16) the f16 codes, which is exact (2 + 4
+// bits).  (One term between the products of a bf16 layer: 106 and 167 us for the two cases of several tokens below, and f16's
+// 11 bits of an activation.)
+// Measured: 32 MXFP4 experts of 2880 x 2880, 4 a token: 16 bf16 tokens 112 us for 373 MB, 3.3 TB/s; one f32 token 35 us for
+// 53 MB.  64 FP8 experts of 3840 x 800, 6 a token: 37 bf16 tokens 179 us for 576 MB, 3.2 TB/s.  The copies alone take 55, 9
 // and 93 us: the compute warps' conversions and latencies bound it (integer pipe 51 %, an instruction in 58 % of the
 // cycles, tensor pipe 19 %), and for one token the routing's exchange between the CTAs and the two phases' starts.
 // (Tried: e4m3 terms and m16n8k32 e4m3 products, which need no conversion of FP8 codes: that form is converted to f16
@@ -53,8 +56,8 @@ struct MlSmem {
     uint64_t full[ML_MAX_STAGES], empty[ML_MAX_STAGES];
     uint64_t rfull[ML_FINISH], rempty[ML_FINISH];  // partial sums of a unit: written by every compute warp / read
     float2 part[ML_THREADS / 32];
-    float unscale[16];          // per token of the group: the power of two its values were divided by
-    int gtok[16], gpair[16];    // the group's tokens and (token, slot) pairs
+    float unscale[8];           // per token of the group: the power of two its values were divided by
+    int gtok[8], gpair[8];      // the group's tokens and (token, slot) pairs
     int n_groups, cnt;
     unsigned x_bits;            // one token: its largest |value|
     int active[MOE_LAYER_MAX_EXPERTS];
@@ -218,6 +221,17 @@ __host__ __device__ constexpr int row_scale_bytes(int cols) {
 }
 // Distance of two columns of the activations: two columns (a phase of a 16-byte load) fall into different banks.
 __host__ __device__ constexpr int act_pitch(int k) { return (2 * k) % 128 == 0 ? 2 * k + 64 : 2 * k; }
+// Columns per activation of a group of cnt tokens: x has x_terms, the activation between the products two if `nt` tiles of
+// eight hold them (else one, and its second term lies in a second set of columns).
+__host__ __device__ constexpr int group_terms(int nt, int cnt, bool down, int x_terms) {
+    return down ? (2 * cnt <= 8 * nt ? 2 : 1) : x_terms;
+}
+// Bytes of a group's columns, whole tiles of eight, of one phase or the other.
+__host__ __device__ constexpr int act_bytes(int nt, int x_terms, int group, int hidden, int inter) {
+    const int x = (group * x_terms + 7) / 8 * 8 * act_pitch(hidden);
+    const int a = (group_terms(nt, group, true, x_terms) == 2 ? 1 : 2) * nt * 8 * act_pitch(inter);
+    return x > a ? x : a;
+}
 // Columns of the contraction per stage: equal parts of at most 46 blocks of 32 (22 for FP8, and for long rows, whose
 // activations take most of shared memory), an even number of them.  A stage holds one block more of every row, back to
 // back as the tile copy lays them: an odd number of 16-byte pieces per row puts the eight rows of a fragment load into
@@ -260,9 +274,9 @@ __device__ __forceinline__ Walk walk_of(const MoeLayer& L, bool down, int n_grou
     return w;
 }
 
-// Eight activations times a power of two, into columns of f16: one term, or a value and its rest.
+// Eight activations times a power of two, into columns of f16: one term, or a value and its rest `rest` bytes on.
 template <int FMT>
-__device__ __forceinline__ void put_columns(const float (&v)[8], float scale, int terms, uint8_t* dst, int xpitch, int k) {
+__device__ __forceinline__ void put_columns(const float (&v)[8], float scale, uint8_t* dst, int rest, int k) {
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -278,13 +292,13 @@ __device__ __forceinline__ void put_columns(const float (&v)[8], float scale, in
         uint8_t* q = dst + 2 * (k & ~31) + ((k & 15) >> 2) * 16 + ((k >> 4) & 1) * 8;
         *reinterpret_cast<uint2*>(q) = make_uint2(hi[0], hi[1]);
         *reinterpret_cast<uint2*>(q + 16) = make_uint2(hi[2], hi[3]);
-        if (terms == 2) {
-            *reinterpret_cast<uint2*>(q + xpitch) = make_uint2(lo[0], lo[1]);
-            *reinterpret_cast<uint2*>(q + xpitch + 16) = make_uint2(lo[2], lo[3]);
+        if (rest) {
+            *reinterpret_cast<uint2*>(q + rest) = make_uint2(lo[0], lo[1]);
+            *reinterpret_cast<uint2*>(q + rest + 16) = make_uint2(lo[2], lo[3]);
         }
     } else {
         *reinterpret_cast<uint4*>(dst + 2 * k) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (terms == 2) *reinterpret_cast<uint4*>(dst + xpitch + 2 * k) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (rest) *reinterpret_cast<uint4*>(dst + rest + 2 * k) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
 }
 // The power of two that brings values of at most |bits| to [2^14, 2^15), and the one that takes it back (kept where both
@@ -361,7 +375,8 @@ __device__ void route_token(const MoeLayer& L, MlSmem& sh, int t, int lane) {
     }
 }
 
-template <int FMT, int NT>
+// SETS: groups may have a second set of columns (a kernel of its own: the others would pay 2 to 9 us for the registers).
+template <int FMT, int NT, bool SETS>
 __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_constant__ MoeLayer L) {
     extern __shared__ __align__(128) uint8_t smem[];
     constexpr int RED = NT * 8 * 16;  // floats of a warp's partial sums of 16 rows
@@ -369,14 +384,14 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
     uint8_t* p = smem + (sizeof(MlSmem) + 127) / 128 * 128;
     float* red = reinterpret_cast<float*>(p);                 // [finish][ML_WARPS][2 tiles][RED]
     p += L.finish * ML_WARPS * 2 * RED * 4;
-    uint8_t* xs = p;                                          // [NT * 8] columns of f16
-    p += (size_t)NT * 8 * max(act_pitch(L.hidden), act_pitch(L.inter));
+    uint8_t* xs = p;                                          // a group's columns of f16
+    p += act_bytes(NT, L.x_terms, L.group, L.hidden, L.inter);
     uint8_t* sbuf = p;                                        // scales of the units' rows, [scale_slots] per phase
     p += 32 * (L.scale_slots[0] * row_scale_bytes<FMT>(L.hidden) + L.scale_slots[1] * row_scale_bytes<FMT>(L.inter));
     uint8_t* ring = smem + (p - smem + 127) / 128 * 128;      // [n_stages][32 rows]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int T = L.tokens, E = L.experts, K = L.top_e;
-    const int terms = L.terms, TG = NT * 8 / terms;  // columns and tokens per group
+    const int TG = L.group;  // tokens per group
     const bool x_wide = (reinterpret_cast<uintptr_t>(L.x) & 15) == 0;  // (rows are multiples of 32 elements)
 
     if (tid == 0) {
@@ -478,7 +493,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                 const int k = (tid + q * ML_THREADS) * 8;
                 if (k >= L.hidden) continue;
                 to_f32(raw[q], L.type, v);
-                put_columns<FMT>(v, down_scale(bits), L.terms, xs, act_pitch(L.hidden), k);
+                put_columns<FMT>(v, down_scale(bits), xs, L.x_terms == 2 ? act_pitch(L.hidden) : 0, k);
             }
         }
         if (tid == 0 && !wait_count(L.route_done, (unsigned)items)) sh.failed = 1;
@@ -620,6 +635,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     if (lane < cnt) pair = sh.gpair[lane];  // (lane i publishes what belongs to token i of the group)
                     const float* all = red + buf * ML_WARPS * 2 * RED;
                     // eight columns at a time, a lane four rows of one column in both tiles; a token's two terms lie in two columns
+                    const int terms = group_terms(NT, cnt, w.is_down, L.x_terms);
                     const int col = lane >> 2, quad = lane & 3, per_tile = 8 / terms;
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
@@ -677,6 +693,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
             const int b0 = pairs && !F8 ? 2 * warp : warp;
             const int tile2 = pairs ? 0 : 16 * w.pitch, scale2 = pairs ? 1 : 16 * srow;
             int cur = -1, cols = 0, slot = 0;
+            uint32_t rest = 0;  // distance of the second set of columns (0: there is none)
             for (int u = ua; u < ub; ++u, ++tile) {
                 if (tile == w.units_per_group) {
                     ++gi, tile = 0;
@@ -689,7 +706,9 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     const int first = (gi - sh.gpre[a]) * TG;
                     const unsigned long long m0 = sh.mask[e][0] | ((unsigned long long)sh.mask[e][1] << 32);
                     const int cnt = min(TG, __popcll(m0) - first);
+                    const int terms = group_terms(NT, cnt, w.is_down, L.x_terms);
                     cols = (cnt * terms + 7) / 8;
+                    if (SETS) rest = w.is_down && terms == 1 ? NT * 8 * xpitch : 0;
                     // the finishers are done with the previous group's units, the compute warps with its activations
                     for (int v = 0; v < L.finish; ++v)
                         if (ok) ok = __all_sync(0xffffffffu, ml_wait<false>(&sh.rempty[v], v < rb ? rlap : rlap ^ 1u));
@@ -708,7 +727,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     if (w.is_down && tid == 0 && ok && !wait_count(L.group_done + gi, (unsigned)(L.inter / 16))) sh.failed = 1;
                     consumers_sync();
                     // the warps share the rows out: `per` warps a token
-                    const int per = cnt >= 9 ? 1 : (cnt >= 5 ? 2 : (cnt >= 3 ? 4 : (cnt == 2 ? 8 : 16)));
+                    const int per = cnt >= 5 ? 2 : (cnt >= 3 ? 4 : (cnt == 2 ? 8 : 16));
                     const int i = warp / per, part = (warp % per) * 32 + lane;
                     if (i < cnt && !(T == 1 && ph == 0)) {  // (a single token's columns were made while the routing was on its way)
                         const void* src = w.is_down ? L.act : L.x;
@@ -728,7 +747,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                             to_f32(next[0], type, v);
                             next[0] = next[1];
                             if (k + per * 512 < w.k) next[1] = fetch(k + per * 512);
-                            put_columns<FMT>(v, scale, terms, xs + (size_t)(i * terms) * xpitch, xpitch, k);
+                            put_columns<FMT>(v, scale, xs + (size_t)(i * terms) * xpitch, terms == 2 ? xpitch : (int)rest, k);
                         }
                     }
                     consumers_sync();
@@ -759,9 +778,10 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     const uint32_t sa = s0 + (FMT == LQ_FMT_NVFP4 ? 2 * (kb0 + b0) + (t4 >> 1) : kb0 + b0), sb = sa + 8 * srow;
                     const uint32_t sc = sa + (FMT == LQ_FMT_NVFP4 && pairs ? 2 : scale2), sd = sc + 8 * srow;
                     const uint32_t xa = xcol + (uint32_t)((kb0 + b0) * 64);
-                    // one step: block b0 + at of both tiles (PAIRS: blocks b0 + at and, `two`, b0 + at + D2 of the one tile)
-                    auto step = [&](auto pairs_tag, int at, bool two) {
-                        constexpr bool PAIRS = decltype(pairs_tag)::value;
+                    // one step: block b0 + at of both tiles (PAIRS: blocks b0 + at and, `two`, b0 + at + D2 of the one tile), with
+                    // the second set of columns (SECOND)
+                    auto step = [&](auto second_tag, auto pairs_tag, int at, bool two) {
+                        constexpr bool PAIRS = decltype(pairs_tag)::value, SECOND = decltype(second_tag)::value;
                         constexpr int D2 = PAIRS ? (F8 ? ML_WARPS : 1) : 0;
                         // lo and hi: the f16 pairs of rows g and g + 8 of the first and the second block
                         uint32_t lo[2][4], hi[2][4];
@@ -817,12 +837,26 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                                 mma_f16(acc2[j], lo[1][0], hi[1][0], lo[1][1], hi[1][1], x1.x, x1.y);
                                 mma_f16(acc[j], lo[0][2], hi[0][2], lo[0][3], hi[0][3], x0.z, x0.w);
                                 mma_f16(acc2[j], lo[1][2], hi[1][2], lo[1][3], hi[1][3], x1.z, x1.w);
+                                if (SECOND) {
+                                    const uint4 y0 = lds_128(xj + rest), y1 = PAIRS ? lds_128(xj + d2 * 64 + rest) : y0;
+                                    mma_f16(acc[j], lo[0][0], hi[0][0], lo[0][1], hi[0][1], y0.x, y0.y);
+                                    mma_f16(acc2[j], lo[1][0], hi[1][0], lo[1][1], hi[1][1], y1.x, y1.y);
+                                    mma_f16(acc[j], lo[0][2], hi[0][2], lo[0][3], hi[0][3], y0.z, y0.w);
+                                    mma_f16(acc2[j], lo[1][2], hi[1][2], lo[1][3], hi[1][3], y1.z, y1.w);
+                                }
                             } else {
                                 float d[4], h[4];
                                 mma_f16_new(d, lo[0][0], hi[0][0], lo[0][1], hi[0][1], x0.x, x0.y);
                                 mma_f16_new(h, lo[1][0], hi[1][0], lo[1][1], hi[1][1], x1.x, x1.y);
                                 mma_f16(d, lo[0][2], hi[0][2], lo[0][3], hi[0][3], x0.z, x0.w);
                                 mma_f16(h, lo[1][2], hi[1][2], lo[1][3], hi[1][3], x1.z, x1.w);
+                                if (SECOND) {
+                                    const uint4 y0 = lds_128(xj + rest), y1 = PAIRS ? lds_128(xj + d2 * 64 + rest) : y0;
+                                    mma_f16(d, lo[0][0], hi[0][0], lo[0][1], hi[0][1], y0.x, y0.y);
+                                    mma_f16(h, lo[1][0], hi[1][0], lo[1][1], hi[1][1], y1.x, y1.y);
+                                    mma_f16(d, lo[0][2], hi[0][2], lo[0][3], hi[0][3], y0.z, y0.w);
+                                    mma_f16(h, lo[1][2], hi[1][2], lo[1][3], hi[1][3], y1.z, y1.w);
+                                }
 #pragma unroll
                                 for (int q = 0; q < 4; ++q) {
                                     acc[j][q] = fmaf(d[q], q < 2 ? f0[0] : f1[0], acc[j][q]);
@@ -832,17 +866,22 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                         }
                     };
                     const int left = blocks - b0;  // (at most 46 blocks a stage, 22 for FP8)
-                    if (!pairs) {
+                    auto steps = [&](auto second) {
+                        if (!pairs) {
 #pragma unroll
-                        for (int i = 0; i < (F8 ? 2 : 3); ++i)
-                            if (i * ML_WARPS < left) step(std::false_type{}, i * ML_WARPS, true);
-                    } else if (F8) {
-                        if (left > 0) step(std::true_type{}, 0, left > ML_WARPS);
-                    } else {
+                            for (int i = 0; i < (F8 ? 2 : 3); ++i)
+                                if (i * ML_WARPS < left) step(second, std::false_type{}, i * ML_WARPS, true);
+                        } else if (F8) {
+                            if (left > 0) step(second, std::true_type{}, 0, left > ML_WARPS);
+                        } else {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            if (i * 2 * ML_WARPS < left) step(std::true_type{}, i * 2 * ML_WARPS, left > i * 2 * ML_WARPS + 1);
-                    }
+                            for (int i = 0; i < 2; ++i)
+                                if (i * 2 * ML_WARPS < left) step(second, std::true_type{}, i * 2 * ML_WARPS, left > i * 2 * ML_WARPS + 1);
+                        }
+                    };
+                    // (apart: a branch inside a step would keep it from overlapping with the next)
+                    if (SETS && rest) steps(std::integral_constant<bool, SETS>{});
+                    else steps(std::false_type{});
                     __syncwarp();
                     if (lane == 0) ml_arrive(&sh.empty[st]);
                     if (++st == L.n_stages) st = 0, lap ^= 1u;
@@ -905,9 +944,9 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
 }
 
 // Shared memory beside the ring and the scales, a unit's scales, a stage.
-size_t fixed_smem(int nt, int finish, int hidden, int inter) {
+size_t fixed_smem(int nt, int finish, int x_terms, int group, int hidden, int inter) {
     return 128 + (sizeof(MlSmem) + 127) / 128 * 128 + finish * (size_t)ML_WARPS * 2 * nt * 8 * 16 * 4 +
-           (size_t)nt * 8 * std::max(act_pitch(hidden), act_pitch(inter));
+           (size_t)act_bytes(nt, x_terms, group, hidden, inter);
 }
 template <int FMT>
 int stage_size(int hidden, int inter) {
@@ -922,14 +961,14 @@ struct Plan {
 // The most stages that fit, with fewer finishers where that leaves under three.  Between a unit's first stage and the stage it
 // replaces lie at most stages / chunks units of a phase: so many slots its scales need, and one.
 template <int FMT>
-Plan plan_ring(int nt, int hidden, int inter) {
+Plan plan_ring(int nt, int x_terms, int group, int hidden, int inter) {
     auto chunks = [](int k) { return (k + chunk_cols<FMT>(k) - 1) / chunk_cols<FMT>(k); };
     Plan p = {};
     for (int finish = ML_FINISH; finish >= 1; --finish) {
         for (int n = ML_MAX_STAGES; n >= 2; --n) {
             const int slots[2] = {(n + chunks(hidden) - 1) / chunks(hidden) + 1, (n + chunks(inter) - 1) / chunks(inter) + 1};
             const size_t scales = 32 * ((size_t)slots[0] * row_scale_bytes<FMT>(hidden) + (size_t)slots[1] * row_scale_bytes<FMT>(inter));
-            const size_t bytes = fixed_smem(nt, finish, hidden, inter) + scales + (size_t)n * stage_size<FMT>(hidden, inter);
+            const size_t bytes = fixed_smem(nt, finish, x_terms, group, hidden, inter) + scales + (size_t)n * stage_size<FMT>(hidden, inter);
             if (bytes <= 227 * 1024) {
                 if (n > p.stages) p = Plan{n, finish, {slots[0], slots[1]}, bytes};
                 break;
@@ -940,9 +979,9 @@ Plan plan_ring(int nt, int hidden, int inter) {
     return p;
 }
 
-template <int FMT, int NT>
+template <int FMT, int NT, bool SETS>
 cudaError_t launch_layer(MoeLayer L, int sm_count, cudaStream_t st) {
-    const Plan p = plan_ring<FMT>(NT, L.hidden, L.inter);
+    const Plan p = plan_ring<FMT>(NT, L.x_terms, L.group, L.hidden, L.inter);
     if (p.stages == 0) return cudaErrorInvalidConfiguration;
     L.n_stages = p.stages, L.finish = p.finish, L.scale_slots[0] = p.slots[0], L.scale_slots[1] = p.slots[1];
     L.stage_bytes = stage_size<FMT>(L.hidden, L.inter);
@@ -951,7 +990,7 @@ cudaError_t launch_layer(MoeLayer L, int sm_count, cudaStream_t st) {
         L.chunk[i] = chunk_cols<FMT>(k);
         L.n_chunks[i] = (k + L.chunk[i] - 1) / L.chunk[i];
     }
-    const void* fn = (const void*)moe_layer_kernel<FMT, NT>;
+    const void* fn = (const void*)moe_layer_kernel<FMT, NT, SETS>;
     cudaError_t e = set_max_dyn_smem(fn, 227 * 1024);
     if (e != cudaSuccess) return e;
     void* args[] = {&L};
@@ -960,19 +999,29 @@ cudaError_t launch_layer(MoeLayer L, int sm_count, cudaStream_t st) {
 
 template <int FMT>
 cudaError_t launch_fmt(MoeLayer L, int sm_count, cudaStream_t st) {
-    L.terms = L.type == LQ_T_BF16 ? 1 : 2;
-    // Two tiles of columns when an expert's tokens are likely to fill more than one (an expert with more tokens than a
-    // group holds is read once per group) and shared memory takes them beside a ring that covers the memory's latency.
-    int nt = L.tokens * L.top_e * L.terms > 5 * L.experts && L.tokens * L.terms > 8 ? 2 : 1;
-    if (nt > 1 && (size_t)plan_ring<FMT>(nt, L.hidden, L.inter).stages * stage_size<FMT>(L.hidden, L.inter) < 48 * 1024) nt = 1;
-    return nt == 1 ? launch_layer<FMT, 1>(L, sm_count, st) : launch_layer<FMT, 2>(L, sm_count, st);
+    L.x_terms = L.type == LQ_T_BF16 ? 1 : 2;
+    // a ring that covers the memory's latency beside the columns of a group
+    auto room = [&](int nt, int group) {
+        return (size_t)plan_ring<FMT>(nt, L.x_terms, group, L.hidden, L.inter).stages * stage_size<FMT>(L.hidden, L.inter) >= 48 * 1024;
+    };
+    // An expert with more tokens than a group holds is read once per group.  Groups of 8 instead of 4 tokens when an expert's
+    // tokens are likely to be more than 4 and shared memory takes them: by a second tile of columns, or for bf16 layers by a
+    // second set of them between the products.  Measured with 4 | 8, bf16 tokens on 32 MXFP4 experts of 2880 x 2880, 4 a
+    // token: 16 tokens 112 | 119 us, 24 141 | 138, 64 248 | 190.  (Groups of 16, with both, gain here and lose there:
+    // 8 NVFP4 experts of 2048 x 1024, 4 a token, 64 tokens 76 against 82 us, 16 tokens 49 against 45.)
+    const bool eight = 2 * L.tokens * L.top_e > 5 * L.experts && L.tokens > 4;
+    L.group = 8;
+    if (L.x_terms == 2 && eight && room(2, 8)) return launch_layer<FMT, 2, false>(L, sm_count, st);
+    if (L.x_terms == 1 && eight && room(1, 8)) return launch_layer<FMT, 1, true>(L, sm_count, st);
+    L.group = 4;
+    return launch_layer<FMT, 1, false>(L, sm_count, st);
 }
 
 }  // namespace
 
 template <int FMT>
 static bool fits(int hidden, int inter) {
-    return plan_ring<FMT>(1, hidden, inter).stages > 0;
+    return plan_ring<FMT>(1, 2, 4, hidden, inter).stages > 0;
 }
 bool moe_layer_supported(int fmt, int hidden, int inter) {
     if (hidden <= 0 || inter <= 0 || hidden % 32 || inter % 32 || hidden > 8192 || inter > 8192) return false;
