@@ -436,7 +436,8 @@ LQ_API int lq_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const float* x, size_t
 /* A whole mixture-of-experts layer for a few tokens, one launch per 64 tokens (cpu_moe_forward,
  * crates/larql-compute/src/cpu/ops/moe/forward.rs:24-140, over dense experts and with the router's product):
  *     logits = x . router^T + bias; the top_e experts by logit (ties to the lower index), softmax weights over all
- *     experts, renormalised over the selected when renormalise != 0;
+ *     experts, renormalised over the selected when renormalise != 0 (a bias of -inf masks an expert: weight 0; an expert
+ *     whose logit is NaN comes last);
  *     out_t = sum_j w_tj down_j (silu(gate_j x_t) * (up_j x_t)), j in selection order.
  * lq_moe_create  gates, ups [inter, hidden] and downs [hidden, inter] (NOT feature-major), n_experts of each, all of
  *                one format (MXFP4, NVFP4, FP8_B128) and device resident (LQ_MAT_DEVICE), codes and FP4 scales 16-byte

@@ -465,7 +465,8 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
             }
             if (on && warp % W == 0 && lane == 0) {
                 if (L.bias) s = pair_add(s, ld_as_f32(L.bias, L.router_type, e));
-                L.logits[it] = __fadd_rn(s.x, s.y);
+                // (the errors of a sum that left f32's range, as with a bias of -inf that masks an expert, are NaN)
+                L.logits[it] = fabsf(s.x) < INFINITY ? __fadd_rn(s.x, s.y) : s.x;
                 add_release(L.route_done, 1u);
             }
         }

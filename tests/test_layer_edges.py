@@ -1,10 +1,12 @@
 """The layer operators at the edges of their types.  The tolerances are those of the operators' own tests (test_layer_ops,
 test_layer_moe), or derived where they stand."""
+import copy
+
 import pytest
 import torch
 
 import larql_b200
-from test_layer_moe import Layer
+from test_layer_moe import Layer, tokens
 from test_layer_ops import TYPES, U, gen, half_step
 
 gpu = pytest.mark.gpu
@@ -49,3 +51,48 @@ def test_layer_keeps_its_activation(be, fmt, hidden, inter, experts, t, kind):
         act = a * torch.sigmoid(a) * (x[i].double() @ up.t())
         want, small = act @ down.t(), act.abs().max() * 2.0 ** -39 * down.abs().sum(1)
         assert ((out[i].cpu().double() - want).abs() <= half_step(kind, want) + (16 * U * want.abs() + small) * (1 + 2.0 ** -8)).all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("mask", ["inf", "lowest"])
+def test_masked_experts_weigh_nothing(be, kind, renorm, mask):
+    """Experts switched off by a bias of minus infinity, or of the type's lowest value: weight 0, and the others as if they were
+    alone, with fewer and with more experts a token than there are unmasked ones."""
+    off = [1, 2, 4, 5, 6]
+    on = [0, 3, 7]
+    low = -float("inf") if mask == "inf" else torch.finfo(TYPES[kind][0]).min
+    for top_e, t in [(2, 1), (2, 9), (6, 9), (8, 40)]:
+        layer = Layer(be, "mxfp4", 64, 64, 8, top_e, kind, True, renorm, seed=3)
+        layer.bias[off] = low
+        x = tokens(gen(t), t, 64, kind)
+        out, idx, w = layer.run(be, x)
+        alone = copy.copy(layer)
+        alone.w = [[per[e] for e in on] for per in layer.w]
+        alone.router, alone.bias, alone.experts, alone.k = layer.router[on], layer.bias[on], 3, min(top_e, 3)
+        want, widx, ww, w_off, o = alone.want(x)
+        logits = (x.cpu().double() @ layer.router.cpu().double().t() + layer.bias.cpu().double()).float().double()
+        assert torch.equal(idx.cpu().long(), torch.argsort(-logits, dim=1, stable=True)[:, :layer.k])
+        assert torch.equal(idx[:, :alone.k].cpu().long(), torch.tensor(on)[widx])
+        assert ((w[:, :alone.k].cpu().double() - ww).abs() <= w_off + U * ww).all()
+        assert (w[:, alone.k:] == 0).all()
+        err = (out[:t].cpu().double() - want).abs()
+        assert (err <= half_step(kind, want) + o * (1 + 2.0 ** -8) + 1e-44).all()
+        assert (out[t:] == 3).all()
+
+
+@gpu
+@pytest.mark.parametrize("renorm", [True, False])
+def test_layer_with_every_expert_masked_is_nan(be, renorm):
+    """softmax over minus infinities alone; a token with an infinity stays NaN beside masked experts."""
+    layer = Layer(be, "mxfp4", 64, 64, 4, 2, "f32", True, renorm, seed=3)
+    layer.bias[1:3] = -float("inf")
+    x = tokens(gen(2), 3, 64, "f32")
+    x[1, 7] = float("inf")
+    out, _, w = layer.run(be, x)
+    assert out[1].isnan().all() and w[1].isnan().all()
+    assert out[[0, 2]].isfinite().all() and w[[0, 2]].isfinite().all()
+    layer.bias[:] = -float("inf")
+    out, _, w = layer.run(be, tokens(gen(2), 3, 64, "f32"))
+    assert out[:3].isnan().all() and w.isnan().all()
