@@ -9,10 +9,11 @@
 //
 // What bounds it is reading h, y, gate and writing h', n once (one token: the two reductions' latency).  Everything is
 // kept in f32 between the loads and the stores, n is taken from the unrounded h'.  A row's squares are summed in f32,
-// pairwise over the threads; when that sum leaves f32's range the row is summed again relative to its largest value
+// pairwise over the threads; when that sum leaves f32's range the row is summed again at 2^-80 of its size
 // (f64 sums, which need no branch, cost 36 us of 159 at 4096 x 8192 bf16: the conversions run at a few lanes a cycle).
 // Underflow needs no branch: what a square loses is below 2^-149 and eps is at least 2^-126.
-// rms is at least sqrt(eps) >= 2^-63, so 1 / rms is a normal f32 and one multiply per element replaces a division.
+// rms is at least sqrt(eps) >= 2^-63; rows with an rms above 2^100 are scaled down before 1 / rms is taken of them, so that
+// it is a normal f32 far from the type's end and one multiply per element replaces a division.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -63,12 +64,11 @@ __device__ __forceinline__ void load_w(const void* w, int type, size_t at, float
     }
 }
 
-// Over the threads of a row, one warp (WARP) or the whole block: the sum, or the maximum of non-negative values.
-template <bool WARP, bool MAX>
-__device__ __forceinline__ float row_reduce(float s, float* red) {
-    auto op = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
+// The sum over the threads of a row, one warp (WARP) or the whole block.
+template <bool WARP>
+__device__ __forceinline__ float row_sum(float s, float* red) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s = op(s, __shfl_xor_sync(0xffffffffu, s, o));
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (WARP) return s;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockDim.x >> 5;
     __syncthreads();  // the previous result has been read
@@ -76,38 +76,43 @@ __device__ __forceinline__ float row_reduce(float s, float* red) {
     __syncthreads();
     s = lane < n ? red[lane] : 0.0f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s = op(s, __shfl_xor_sync(0xffffffffu, s, o));
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s;
 }
 
-// inverse_rms for a row whose squares' sum s left f32's range (or is NaN).
-template <bool WARP, int N>
-__device__ __forceinline__ float inverse_rms_beyond(const float (&v)[N], float s, float inv_cols, float eps, float* red) {
-    if (s != s) return s;
-    float m = 0.0f;  // (the same for every thread of the row)
-#pragma unroll
-    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(v[i]));
-    m = row_reduce<WARP, true>(m, red);
-    if (m > 3.4e38f) return 0.0f;  // an infinity: finite / inf, and inf * 0 = NaN where it stands
-    float t = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) t = fmaf(v[i] / m, v[i] / m, t);
-    t = row_reduce<WARP, false>(t, red);
-    return 1.0f / m / sqrtf(fmaf(t, inv_cols, eps / m / m));
-}
-// 1 / rms of the row whose elements the threads hold N each (zero past the end).
-template <bool WARP, int N>
-__device__ __forceinline__ float inverse_rms(const float (&v)[N], float inv_cols, float eps, float* red) {
+// Sum of N squares, pairwise.
+template <int N>
+__device__ __forceinline__ float square_sum(const float (&v)[N], float scale) {
     float q[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) q[i] = v[i] * v[i];
+    for (int i = 0; i < N; ++i) q[i] = (v[i] * scale) * (v[i] * scale);
 #pragma unroll
     for (int n = N / 2; n > 0; n >>= 1)
 #pragma unroll
         for (int i = 0; i < n; ++i) q[i] += q[i + n];
-    const float s = row_reduce<WARP, false>(q[0], red);
+    return q[0];
+}
+// inverse_rms for a row whose squares' sum left f32's range: its mean square lies between 2^112 (cols <= 2^14) and 2^256.  Such a
+// row is measured at 2^-80 of its size; above an rms of 2^100 it also goes on at 2^-64 (`shrink`, for the caller to apply to
+// its elements), or 1 / rms and its products with small weights would be subnormal.  An infinity gives 0 (finite / inf, and
+// inf * 0 = NaN where it stands), a NaN NaN.
+template <bool WARP, int N>
+__device__ __forceinline__ float inverse_rms_beyond(const float (&v)[N], float inv_cols, float eps, float* red, float& shrink) {
+    const float t = row_sum<WARP>(square_sum(v, 0x1p-80f), red);
+    const float inv = 1.0f / sqrtf(fmaf(t, inv_cols, eps * 0x1p-80f * 0x1p-80f));  // of the row at 2^-80, at least 2^-48
+    shrink = inv < 0x1p-20f ? 0x1p-64f : 1.0f;
+    return inv * (inv < 0x1p-20f ? 0x1p-16f : 0x1p-80f);
+}
+// 1 / rms of the row whose elements the threads hold N each (zero past the end; scaled down with it where they are too large).
+template <bool WARP, int N>
+__device__ __forceinline__ float inverse_rms(float (&v)[N], float inv_cols, float eps, float* red) {
+    const float s = row_sum<WARP>(square_sum(v, 1.0f), red);
     if (s <= 1e38f) return 1.0f / sqrtf(s * inv_cols + eps);
-    return inverse_rms_beyond<WARP>(v, s, inv_cols, eps, red);
+    float shrink;
+    const float inv = inverse_rms_beyond<WARP>(v, inv_cols, eps, red, shrink);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] *= shrink;
+    return inv;
 }
 
 // One row per warp (WARP: blockDim = 32 x rows) or per block; a thread holds NV packs of VEC elements.  AHEAD: weights are
@@ -211,11 +216,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_kernel(con
                     weights(a.pre_w, i, w);
                     P o;
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        float x = v[i * VEC + j] * inv;
-                        if (a.pre_w) x *= a.w_offset + w[j];
-                        o.v[j] = from_f32<T>(x);
-                    }
+                    for (int j = 0; j < VEC; ++j) o.v[j] = from_f32<T>(v[i * VEC + j] * (a.pre_w ? inv * (a.w_offset + w[j]) : inv));
                     *reinterpret_cast<P*>(static_cast<T*>(a.n_out) + (size_t)row * a.n_out_stride + (size_t)p * VEC) = o;
                 }
             }
@@ -275,7 +276,7 @@ __device__ __forceinline__ void put_pair(T* at, F2 v) {
 }
 // inverse_rms of elements held in pairs, by the whole block.
 template <int N>
-__device__ __forceinline__ float inverse_rms_pairs(const F2 (&v)[N], float inv_cols, float eps, float* red) {
+__device__ __forceinline__ float inverse_rms_pairs(F2 (&v)[N], float inv_cols, float eps, float* red) {
     F2 q[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) q[i] = mul2(v[i], v[i]);
@@ -284,7 +285,7 @@ __device__ __forceinline__ float inverse_rms_pairs(const F2 (&v)[N], float inv_c
 #pragma unroll
         for (int i = 0; i < n; ++i) q[i] = add2(q[i], q[i + n]);
     const float2 f = halves(q[0]);
-    const float s = row_reduce<false, false>(f.x + f.y, red);
+    const float s = row_sum<false>(f.x + f.y, red);
     if (s <= 1e38f) return 1.0f / sqrtf(s * inv_cols + eps);
     float e[2 * N];
 #pragma unroll
@@ -292,7 +293,11 @@ __device__ __forceinline__ float inverse_rms_pairs(const F2 (&v)[N], float inv_c
         const float2 h = halves(v[i]);
         e[2 * i] = h.x, e[2 * i + 1] = h.y;
     }
-    return inverse_rms_beyond<false>(e, s, inv_cols, eps, red);
+    float shrink;
+    const float inv = inverse_rms_beyond<false>(e, inv_cols, eps, red, shrink);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = mul2(v[i], pair(shrink, shrink));
+    return inv;
 }
 
 // Many long rows: a block walks its rows with the next one's operands on their way into shared memory (bulk copies), so

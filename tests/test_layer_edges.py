@@ -7,7 +7,7 @@ import torch
 
 import larql_b200
 from test_layer_moe import Layer, tokens
-from test_layer_ops import TYPES, U, gen, half_step
+from test_layer_ops import TYPES, U, check_norm, gen, half_step, norm_args, norm_case
 
 gpu = pytest.mark.gpu
 
@@ -96,3 +96,47 @@ def test_layer_with_every_expert_masked_is_nan(be, renorm):
     layer.bias[:] = -float("inf")
     out, _, w = layer.run(be, tokens(gen(2), 3, 64, "f32"))
     assert out[:3].isnan().all() and w.isnan().all()
+
+
+# ----------------------------------------------------------- block norm ----
+BIG = torch.finfo(torch.float32).max
+
+
+def large_rows(cols, g):
+    """f32 rows whose squares leave the type's range, up to the values at its end."""
+    r = torch.randn(8, cols, generator=g)
+    r[0] = torch.where(r[0] < 0, -BIG, BIG)      # the largest values throughout
+    r[1, 0], r[1, 1:] = -BIG, 1.0                # the lowest value, as a mask writes it, beside ordinary ones
+    r[2] = r[2].clamp(-3, 3) * 1e38
+    r[3] *= 1e37
+    r[3, cols // 2] = -BIG
+    r[4] *= 1e30
+    r[5] *= 1e20
+    r[6] = r[6].abs() * 3.0e37 + 1.0e38          # 1 / rms subnormal
+    return r
+
+
+@gpu
+@pytest.mark.parametrize("weight", [1.0, 1e-3, 1e-8, 1e3])
+@pytest.mark.parametrize("rows,cols", [(8, 256), (300, 200), (8, 512), (8, 2885), (8, 4096), (1300, 4096), (8, 16384), (1300, 2880)])
+@pytest.mark.parametrize("post", [True, False])
+def test_block_norm_at_the_end_of_f32(be, rows, cols, weight, post):
+    """Both norms, in every kernel (a warp a row, a block a row, blocks that walk many rows), of rows at the end of f32's range and
+    with weights that a subnormal 1 / rms would lose bits with."""
+    c = norm_case(rows, cols, "f32", "f32", post, "none", 0, 5, offset=0.0, y_scale=1.0)
+    big, plain = ("y", "h") if post else ("h", "y")
+    c[big][:8] = large_rows(cols, gen(cols)).cuda()
+    c[plain].zero_()
+    for k in ("post_w", "pre_w"):
+        c[k].copy_(weight * (1 + 0.2 * torch.randn(cols, generator=gen(7))))
+    h_out, n_out = torch.empty(rows, cols, device="cuda"), torch.empty(rows, cols, device="cuda")
+    torch.cuda.synchronize()
+    assert be.dev_block_norm(norm_args(c, h_out, n_out))
+    be.synchronize()
+    check_norm(c, h_out, n_out)
+    c[big][6, 3] = -float("inf")
+    torch.cuda.synchronize()
+    assert be.dev_block_norm(norm_args(c, h_out, n_out))
+    be.synchronize()
+    o = h_out if post else n_out
+    assert o[6, 3].isnan() and (o[6, :3] == 0).all() and (o[6, 4:] == 0).all()
