@@ -383,7 +383,8 @@ LQ_API int lq_moe_walk_ffn(lq_ctx* ctx, const lq_matrix* gates, const lq_matrix*
  * outputs is ordered against lq_stream(ctx) by the caller.  They may be captured into a graph on that stream; what a
  * call needs of the context's workspace has to be there already then (run the same call once before the capture:
  * "workspace growth during capture" otherwise), and graphs of one context share that workspace, so they are
- * replayed one after another.  Workspace a graph may hold stays allocated until lq_destroy.
+ * replayed one after another.  Workspace a graph may hold stays allocated until lq_destroy, a destroyed layer handle's
+ * too (not so the caller's matrices and activations).
  *
  * lq_dev_block_norm: the norms before and after a block, its gate and residual scale, in one pass over the rows:
  *     z  = y / rms(y) * (w_offset + post_w)           z = y when post_norm is 0; post_w NULL: unit weight

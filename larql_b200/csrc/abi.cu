@@ -78,6 +78,8 @@ struct lq_moe {
     size_t max_tokens = 0;     // per launch
     uint8_t* raw = nullptr;    // table and workspace, one allocation
     size_t sync_bytes = 0;     // the counters: from layer.exits on
+    bool captured = false;     // a graph holds the workspace's addresses: it stays until the context goes
+    bool gone = false;         // destroyed by its owner, not freed yet
 };
 
 struct lq_ctx {
@@ -829,7 +831,10 @@ void lq_destroy(lq_ctx* ctx) {
     cudaFree(ctx->tc_scratch);
     for (lq_ctx::OpBuf* b : {&ctx->op_codes, &ctx->op_part, &ctx->op_done}) cudaFree(b->p);
     for (void* p : ctx->retired) cudaFree(p);
-    for (lq_moe* m : ctx->moes) m->ctx = nullptr;  // (a handle that outlives its context frees its own memory)
+    for (lq_moe* m : ctx->moes) {
+        m->ctx = nullptr;  // (a handle that outlives its context frees its own memory)
+        if (m->gone) cudaFree(m->raw), delete m;
+    }
     cudaFree(ctx->stage);
     cudaFree(ctx->sort_buf);
     cudaFree(ctx->d_err);
@@ -2517,7 +2522,7 @@ int lq_moe_create(lq_ctx* ctx, const lq_matrix* gates, const lq_matrix* ups, con
 int lq_dev_moe_ffn(lq_ctx* ctx, lq_moe* moe, const void* x, int type, size_t tokens, void* out, uint32_t* idx_out, float* w_out) {
     DevGuard dev_guard(ctx);
     if (!ctx || !moe) return LQ_ERR_ARGUMENT;
-    if (moe->ctx != ctx) return fail(ctx, LQ_ERR_ARGUMENT, "moe: the handle belongs to another context");
+    if (moe->ctx != ctx || moe->gone) return fail(ctx, LQ_ERR_ARGUMENT, "moe: the handle belongs to another context");
     if (!float_type(type)) return fail(ctx, LQ_REFUSED_UNSUPPORTED, "moe: element type");
     if (tokens == 0) return LQ_OK;
     if (!x || !out) return fail(ctx, LQ_ERR_ARGUMENT, "moe: null pointer");
@@ -2526,6 +2531,11 @@ int lq_dev_moe_ffn(lq_ctx* ctx, lq_moe* moe, const void* x, int type, size_t tok
         return fail(ctx, LQ_ERR_ARGUMENT, "moe: pointer not aligned to its elements");
     const size_t H = (size_t)moe->layer.hidden, k = (size_t)moe->layer.top_e;
     if (tokens > 0x7fffffffu) return fail(ctx, LQ_REFUSED_UNSUPPORTED, "moe: too many tokens");
+    if (!moe->captured) {
+        cudaStreamCaptureStatus cs;
+        CK(cudaStreamIsCapturing(ctx->stream, &cs));
+        moe->captured = cs != cudaStreamCaptureStatusNone;
+    }
     if (k == 0) {
         CK(cudaMemsetAsync(out, 0, tokens * H * z, ctx->stream));
         return LQ_OK;
@@ -2567,12 +2577,16 @@ int lq_moe_ffn(lq_ctx* ctx, lq_moe* moe, const float* x, size_t x_len, size_t to
 void lq_moe_destroy(lq_ctx* ctx, lq_moe* moe) {
     if (!moe) return;
     DevGuard dev_guard(moe->ctx);
+    (void)ctx;
     if (moe->ctx) {
+        if (moe->captured) {
+            moe->gone = true;
+            return;
+        }
         cudaStreamSynchronize(moe->ctx->stream);
         auto& v = moe->ctx->moes;
         v.erase(std::remove(v.begin(), v.end(), moe), v.end());
     }
-    (void)ctx;
     cudaFree(moe->raw);
     delete moe;
 }

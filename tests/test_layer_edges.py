@@ -98,6 +98,37 @@ def test_layer_with_every_expert_masked_is_nan(be, renorm):
     assert out[:3].isnan().all() and w.isnan().all()
 
 
+@gpu
+def test_graph_outlives_its_layer():
+    """A graph that holds a layer's call is replayed after the handle was destroyed: the workspace it works in is still there,
+    and its counters in order, until the context goes."""
+    b = larql_b200.CudaBackend(0)
+    try:
+        layer = Layer(b, "mxfp4", 512, 96, 8, 2, "bf16", False, True, 5)
+        x, out = tokens(gen(1), 20, 512, "bf16"), torch.empty(20, 512, dtype=torch.bfloat16, device="cuda")
+        call = lambda: b.dev_moe_ffn(layer.layer, x.data_ptr(), larql_b200.T_BF16, 20, out.data_ptr())
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=torch.cuda.ExternalStream(b.stream()), capture_error_mode="thread_local"):
+            assert call()
+        assert call()
+        b.synchronize()
+        want = out.clone()
+        layer.layer.close()
+        other = [Layer(b, "mxfp4", 512, 96, 8, 2, "bf16", False, True, 6) for _ in range(3)]  # (what was freed would be theirs)
+        for o in other:
+            o.run(b, x)
+        out.zero_()
+        torch.cuda.synchronize()
+        for _ in range(2):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        del graph
+    finally:
+        b.close()
+
+
 # ----------------------------------------------------------- block norm ----
 BIG = torch.finfo(torch.float32).max
 
