@@ -458,6 +458,26 @@ int check_device_err(lq_ctx* ctx) {
     return fail(ctx, LQ_ERR_CUDA, "device-side internal error");
 }
 
+// Frees the destroyed layer handles: not during a capture of the context's stream (a later call does it), and not those that a
+// graph holds.
+void sweep_moes(lq_ctx* ctx) {
+    cudaStreamCaptureStatus cs;
+    if (cudaStreamIsCapturing(ctx->stream, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) return;
+    bool waited = false;
+    auto& v = ctx->moes;
+    for (size_t i = 0; i < v.size();) {
+        lq_moe* m = v[i];
+        if (!m->gone || m->captured) {
+            ++i;
+            continue;
+        }
+        if (!waited) cudaStreamSynchronize(ctx->stream), waited = true;
+        cudaFree(m->raw);
+        delete m;
+        v.erase(v.begin() + (ptrdiff_t)i);
+    }
+}
+
 bool float_type(int t) { return t == LQ_T_F32 || t == LQ_T_BF16 || t == LQ_T_F16; }
 size_t type_bytes(int t) { return t == LQ_T_F32 ? 4 : (t == LQ_T_E4M3 ? 1 : 2); }
 
@@ -2448,6 +2468,7 @@ int lq_moe_create(lq_ctx* ctx, const lq_matrix* gates, const lq_matrix* ups, con
     if (cs != cudaStreamCaptureStatusNone) return fail(ctx, LQ_ERR_ARGUMENT, "moe: create the layer outside a capture");
     const int64_t inter = gates[0].rows, hidden = gates[0].cols;
     std::vector<MoeExpert> table(n_experts);
+    sweep_moes(ctx);
     ctx->moes.reserve(ctx->moes.size() + 1);  // (nothing below throws while it holds device memory)
     for (size_t e = 0; e < n_experts; ++e) {
         const lq_matrix* m[3] = {gates + e, ups + e, downs + e};
@@ -2578,17 +2599,13 @@ void lq_moe_destroy(lq_ctx* ctx, lq_moe* moe) {
     if (!moe) return;
     DevGuard dev_guard(moe->ctx);
     (void)ctx;
-    if (moe->ctx) {
-        if (moe->captured) {
-            moe->gone = true;
-            return;
-        }
-        cudaStreamSynchronize(moe->ctx->stream);
-        auto& v = moe->ctx->moes;
-        v.erase(std::remove(v.begin(), v.end(), moe), v.end());
-    }
-    cudaFree(moe->raw);
-    delete moe;
+    // (a collector may destroy a handle while this thread captures something: waiting for a stream and freeing must not end that)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    moe->gone = true;
+    if (moe->ctx) sweep_moes(moe->ctx);
+    else cudaFree(moe->raw), delete moe;
+    cudaThreadExchangeStreamCaptureMode(&mode);
 }
 
 }  // extern "C"

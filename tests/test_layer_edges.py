@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import larql_b200
-from test_layer_moe import Layer, tokens
+from test_layer_moe import Layer, check, tokens
 from test_layer_ops import TYPES, U, check_norm, gen, half_step, norm_args, norm_case
 
 gpu = pytest.mark.gpu
@@ -124,6 +124,37 @@ def test_graph_outlives_its_layer():
             graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+        del graph
+    finally:
+        b.close()
+
+
+@gpu
+@pytest.mark.parametrize("where,mode", [("library", "thread_local"), ("library", "global"), ("torch", "thread_local"), ("torch", "global")])
+def test_layer_closed_during_a_capture(where, mode):
+    """A handle destroyed while its own stream, or another one, is being captured (a garbage collector picks its time) neither
+    ends the capture nor is lost."""
+    b = larql_b200.CudaBackend(0)
+    try:
+        layer, other = (Layer(b, "mxfp4", 64, 96, 4, 2, "f32", False, True, 5 + i) for i in range(2))
+        x = tokens(gen(1), 5, 64, "f32")
+        want, out = layer.run(b, x)[0][:5], torch.zeros(5, 64, device="cuda")
+        other.run(b, x)
+        stream = torch.cuda.ExternalStream(b.stream()) if where == "library" else torch.cuda.Stream()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode=mode):
+            if where == "library":
+                assert b.dev_moe_ffn(layer.layer, x.data_ptr(), larql_b200.T_F32, 5, out.data_ptr())
+            else:
+                out.copy_(want)
+            other.layer.close()
+        again = Layer(b, "mxfp4", 64, 96, 4, 2, "f32", False, True, 6)
+        check(again, x, again.run(b, x))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        b.synchronize()
         del graph
     finally:
         b.close()
