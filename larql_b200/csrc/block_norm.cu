@@ -313,7 +313,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_stream_ker
     const float inv_cols = 1.0f / (float)a.cols, eps = (float)a.eps;
     using P = Pack<T, VEC>;
     const uint32_t row_bytes = (uint32_t)a.cols * sizeof(T), stage = row_bytes * (gate_rows ? 3 : 2);
+    unsigned issued = 0;  // (thread 0)
     auto issue = [&](int s, int row) {  // h, y and the row's own gate row, behind one another
+        ++issued;
         uint8_t* dst = smem + (size_t)s * stage;
         mbar_expect_tx(&full[s], stage);
         tma_bulk_g2s(dst, static_cast<const T*>(a.h) + (size_t)row * a.h_stride, row_bytes, &full[s]);
@@ -444,7 +446,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_stream_ker
         s ^= 1;
         if (s == 0) phase ^= 1;
     }
-    if (!ok && tid == 0) set_err(a.err, DEV_ERR_TMA_TIMEOUT);
+    if (!ok) {  // (whichever thread's wait ran out)
+        set_err(a.err, DEV_ERR_TMA_TIMEOUT);
+        // the copies in flight have to land before the block's shared memory goes away
+        for (unsigned n = issued > 2 ? issued - 2 : 0; n < issued; ++n) mbar_wait(&full[n & 1], (n >> 1) & 1u);
+    }
 }
 
 template <class T, int VEC, int NV, bool SAME, int THREADS>
