@@ -160,6 +160,33 @@ def test_layer_closed_during_a_capture(where, mode):
         b.close()
 
 
+@gpu
+@pytest.mark.parametrize("kind,t", [("f32", 1), ("f32", 9), ("bf16", 9)])
+def test_moe_layer_scales_over_many_octaves(be, kind, t):
+    """MXFP4 scales of 2^-43 to 2^29, as far as no f32 in between overflows (at most 64 x 6 x 4 x 2^29 a product, 2^117 an
+    output): the formula's results, not only finite ones."""
+    layer = Layer(be, "mxfp4", 64, 64, 3, 2, kind, False, True, 8, spread=36)
+    x = tokens(gen(t), t, 64, kind).clamp_(-4, 4)
+    check(layer, x, layer.run(be, x))
+
+
+@gpu
+@pytest.mark.parametrize("shift,down_shift,x_shift", [(101, 0, -94), (0, 101, 0), (-117, 0, 117), (0, -117, 0)])
+def test_moe_layer_scales_at_the_ends(be, shift, down_shift, x_shift):
+    """MXFP4 scales of 2^92 to 2^96, above which a sum may leave f32's range, and of 2^-126 to 2^-122, on tokens that keep the
+    activation in range."""
+    layer = Layer(be, "mxfp4", 64, 64, 3, 2, "f32", True, True, 8)
+    layer.router.zero_()
+    for i, s in enumerate((shift, shift, down_shift)):
+        for e in range(3):
+            layer.keep[2 * (3 * i + e) + 1] += s
+            layer.w[i][e] = (*layer.w[i][e][:3], layer.w[i][e][3] * 2.0 ** s)
+    scales = torch.stack([layer.keep[2 * m + 1] for m in range(9)]).cpu()
+    assert 1 <= scales.min() and scales.max() <= 223
+    x = tokens(gen(5), 7, 64, "f32").clamp_(-4, 4) * 2.0 ** x_shift
+    check(layer, x, layer.run(be, x))
+
+
 # ----------------------------------------------------------- block norm ----
 BIG = torch.finfo(torch.float32).max
 
@@ -202,3 +229,18 @@ def test_block_norm_at_the_end_of_f32(be, rows, cols, weight, post):
     be.synchronize()
     o = h_out if post else n_out
     assert o[6, 3].isnan() and (o[6, :3] == 0).all() and (o[6, 4:] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("rows", [3, 1300])
+def test_block_norm_n_beside_an_eps_beyond_f32(be, rows):
+    """An eps of the size of squares that leave f32's range, in both norms: n to its bound."""
+    c = norm_case(rows, 4096, "f32", "f32", True, "none", 0, 5, y_scale=1.0)
+    c["h"].zero_()
+    c["y"].mul_(1e18)  # sum of squares 4e39, mean 1e36
+    c["eps"] = 1e36
+    h_out, n_out = torch.empty(rows, 4096, device="cuda"), torch.empty(rows, 4096, device="cuda")
+    torch.cuda.synchronize()
+    assert be.dev_block_norm(norm_args(c, h_out, n_out))
+    be.synchronize()
+    check_norm(c, h_out, n_out)
