@@ -426,15 +426,15 @@ LQ_API int lq_dev_fp8_quantize(lq_ctx* ctx, const void* x, int x_type, size_t to
 /* out[t, r] = sum_b sx[t,b] sw[r/128,b] sum_{k in block b} qx[t,k] qw[r,k] for an LQ_FMT_FP8_B128 matrix (device
  * resident, LQ_MAT_DEVICE).  x is quantised on the way as lq_dev_fp8_quantize does (x_scales NULL), or holds codes
  * already: x_type LQ_T_E4M3 with x_scales [tokens, ceil(cols / 128)] (16-byte aligned, x_stride a multiple of 16).
- * cols is a multiple of 16, the matrix's codes 16-byte aligned.  out [tokens, rows] of LQ_T_F32 / BF16 / F16,
- * out_stride elements between tokens; it may not overlap an input. */
+ * sx sw is formed first, in f32 (it has to lie in f32's range).  cols is a multiple of 16, the matrix's codes 16-byte
+ * aligned.  out [tokens, rows] of LQ_T_F32 / BF16 / F16, out_stride elements between tokens; it may not overlap an input. */
 LQ_API int lq_dev_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const void* x, int x_type, const float* x_scales,
                              size_t tokens, size_t x_stride, void* out, int out_type, size_t out_stride);
 /* The same with host pointers, f32 in and out (as lq_q4k_matmul): x [tokens, cols] -> out [tokens, rows]. */
 LQ_API int lq_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const float* x, size_t x_len, size_t tokens, float* out,
                          size_t out_len);
 
-/* A whole mixture-of-experts layer for a few tokens, one launch per 64 tokens (cpu_moe_forward,
+/* A whole mixture-of-experts layer for a few tokens, one launch per min(64, 1024 / top_e) tokens (cpu_moe_forward,
  * crates/larql-compute/src/cpu/ops/moe/forward.rs:24-140, over dense experts and with the router's product):
  *     logits = x . router^T + bias; the top_e experts by logit (ties to the lower index), softmax weights over all
  *     experts, renormalised over the selected when renormalise != 0 (a bias of -inf masks an expert: weight 0; an expert
@@ -444,7 +444,7 @@ LQ_API int lq_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const float* x, size_t
  *                one format (MXFP4, NVFP4, FP8_B128) and device resident (LQ_MAT_DEVICE), codes and FP4 scales 16-byte
  *                aligned; hidden and inter multiples of 32, at most 8192 (NVFP4: 6144); 1..256 experts, top_e <= 32.  router
  *                [n_experts, hidden] and router_bias [n_experts] (may be NULL) are device pointers of router_type.
- *                The handle keeps the pointers, not the data, and a workspace for 64 tokens; MXFP4 scales are looked
+ *                The handle keeps the pointers, not the data, and a workspace for a launch; MXFP4 scales are looked
  *                through once (an e8m0 NaN, 255, is refused).  Weights are immutable while a handle holds them.  Not
  *                during a capture (LQ_ERR_ARGUMENT).
  * lq_dev_moe_ffn x, out [tokens, hidden] of type (LQ_T_F32 / BF16 / F16; out may be x); idx_out, w_out [tokens,
@@ -452,6 +452,7 @@ LQ_API int lq_fp8_matmul(lq_ctx* ctx, const lq_matrix* w, const float* x, size_t
  * lq_moe_ffn     the same with host pointers, f32 (the handle's matrices stay on the device).
  * Both products take their activations in two f16 terms, off by at most 2^-23 of the value plus 2^-39 of the token's largest
  * (a bf16 x in one: 2^-39 alone); nothing between them is rounded to the layer's type.
+ * MXFP4 scales: 2^(byte - 127), a byte of 0 is 0 (as in the walk); scales above 2^96 (FP8_B128: 2^90) may leave f32's range.
  * A token with a NaN or infinity gets NaN outputs and weights; the other tokens are not touched by it. */
 typedef struct lq_moe lq_moe;
 LQ_API int lq_moe_create(lq_ctx* ctx, const lq_matrix* gates, const lq_matrix* ups, const lq_matrix* downs, size_t n_experts,

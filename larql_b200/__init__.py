@@ -663,7 +663,7 @@ class CudaBackend:
         return MoeLayer(self, h, gates[0].cols, min(int(top_e), n), (gates, ups, downs, keepalive)) if ok else None
 
     def dev_moe_ffn(self, layer: MoeLayer, x_ptr: int, x_type: int, tokens: int, out_ptr: int, idx_ptr: int = 0, w_ptr: int = 0):
-        """out [tokens, hidden] of the layer for x [tokens, hidden], one launch per 64 tokens."""
+        """out [tokens, hidden] of the layer for x [tokens, hidden], one launch per min(64, 1024 // top_e) tokens."""
         return self._status(self._lib.lq_dev_moe_ffn(self._h, layer.handle, x_ptr, x_type, tokens, out_ptr, idx_ptr or None,
                                                      w_ptr or None))
 
