@@ -11,7 +11,7 @@
 //   route    the T x E router products (twice f32's precision: which of two near logits is larger decides a whole
 //            expert), spread over the grid; then every CTA picks the experts itself;
 //   gate/up  units of 16 features of one expert for one group of its tokens: act = silu(gate) * up, f32, to global;
-//   down     units of 16 or 32 output rows, as soon as the expert's activations are complete (a counter per group, no
+//   down     units of 32 output rows, as soon as the expert's activations are complete (a counter per group, no
 //            grid barrier); when the last unit of all is done, the tokens' results are added up in selection order.
 // Warps have three jobs.  A producer streams the units' rows through a ring in shared memory (one tile copy per 16
 // rows); it needs only the routing, so it runs ahead from gate/up into down while the activations are still on
@@ -26,10 +26,10 @@
 // single one, which has all of its bits.  The terms are a column each, or, where a bf16 layer's group has too many tokens
 // for that behind gate/up, two sets of columns multiplied one after the other into the same sums.  Scales: e8m0 (per row
 // and 32) and FP8 blocks multiply the f32 sums of 32 products, e4m3 (per row and 16) the f16 codes, which is exact (2 + 4
-// bits).  (One term between the products of a bf16 layer: 106 and 167 us for the two cases of several tokens below, and f16's
+// bits).  (One term between the products of a bf16 layer saves about 5 us in the two cases of several tokens below and keeps
 // 11 bits of an activation.)
-// Measured: 32 MXFP4 experts of 2880 x 2880, 4 a token: 16 bf16 tokens 112 us for 373 MB, 3.3 TB/s; one f32 token 35 us for
-// 53 MB.  64 FP8 experts of 3840 x 800, 6 a token: 37 bf16 tokens 179 us for 576 MB, 3.2 TB/s.  The copies alone take 55, 9
+// Measured: 32 MXFP4 experts of 2880 x 2880, 4 a token: 16 bf16 tokens 107 us for 373 MB, 3.5 TB/s; one f32 token 33 us for
+// 53 MB.  64 FP8 experts of 3840 x 800, 6 a token: 37 bf16 tokens 173 us for 576 MB, 3.3 TB/s.  The copies alone take 55, 9
 // and 93 us: the compute warps' conversions and latencies bound it (integer pipe 51 %, an instruction in 58 % of the
 // cycles, tensor pipe 19 %), and for one token the routing's exchange between the CTAs and the two phases' starts.
 // (Tried: e4m3 terms and m16n8k32 e4m3 products, which need no conversion of FP8 codes: that form is converted to f16
@@ -247,7 +247,7 @@ __host__ __device__ constexpr int stage_cols(int k) { return chunk_cols<FMT>(k) 
 // One phase's products as the kernel walks them.
 struct Walk {
     int k, chunk, n_chunks, pitch;  // contraction, columns per stage, stages per unit, bytes between stage rows
-    int units_per_group, tiles;     // 16-row tiles per unit: 2 (gate + up, or 32 rows) or 1
+    int units_per_group;            // a unit is two tiles of 16 rows: gate and up, or 32 rows of down
     int is_down;
     uint8_t* scales;                // [slots] scales of a unit's rows
     int slots;
@@ -264,9 +264,10 @@ __device__ __forceinline__ Walk walk_of(const MoeLayer& L, bool down, int n_grou
     w.chunk = L.chunk[down];
     w.n_chunks = L.n_chunks[down];
     w.pitch = code_bytes<FMT>(w.chunk + 32);
-    // 32 rows a down unit share the loads of the activations; 16 when there are too few units to even the SMs out
-    w.tiles = !down || n_groups * (L.hidden / 32) >= 8 * (int)gridDim.x ? 2 : 1;
-    w.units_per_group = down ? L.hidden / (16 * w.tiles) : L.inter / 16;
+    // (units of 16 rows of down, which share the load out more evenly, were slower: both tiles take one load of the activations,
+    // and the code for one tile costs registers; one bf16 token on 32 MXFP4 experts of 2880 x 2880 33.3 against 31.5 us, 16
+    // tokens 126 against 108)
+    w.units_per_group = down ? L.hidden / 32 : L.inter / 16;
     // (at most 1024 groups of 512 units, 2^10 CTAs: 32 bits hold the products)
     const unsigned total = (unsigned)(n_groups * w.units_per_group);
     w.first = (int)(total * blockIdx.x / gridDim.x);
@@ -562,23 +563,23 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                         m0 = &ex.map[w.is_down ? 2 : 0], m1 = &ex.map[w.is_down ? 2 : 1];
                         sc0 = ex.scales[w.is_down ? 2 : 0], sc1 = ex.scales[w.is_down ? 2 : 1];
                     }
-                    const int row0 = (w.is_down ? tile * w.tiles : tile) * 16, row1 = w.is_down ? row0 + 16 : row0;
+                    const int row0 = tile * (w.is_down ? 32 : 16), row1 = w.is_down ? row0 + 16 : row0;
                     for (int c = 0; c < w.n_chunks; ++c, ++n) {
                         ok = ml_wait<true>(&sh.empty[st], lap ^ 1u);
                         if (!ok) break;
                         // (columns past the row's end arrive as zeros and count as bytes)
                         const bool with_scales = sbytes16 && c == 0;
-                        mbar_expect_tx(&sh.full[st], (code16 + (with_scales ? sbytes16 : 0u)) * w.tiles);
+                        mbar_expect_tx(&sh.full[st], (code16 + (with_scales ? sbytes16 : 0u)) * 2u);
                         uint8_t* dst = ring + (size_t)st * L.stage_bytes;
                         const int x = code_bytes<FMT>(c * w.chunk) / 4;
                         tma_load_2d(dst, m0, x, row0, &sh.full[st]);
-                        if (w.tiles == 2) tma_load_2d(dst + code16, m1, x, row1, &sh.full[st]);
+                        tma_load_2d(dst + code16, m1, x, row1, &sh.full[st]);
                         if (with_scales) {
                             // the unit's scales come with its first stage.  Their slot is free: the stage this one replaces was
                             // consumed, and scale_slots units do not fit between the two
                             uint8_t* sd = w.scales + slot * 2 * sbytes16;
                             tma_bulk_g2s(sd, sc0 + (size_t)(row0 >> 4) * sbytes16, sbytes16, &sh.full[st]);
-                            if (w.tiles == 2) tma_bulk_g2s(sd + sbytes16, sc1 + (size_t)(row1 >> 4) * sbytes16, sbytes16, &sh.full[st]);
+                            tma_bulk_g2s(sd + sbytes16, sc1 + (size_t)(row1 >> 4) * sbytes16, sbytes16, &sh.full[st]);
                         }
                         if (++st == L.n_stages) st = 0, lap ^= 1u;
                     }
@@ -674,12 +675,10 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                             const unsigned mine = __shfl_sync(0xffffffffu, m, (lane - j * per_tile) * terms * 4 & 31);
                             if (lane >= j * per_tile && lane < min(cnt, (j + 1) * per_tile)) top = max(top, mine);  // (columns past the group hold anything)
                         } else {
-                            float* o = L.pair_out + (size_t)at * L.hidden + tile * w.tiles * 16 + 4 * quad;
+                            float* o = L.pair_out + (size_t)at * L.hidden + tile * 32 + 4 * quad;
                             if (live) __stcg(reinterpret_cast<float4*>(o), a0);
-                            if (w.tiles == 2) {
-                                const float4 a1 = sums(all + RED, ts1);
-                                if (live) __stcg(reinterpret_cast<float4*>(o + 16), a1);
-                            }
+                            const float4 a1 = sums(all + RED, ts1);
+                            if (live) __stcg(reinterpret_cast<float4*>(o + 16), a1);
                         }
                     }
                     __syncwarp();
@@ -688,11 +687,9 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                 publish();
                 continue;
             }
-            // A compute warp takes every 16th block of the contraction, of both tiles; with one tile, two blocks at a time.
+            // A compute warp takes every 16th block of the contraction, of both tiles.
             constexpr bool F8 = FMT == LQ_FMT_FP8_B128;
-            const bool pairs = w.tiles == 1;
-            const int b0 = pairs && !F8 ? 2 * warp : warp;
-            const int tile2 = pairs ? 0 : 16 * w.pitch, scale2 = pairs ? 1 : 16 * srow;
+            const int tile2 = 16 * w.pitch, scale2 = 16 * srow;
             int cur = -1, cols = 0, slot = 0;
             uint32_t rest = 0;  // distance of the second set of columns (0: there is none)
             for (int u = ua; u < ub; ++u, ++tile) {
@@ -761,39 +758,36 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                 const uint32_t s0 = smem_u32(w.scales) + (uint32_t)(slot * 32 * srow + g * srow);
                 const float *fs = nullptr, *fs2 = nullptr;
                 if (F8) {
-                    const int row_blocks = (w.k + 127) >> 7, row = (w.is_down ? tile * w.tiles : tile) * 16;
+                    const int row_blocks = (w.k + 127) >> 7, row = tile * (w.is_down ? 32 : 16);
                     fs = reinterpret_cast<const float*>(L.table[e].scales[w.is_down ? 2 : 0]) + (size_t)(row >> 7) * row_blocks;
                     // (32 rows of a down unit start at a multiple of 32: one row of scale blocks)
                     fs2 = w.is_down ? fs : reinterpret_cast<const float*>(L.table[e].scales[1]) + (size_t)(row >> 7) * row_blocks;
                 }
-                // fragment rows: FP4: lanes 0-15 name the rows of the first block, 16-31 those of the second; FP8: the halves
+                // fragment rows: FP4: lanes 0-15 name the rows of the first tile, 16-31 those of the second; FP8: the halves
                 // of a block
-                const uint32_t frag = smem_u32(ring) + (uint32_t)((lane & 15) * w.pitch + (lane >> 4) * (F8 || pairs ? 16 : tile2));
+                const uint32_t frag = smem_u32(ring) + (uint32_t)((lane & 15) * w.pitch + (lane >> 4) * (F8 ? 16 : tile2));
                 const uint32_t xcol = smem_u32(xs) + (uint32_t)(g * xpitch + t4 * 16);
                 if (++slot == w.slots) slot = 0;
                 for (int c = 0; c < w.n_chunks; ++c) {
                     const int kb0 = c * (w.chunk / 32), blocks = min(w.chunk / 32, w.k / 32 - kb0);
                     if (ok) ok = __all_sync(0xffffffffu, ml_wait<false>(&sh.full[st], lap));
                     // addresses of the warp's first block; the others lie at constant distances
-                    const uint32_t ra = frag + (uint32_t)(st * L.stage_bytes + b0 * (F8 ? 32 : 16));
-                    const uint32_t sa = s0 + (FMT == LQ_FMT_NVFP4 ? 2 * (kb0 + b0) + (t4 >> 1) : kb0 + b0), sb = sa + 8 * srow;
-                    const uint32_t sc = sa + (FMT == LQ_FMT_NVFP4 && pairs ? 2 : scale2), sd = sc + 8 * srow;
-                    const uint32_t xa = xcol + (uint32_t)((kb0 + b0) * 64);
-                    // one step: block b0 + at of both tiles (PAIRS: blocks b0 + at and, `two`, b0 + at + D2 of the one tile), with
-                    // the second set of columns (SECOND)
-                    auto step = [&](auto second_tag, auto pairs_tag, int at, bool two) {
-                        constexpr bool PAIRS = decltype(pairs_tag)::value, SECOND = decltype(second_tag)::value;
-                        constexpr int D2 = PAIRS ? (F8 ? ML_WARPS : 1) : 0;
-                        // lo and hi: the f16 pairs of rows g and g + 8 of the first and the second block
+                    const uint32_t ra = frag + (uint32_t)(st * L.stage_bytes + warp * (F8 ? 32 : 16));
+                    const uint32_t sa = s0 + (FMT == LQ_FMT_NVFP4 ? 2 * (kb0 + warp) + (t4 >> 1) : kb0 + warp), sb = sa + 8 * srow;
+                    const uint32_t sc = sa + scale2, sd = sc + 8 * srow;
+                    const uint32_t xa = xcol + (uint32_t)((kb0 + warp) * 64);
+                    // one step: block warp + at of both tiles, with the second set of columns (SECOND)
+                    auto step = [&](auto second_tag, int at) {
+                        constexpr bool SECOND = decltype(second_tag)::value;
+                        // lo and hi: the f16 pairs of rows g and g + 8 of the first and the second tile
                         uint32_t lo[2][4], hi[2][4];
                         float f0[2] = {0.0f, 0.0f}, f1[2] = {0.0f, 0.0f};
-                        const int d2 = PAIRS && !two ? 0 : D2;  // (past the end the second repeats the first, scaled by zero)
                         if (F8) {
                             uint32_t r[2][4];
                             ldmatrix4(r[0], ra + at * 32);
-                            ldmatrix4(r[1], ra + tile2 + (at + d2) * 32);
-                            f0[0] = f1[0] = __ldg(fs + ((kb0 + b0 + at) >> 2));
-                            f0[1] = f1[1] = !PAIRS || two ? __ldg(fs2 + ((kb0 + b0 + at + d2) >> 2)) : 0.0f;
+                            ldmatrix4(r[1], ra + tile2 + at * 32);
+                            f0[0] = f1[0] = __ldg(fs + ((kb0 + warp + at) >> 2));
+                            f0[1] = f1[1] = __ldg(fs2 + ((kb0 + warp + at) >> 2));
 #pragma unroll
                             for (int q = 0; q < 2; ++q) {
                                 lo[q][0] = e4m3x2_f16(r[q][0]), lo[q][1] = e4m3x2_f16(r[q][0] >> 16);
@@ -804,9 +798,8 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                         } else {
                             constexpr int SB = FMT == LQ_FMT_NVFP4 ? 2 : 1;  // scales per block
                             uint32_t r[4];
-                            ldmatrix4(r, ra + at * 16);  // (one tile, past the end: any codes)
-                            const uint32_t u[4] = {lds_u8(sa + at * SB), lds_u8(sb + at * SB), !PAIRS || two ? lds_u8(sc + at * SB) : 0u,
-                                                   !PAIRS || two ? lds_u8(sd + at * SB) : 0u};
+                            ldmatrix4(r, ra + at * 16);
+                            const uint32_t u[4] = {lds_u8(sa + at * SB), lds_u8(sb + at * SB), lds_u8(sc + at * SB), lds_u8(sd + at * SB)};
                             if (FMT == LQ_FMT_MXFP4) {
                                 // 2^(byte - 127), 0 for 0 (e8m0_to_f32; a NaN scale was refused when the layer was made)
                                 f0[0] = __uint_as_float(u[0] << 23), f1[0] = __uint_as_float(u[1] << 23);
@@ -830,33 +823,31 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                         for (int j = 0; j < NT; ++j) {
                             if (NT > 1 && j >= cols) break;
                             const uint32_t xj = xa + j * 8 * xpitch + at * 64;
-                            const uint4 x0 = lds_128(xj);
-                            uint4 x1 = x0;
-                            if (PAIRS) x1 = lds_128(xj + d2 * 64);
+                            const uint4 x = lds_128(xj);
                             if (FMT == LQ_FMT_NVFP4) {
-                                mma_f16(acc[j], lo[0][0], hi[0][0], lo[0][1], hi[0][1], x0.x, x0.y);
-                                mma_f16(acc2[j], lo[1][0], hi[1][0], lo[1][1], hi[1][1], x1.x, x1.y);
-                                mma_f16(acc[j], lo[0][2], hi[0][2], lo[0][3], hi[0][3], x0.z, x0.w);
-                                mma_f16(acc2[j], lo[1][2], hi[1][2], lo[1][3], hi[1][3], x1.z, x1.w);
+                                mma_f16(acc[j], lo[0][0], hi[0][0], lo[0][1], hi[0][1], x.x, x.y);
+                                mma_f16(acc2[j], lo[1][0], hi[1][0], lo[1][1], hi[1][1], x.x, x.y);
+                                mma_f16(acc[j], lo[0][2], hi[0][2], lo[0][3], hi[0][3], x.z, x.w);
+                                mma_f16(acc2[j], lo[1][2], hi[1][2], lo[1][3], hi[1][3], x.z, x.w);
                                 if (SECOND) {
-                                    const uint4 y0 = lds_128(xj + rest), y1 = PAIRS ? lds_128(xj + d2 * 64 + rest) : y0;
-                                    mma_f16(acc[j], lo[0][0], hi[0][0], lo[0][1], hi[0][1], y0.x, y0.y);
-                                    mma_f16(acc2[j], lo[1][0], hi[1][0], lo[1][1], hi[1][1], y1.x, y1.y);
-                                    mma_f16(acc[j], lo[0][2], hi[0][2], lo[0][3], hi[0][3], y0.z, y0.w);
-                                    mma_f16(acc2[j], lo[1][2], hi[1][2], lo[1][3], hi[1][3], y1.z, y1.w);
+                                    const uint4 y = lds_128(xj + rest);
+                                    mma_f16(acc[j], lo[0][0], hi[0][0], lo[0][1], hi[0][1], y.x, y.y);
+                                    mma_f16(acc2[j], lo[1][0], hi[1][0], lo[1][1], hi[1][1], y.x, y.y);
+                                    mma_f16(acc[j], lo[0][2], hi[0][2], lo[0][3], hi[0][3], y.z, y.w);
+                                    mma_f16(acc2[j], lo[1][2], hi[1][2], lo[1][3], hi[1][3], y.z, y.w);
                                 }
                             } else {
                                 float d[4], h[4];
-                                mma_f16_new(d, lo[0][0], hi[0][0], lo[0][1], hi[0][1], x0.x, x0.y);
-                                mma_f16_new(h, lo[1][0], hi[1][0], lo[1][1], hi[1][1], x1.x, x1.y);
-                                mma_f16(d, lo[0][2], hi[0][2], lo[0][3], hi[0][3], x0.z, x0.w);
-                                mma_f16(h, lo[1][2], hi[1][2], lo[1][3], hi[1][3], x1.z, x1.w);
+                                mma_f16_new(d, lo[0][0], hi[0][0], lo[0][1], hi[0][1], x.x, x.y);
+                                mma_f16_new(h, lo[1][0], hi[1][0], lo[1][1], hi[1][1], x.x, x.y);
+                                mma_f16(d, lo[0][2], hi[0][2], lo[0][3], hi[0][3], x.z, x.w);
+                                mma_f16(h, lo[1][2], hi[1][2], lo[1][3], hi[1][3], x.z, x.w);
                                 if (SECOND) {
-                                    const uint4 y0 = lds_128(xj + rest), y1 = PAIRS ? lds_128(xj + d2 * 64 + rest) : y0;
-                                    mma_f16(d, lo[0][0], hi[0][0], lo[0][1], hi[0][1], y0.x, y0.y);
-                                    mma_f16(h, lo[1][0], hi[1][0], lo[1][1], hi[1][1], y1.x, y1.y);
-                                    mma_f16(d, lo[0][2], hi[0][2], lo[0][3], hi[0][3], y0.z, y0.w);
-                                    mma_f16(h, lo[1][2], hi[1][2], lo[1][3], hi[1][3], y1.z, y1.w);
+                                    const uint4 y = lds_128(xj + rest);
+                                    mma_f16(d, lo[0][0], hi[0][0], lo[0][1], hi[0][1], y.x, y.y);
+                                    mma_f16(h, lo[1][0], hi[1][0], lo[1][1], hi[1][1], y.x, y.y);
+                                    mma_f16(d, lo[0][2], hi[0][2], lo[0][3], hi[0][3], y.z, y.w);
+                                    mma_f16(h, lo[1][2], hi[1][2], lo[1][3], hi[1][3], y.z, y.w);
                                 }
 #pragma unroll
                                 for (int q = 0; q < 4; ++q) {
@@ -866,19 +857,11 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                             }
                         }
                     };
-                    const int left = blocks - b0;  // (at most 46 blocks a stage, 22 for FP8)
+                    const int left = blocks - warp;  // (at most 46 blocks a stage, 22 for FP8)
                     auto steps = [&](auto second) {
-                        if (!pairs) {
 #pragma unroll
-                            for (int i = 0; i < (F8 ? 2 : 3); ++i)
-                                if (i * ML_WARPS < left) step(second, std::false_type{}, i * ML_WARPS, true);
-                        } else if (F8) {
-                            if (left > 0) step(second, std::true_type{}, 0, left > ML_WARPS);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 2; ++i)
-                                if (i * 2 * ML_WARPS < left) step(second, std::true_type{}, i * 2 * ML_WARPS, left > i * 2 * ML_WARPS + 1);
-                        }
+                        for (int i = 0; i < (F8 ? 2 : 3); ++i)
+                            if (i * ML_WARPS < left) step(second, i * ML_WARPS);
                     };
                     // (apart: a branch inside a step would keep it from overlapping with the next)
                     if (SETS && rest) steps(std::integral_constant<bool, SETS>{});
@@ -896,12 +879,8 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     const int at[4] = {red_at(col, g), red_at(col + 1, g), red_at(col, g + 8), red_at(col + 1, g + 8)};
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        if (w.tiles == 2) {
-                            mine[at[q]] = acc[j][q];
-                            mine[RED + at[q]] = acc2[j][q];
-                        } else {
-                            mine[at[q]] = acc[j][q] + acc2[j][q];
-                        }
+                        mine[at[q]] = acc[j][q];
+                        mine[RED + at[q]] = acc2[j][q];
                     }
                 }
                 __syncwarp();
