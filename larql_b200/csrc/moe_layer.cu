@@ -23,10 +23,9 @@
 // The products run on the tensor cores (mma.sync m16n8k16, f16 x f16 -> f32): weights are the 16 rows of A, tokens the 8
 // columns of B.  The codes of all three formats are exact in f16.  An activation is brought to [2^14, 2^15) by a
 // power of two per token and held as two f16 terms (22 bits), in both products and for every type; only a bf16 x takes a
-// single one, which has all of its bits.  The terms are a column each, or, where a bf16 layer's group has too many tokens
-// for that behind gate/up, two sets of columns multiplied one after the other into the same sums.  Scales: e8m0 (per row
-// and 32) and FP8 blocks multiply the f32 sums of 32 products, e4m3 (per row and 16) the f16 codes, which is exact (2 + 4
-// bits).  (One term between the products of a bf16 layer saves about 5 us in the two cases of several tokens below and keeps
+// single one, which has all of its bits.  The terms are a column each, or, in a group of more than four tokens, two sets of
+// columns multiplied one after the other into the same sums.  Scales: e8m0 (per row and 32) and FP8 blocks multiply the
+// f32 sums of 32 products, e4m3 (per row and 16) the f16 codes, which is exact (2 + 4 bits).  (One term between the products of a bf16 layer saves about 5 us in the two cases of several tokens below and keeps
 // 11 bits of an activation.)
 // Measured: 32 MXFP4 experts of 2880 x 2880, 4 a token: 16 bf16 tokens 107 us for 373 MB, 3.5 TB/s; one f32 token 33 us for
 // 53 MB.  64 FP8 experts of 3840 x 800, 6 a token: 37 bf16 tokens 173 us for 576 MB, 3.3 TB/s.  The copies alone take 55, 9
@@ -221,15 +220,14 @@ __host__ __device__ constexpr int row_scale_bytes(int cols) {
 }
 // Distance of two columns of the activations: two columns (a phase of a 16-byte load) fall into different banks.
 __host__ __device__ constexpr int act_pitch(int k) { return (2 * k) % 128 == 0 ? 2 * k + 64 : 2 * k; }
-// Columns per activation of a group of cnt tokens: x has x_terms, the activation between the products two if `nt` tiles of
-// eight hold them (else one, and its second term lies in a second set of columns).
-__host__ __device__ constexpr int group_terms(int nt, int cnt, bool down, int x_terms) {
-    return down ? (2 * cnt <= 8 * nt ? 2 : 1) : x_terms;
-}
-// Bytes of a group's columns, whole tiles of eight, of one phase or the other.
-__host__ __device__ constexpr int act_bytes(int nt, int x_terms, int group, int hidden, int inter) {
-    const int x = (group * x_terms + 7) / 8 * 8 * act_pitch(hidden);
-    const int a = (group_terms(nt, group, true, x_terms) == 2 ? 1 : 2) * nt * 8 * act_pitch(inter);
+// Columns per activation of a group of cnt tokens: its terms if eight columns hold them, else one, and the second terms lie
+// in a second set of columns.
+__host__ __device__ constexpr int group_columns(int cnt, int terms) { return terms == 2 && cnt <= 4 ? 2 : 1; }
+__host__ __device__ constexpr int second_set(int cnt, int terms, int pitch) { return terms == 2 && cnt > 4 ? 8 * pitch : 0; }
+// Bytes of a group's columns, of one phase or the other.
+__host__ __device__ constexpr int act_bytes(int x_terms, int group, int hidden, int inter) {
+    const int x = 8 * act_pitch(hidden) + second_set(group, x_terms, act_pitch(hidden));
+    const int a = 8 * act_pitch(inter) + second_set(group, 2, act_pitch(inter));
     return x > a ? x : a;
 }
 // Columns of the contraction per stage: equal parts of at most 46 blocks of 32 (22 for FP8, and for long rows, whose
@@ -249,6 +247,7 @@ struct Walk {
     int k, chunk, n_chunks, pitch;  // contraction, columns per stage, stages per unit, bytes between stage rows
     int units_per_group;            // a unit is two tiles of 16 rows: gate and up, or 32 rows of down
     int is_down;
+    int terms;                      // f16 terms per activation
     uint8_t* scales;                // [slots] scales of a unit's rows
     int slots;
     int first, end;                 // this CTA's units
@@ -260,6 +259,7 @@ __device__ __forceinline__ Walk walk_of(const MoeLayer& L, bool down, int n_grou
     w.scales = sbuf + (down ? 32 * L.scale_slots[0] * row_scale_bytes<FMT>(L.hidden) : 0);
     w.slots = L.scale_slots[down];
     w.is_down = down;
+    w.terms = down ? 2 : L.x_terms;
     w.k = down ? L.inter : L.hidden;
     w.chunk = L.chunk[down];
     w.n_chunks = L.n_chunks[down];
@@ -376,17 +376,17 @@ __device__ void route_token(const MoeLayer& L, MlSmem& sh, int t, int lane) {
     }
 }
 
-// SETS: groups may have a second set of columns (a kernel of its own: the others would pay 2 to 9 us for the registers).
-template <int FMT, int NT, bool SETS>
+// SETS: groups may have a second set of columns.
+template <int FMT, bool SETS>
 __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_constant__ MoeLayer L) {
     extern __shared__ __align__(128) uint8_t smem[];
-    constexpr int RED = NT * 8 * 16;  // floats of a warp's partial sums of 16 rows
+    constexpr int RED = 8 * 16;  // floats of a warp's partial sums of 16 rows
     MlSmem& sh = *reinterpret_cast<MlSmem*>(smem);
     uint8_t* p = smem + (sizeof(MlSmem) + 127) / 128 * 128;
     float* red = reinterpret_cast<float*>(p);                 // [finish][ML_WARPS][2 tiles][RED]
     p += L.finish * ML_WARPS * 2 * RED * 4;
     uint8_t* xs = p;                                          // a group's columns of f16
-    p += act_bytes(NT, L.x_terms, L.group, L.hidden, L.inter);
+    p += act_bytes(L.x_terms, L.group, L.hidden, L.inter);
     uint8_t* sbuf = p;                                        // scales of the units' rows, [scale_slots] per phase
     p += 32 * (L.scale_slots[0] * row_scale_bytes<FMT>(L.hidden) + L.scale_slots[1] * row_scale_bytes<FMT>(L.inter));
     uint8_t* ring = smem + (p - smem + 127) / 128 * 128;      // [n_stages][32 rows]
@@ -416,6 +416,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
         constexpr int WARPS = ML_THREADS / 32;
         const int items = T * E;
         const bool r_wide = (reinterpret_cast<uintptr_t>(L.router) & 15) == 0;
+        // (1 | 4 | 20 warps an item: 32 items 41 | 35 | 34 us, 256 75 | 69 | 70, 1024 146 | 143 | 149, 4096 215 | 220 | 249)
         const int W = items <= (int)gridDim.x ? WARPS : (items <= 5 * (int)gridDim.x ? 4 : (items <= 10 * (int)gridDim.x ? 2 : 1));
         const int per_cta = WARPS / W, sub = warp / W, part = (warp % W) * 32 + lane;
         const int rounds = (items + (int)gridDim.x * per_cta - 1) / ((int)gridDim.x * per_cta);
@@ -636,50 +637,43 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     const int cnt = sh.cnt;
                     if (lane < cnt) pair = sh.gpair[lane];  // (lane i publishes what belongs to token i of the group)
                     const float* all = red + buf * ML_WARPS * 2 * RED;
-                    // eight columns at a time, a lane four rows of one column in both tiles; a token's two terms lie in two columns
-                    const int terms = group_terms(NT, cnt, w.is_down, L.x_terms);
-                    const int col = lane >> 2, quad = lane & 3, per_tile = 8 / terms;
+                    // a lane takes four rows of one column in both tiles; a token's two terms may lie in two columns
+                    const int per = group_columns(cnt, w.terms);
+                    const int col = lane >> 2, quad = lane & 3, i = col / per;
+                    const bool live = i < cnt && (per == 1 || (col & 1) == 0);
+                    const int at = sh.gpair[i < cnt ? i : 0];
+                    // (the routing weight goes into the power of two, so that only the weighted output has to be in range)
+                    const float scale = sh.unscale[i < cnt ? i : 0] * (w.is_down ? sh.w[at] : 1.0f);
+                    auto sums = [&](const float* part, float f) {  // the warps' parts in order
+                        const float* from = part + red_at(col, 4 * quad);
+                        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        if (j * per_tile >= cnt) break;
-                        const int i = j * per_tile + col / terms;
-                        const bool live = i < cnt && (terms == 1 || (col & 1) == 0);
-                        const int at = sh.gpair[i < cnt ? i : 0];
-                        // (the routing weight goes into the power of two, so that only the weighted output has to be in range)
-                        const float scale = sh.unscale[i < cnt ? i : 0] * (w.is_down ? sh.w[at] : 1.0f);
-                        auto sums = [&](const float* part, float f) {  // the warps' parts in order
-                            const float* from = part + red_at(j * 8 + col, 4 * quad);
-                            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                            for (int q = 0; q < ML_WARPS; ++q) {
-                                const float4 u = *reinterpret_cast<const float4*>(from + q * 2 * RED);
-                                v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-                            }
-                            if (terms == 2) {
-                                v.x += __shfl_xor_sync(0xffffffffu, v.x, 4), v.y += __shfl_xor_sync(0xffffffffu, v.y, 4);
-                                v.z += __shfl_xor_sync(0xffffffffu, v.z, 4), v.w += __shfl_xor_sync(0xffffffffu, v.w, 4);
-                            }
-                            return make_float4(v.x * scale * f, v.y * scale * f, v.z * scale * f, v.w * scale * f);
-                        };
-                        const float4 a0 = sums(all, ts0);
-                        if (!w.is_down) {
-                            const float4 a1 = sums(all + RED, ts1);
-                            auto silu = [](float g, float u) { return g / (1.0f + expf(-g)) * u; };
-                            const float4 act = make_float4(silu(a0.x, a1.x), silu(a0.y, a1.y), silu(a0.z, a1.z), silu(a0.w, a1.w));
-                            if (live) __stcg(reinterpret_cast<float4*>(L.act + (size_t)at * L.inter + tile * 16 + 4 * quad), act);
-                            // the pairs' largest |value| (a NaN's bits are above every number's)
-                            auto bits = [](float v) { return __float_as_uint(v) & 0x7fffffffu; };
-                            unsigned m = max(max(bits(act.x), bits(act.y)), max(bits(act.z), bits(act.w)));
-                            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                            const unsigned mine = __shfl_sync(0xffffffffu, m, (lane - j * per_tile) * terms * 4 & 31);
-                            if (lane >= j * per_tile && lane < min(cnt, (j + 1) * per_tile)) top = max(top, mine);  // (columns past the group hold anything)
-                        } else {
-                            float* o = L.pair_out + (size_t)at * L.hidden + tile * 32 + 4 * quad;
-                            if (live) __stcg(reinterpret_cast<float4*>(o), a0);
-                            const float4 a1 = sums(all + RED, ts1);
-                            if (live) __stcg(reinterpret_cast<float4*>(o + 16), a1);
+                        for (int q = 0; q < ML_WARPS; ++q) {
+                            const float4 u = *reinterpret_cast<const float4*>(from + q * 2 * RED);
+                            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
                         }
+                        if (per == 2) {
+                            v.x += __shfl_xor_sync(0xffffffffu, v.x, 4), v.y += __shfl_xor_sync(0xffffffffu, v.y, 4);
+                            v.z += __shfl_xor_sync(0xffffffffu, v.z, 4), v.w += __shfl_xor_sync(0xffffffffu, v.w, 4);
+                        }
+                        return make_float4(v.x * scale * f, v.y * scale * f, v.z * scale * f, v.w * scale * f);
+                    };
+                    const float4 a0 = sums(all, ts0), a1 = sums(all + RED, ts1);
+                    if (!w.is_down) {
+                        auto silu = [](float g, float u) { return g / (1.0f + expf(-g)) * u; };
+                        const float4 act = make_float4(silu(a0.x, a1.x), silu(a0.y, a1.y), silu(a0.z, a1.z), silu(a0.w, a1.w));
+                        if (live) __stcg(reinterpret_cast<float4*>(L.act + (size_t)at * L.inter + tile * 16 + 4 * quad), act);
+                        // the pairs' largest |value| (a NaN's bits are above every number's)
+                        auto bits = [](float v) { return __float_as_uint(v) & 0x7fffffffu; };
+                        unsigned m = max(max(bits(act.x), bits(act.y)), max(bits(act.z), bits(act.w)));
+                        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                        const unsigned mine = __shfl_sync(0xffffffffu, m, lane * per * 4 & 31);
+                        if (lane < cnt) top = max(top, mine);  // (columns past the group hold anything)
+                    } else if (live) {
+                        float* o = L.pair_out + (size_t)at * L.hidden + tile * 32 + 4 * quad;
+                        __stcg(reinterpret_cast<float4*>(o), a0);
+                        __stcg(reinterpret_cast<float4*>(o + 16), a1);
                     }
                     __syncwarp();
                     if (lane == 0) ml_arrive(&sh.rempty[buf]);
@@ -690,7 +684,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
             // A compute warp takes every 16th block of the contraction, of both tiles.
             constexpr bool F8 = FMT == LQ_FMT_FP8_B128;
             const int tile2 = 16 * w.pitch, scale2 = 16 * srow;
-            int cur = -1, cols = 0, slot = 0;
+            int cur = -1, slot = 0;
             uint32_t rest = 0;  // distance of the second set of columns (0: there is none)
             for (int u = ua; u < ub; ++u, ++tile) {
                 if (tile == w.units_per_group) {
@@ -704,9 +698,8 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     const int first = (gi - sh.gpre[a]) * TG;
                     const unsigned long long m0 = sh.mask[e][0] | ((unsigned long long)sh.mask[e][1] << 32);
                     const int cnt = min(TG, __popcll(m0) - first);
-                    const int terms = group_terms(NT, cnt, w.is_down, L.x_terms);
-                    cols = (cnt * terms + 7) / 8;
-                    if (SETS) rest = w.is_down && terms == 1 ? NT * 8 * xpitch : 0;
+                    const int columns = group_columns(cnt, w.terms);
+                    if (SETS) rest = second_set(cnt, w.terms, xpitch);
                     // the finishers are done with the previous group's units, the compute warps with its activations
                     for (int v = 0; v < L.finish; ++v)
                         if (ok) ok = __all_sync(0xffffffffu, ml_wait<false>(&sh.rempty[v], v < rb ? rlap : rlap ^ 1u));
@@ -745,16 +738,12 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                             to_f32(next[0], type, v);
                             next[0] = next[1];
                             if (k + per * 512 < w.k) next[1] = fetch(k + per * 512);
-                            put_columns<FMT>(v, scale, xs + (size_t)(i * terms) * xpitch, terms == 2 ? xpitch : (int)rest, k);
+                            put_columns<FMT>(v, scale, xs + (size_t)(i * columns) * xpitch, columns == 2 ? xpitch : (int)rest, k);
                         }
                     }
                     consumers_sync();
                 }
-                float acc[NT][4], acc2[NT][4];
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) acc[j][q] = acc2[j][q] = 0.0f;
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, acc2[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 const uint32_t s0 = smem_u32(w.scales) + (uint32_t)(slot * 32 * srow + g * srow);
                 const float *fs = nullptr, *fs2 = nullptr;
                 if (F8) {
@@ -819,41 +808,37 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                                 }
                             }
                         }
+                        const uint32_t xj = xa + at * 64;
+                        const uint4 x = lds_128(xj);
+                        if (FMT == LQ_FMT_NVFP4) {
+                            mma_f16(acc, lo[0][0], hi[0][0], lo[0][1], hi[0][1], x.x, x.y);
+                            mma_f16(acc2, lo[1][0], hi[1][0], lo[1][1], hi[1][1], x.x, x.y);
+                            mma_f16(acc, lo[0][2], hi[0][2], lo[0][3], hi[0][3], x.z, x.w);
+                            mma_f16(acc2, lo[1][2], hi[1][2], lo[1][3], hi[1][3], x.z, x.w);
+                            if (SECOND) {
+                                const uint4 y = lds_128(xj + rest);
+                                mma_f16(acc, lo[0][0], hi[0][0], lo[0][1], hi[0][1], y.x, y.y);
+                                mma_f16(acc2, lo[1][0], hi[1][0], lo[1][1], hi[1][1], y.x, y.y);
+                                mma_f16(acc, lo[0][2], hi[0][2], lo[0][3], hi[0][3], y.z, y.w);
+                                mma_f16(acc2, lo[1][2], hi[1][2], lo[1][3], hi[1][3], y.z, y.w);
+                            }
+                        } else {
+                            float d[4], h[4];
+                            mma_f16_new(d, lo[0][0], hi[0][0], lo[0][1], hi[0][1], x.x, x.y);
+                            mma_f16_new(h, lo[1][0], hi[1][0], lo[1][1], hi[1][1], x.x, x.y);
+                            mma_f16(d, lo[0][2], hi[0][2], lo[0][3], hi[0][3], x.z, x.w);
+                            mma_f16(h, lo[1][2], hi[1][2], lo[1][3], hi[1][3], x.z, x.w);
+                            if (SECOND) {
+                                const uint4 y = lds_128(xj + rest);
+                                mma_f16(d, lo[0][0], hi[0][0], lo[0][1], hi[0][1], y.x, y.y);
+                                mma_f16(h, lo[1][0], hi[1][0], lo[1][1], hi[1][1], y.x, y.y);
+                                mma_f16(d, lo[0][2], hi[0][2], lo[0][3], hi[0][3], y.z, y.w);
+                                mma_f16(h, lo[1][2], hi[1][2], lo[1][3], hi[1][3], y.z, y.w);
+                            }
 #pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            if (NT > 1 && j >= cols) break;
-                            const uint32_t xj = xa + j * 8 * xpitch + at * 64;
-                            const uint4 x = lds_128(xj);
-                            if (FMT == LQ_FMT_NVFP4) {
-                                mma_f16(acc[j], lo[0][0], hi[0][0], lo[0][1], hi[0][1], x.x, x.y);
-                                mma_f16(acc2[j], lo[1][0], hi[1][0], lo[1][1], hi[1][1], x.x, x.y);
-                                mma_f16(acc[j], lo[0][2], hi[0][2], lo[0][3], hi[0][3], x.z, x.w);
-                                mma_f16(acc2[j], lo[1][2], hi[1][2], lo[1][3], hi[1][3], x.z, x.w);
-                                if (SECOND) {
-                                    const uint4 y = lds_128(xj + rest);
-                                    mma_f16(acc[j], lo[0][0], hi[0][0], lo[0][1], hi[0][1], y.x, y.y);
-                                    mma_f16(acc2[j], lo[1][0], hi[1][0], lo[1][1], hi[1][1], y.x, y.y);
-                                    mma_f16(acc[j], lo[0][2], hi[0][2], lo[0][3], hi[0][3], y.z, y.w);
-                                    mma_f16(acc2[j], lo[1][2], hi[1][2], lo[1][3], hi[1][3], y.z, y.w);
-                                }
-                            } else {
-                                float d[4], h[4];
-                                mma_f16_new(d, lo[0][0], hi[0][0], lo[0][1], hi[0][1], x.x, x.y);
-                                mma_f16_new(h, lo[1][0], hi[1][0], lo[1][1], hi[1][1], x.x, x.y);
-                                mma_f16(d, lo[0][2], hi[0][2], lo[0][3], hi[0][3], x.z, x.w);
-                                mma_f16(h, lo[1][2], hi[1][2], lo[1][3], hi[1][3], x.z, x.w);
-                                if (SECOND) {
-                                    const uint4 y = lds_128(xj + rest);
-                                    mma_f16(d, lo[0][0], hi[0][0], lo[0][1], hi[0][1], y.x, y.y);
-                                    mma_f16(h, lo[1][0], hi[1][0], lo[1][1], hi[1][1], y.x, y.y);
-                                    mma_f16(d, lo[0][2], hi[0][2], lo[0][3], hi[0][3], y.z, y.w);
-                                    mma_f16(h, lo[1][2], hi[1][2], lo[1][3], hi[1][3], y.z, y.w);
-                                }
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) {
-                                    acc[j][q] = fmaf(d[q], q < 2 ? f0[0] : f1[0], acc[j][q]);
-                                    acc2[j][q] = fmaf(h[q], q < 2 ? f0[1] : f1[1], acc2[j][q]);
-                                }
+                            for (int q = 0; q < 4; ++q) {
+                                acc[q] = fmaf(d[q], q < 2 ? f0[0] : f1[0], acc[q]);
+                                acc2[q] = fmaf(h[q], q < 2 ? f0[1] : f1[1], acc2[q]);
                             }
                         }
                     };
@@ -872,16 +857,11 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                 }
                 if (ok) ok = __all_sync(0xffffffffu, ml_wait<false>(&sh.rempty[rb], rlap ^ 1u));
                 float* mine = red + (rb * ML_WARPS + warp) * 2 * RED;
+                const int col = 2 * t4, at[4] = {red_at(col, g), red_at(col + 1, g), red_at(col, g + 8), red_at(col + 1, g + 8)};
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    if (NT > 1 && j >= cols) break;
-                    const int col = j * 8 + 2 * t4;
-                    const int at[4] = {red_at(col, g), red_at(col + 1, g), red_at(col, g + 8), red_at(col + 1, g + 8)};
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        mine[at[q]] = acc[j][q];
-                        mine[RED + at[q]] = acc2[j][q];
-                    }
+                for (int q = 0; q < 4; ++q) {
+                    mine[at[q]] = acc[q];
+                    mine[RED + at[q]] = acc2[q];
                 }
                 __syncwarp();
                 if (lane == 0) ml_arrive(&sh.rfull[rb]);
@@ -924,9 +904,9 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
 }
 
 // Shared memory beside the ring and the scales, a unit's scales, a stage.
-size_t fixed_smem(int nt, int finish, int x_terms, int group, int hidden, int inter) {
-    return 128 + (sizeof(MlSmem) + 127) / 128 * 128 + finish * (size_t)ML_WARPS * 2 * nt * 8 * 16 * 4 +
-           (size_t)act_bytes(nt, x_terms, group, hidden, inter);
+size_t fixed_smem(int finish, int x_terms, int group, int hidden, int inter) {
+    return 128 + (sizeof(MlSmem) + 127) / 128 * 128 + finish * (size_t)ML_WARPS * 2 * 8 * 16 * 4 +
+           (size_t)act_bytes(x_terms, group, hidden, inter);
 }
 template <int FMT>
 int stage_size(int hidden, int inter) {
@@ -941,14 +921,14 @@ struct Plan {
 // The most stages that fit, with fewer finishers where that leaves under three.  Between a unit's first stage and the stage it
 // replaces lie at most stages / chunks units of a phase: so many slots its scales need, and one.
 template <int FMT>
-Plan plan_ring(int nt, int x_terms, int group, int hidden, int inter) {
+Plan plan_ring(int x_terms, int group, int hidden, int inter) {
     auto chunks = [](int k) { return (k + chunk_cols<FMT>(k) - 1) / chunk_cols<FMT>(k); };
     Plan p = {};
     for (int finish = ML_FINISH; finish >= 1; --finish) {
         for (int n = ML_MAX_STAGES; n >= 2; --n) {
             const int slots[2] = {(n + chunks(hidden) - 1) / chunks(hidden) + 1, (n + chunks(inter) - 1) / chunks(inter) + 1};
             const size_t scales = 32 * ((size_t)slots[0] * row_scale_bytes<FMT>(hidden) + (size_t)slots[1] * row_scale_bytes<FMT>(inter));
-            const size_t bytes = fixed_smem(nt, finish, x_terms, group, hidden, inter) + scales + (size_t)n * stage_size<FMT>(hidden, inter);
+            const size_t bytes = fixed_smem(finish, x_terms, group, hidden, inter) + scales + (size_t)n * stage_size<FMT>(hidden, inter);
             if (bytes <= 227 * 1024) {
                 if (n > p.stages) p = Plan{n, finish, {slots[0], slots[1]}, bytes};
                 break;
@@ -959,9 +939,9 @@ Plan plan_ring(int nt, int x_terms, int group, int hidden, int inter) {
     return p;
 }
 
-template <int FMT, int NT, bool SETS>
+template <int FMT, bool SETS>
 cudaError_t launch_layer(MoeLayer L, int sm_count, cudaStream_t st) {
-    const Plan p = plan_ring<FMT>(NT, L.x_terms, L.group, L.hidden, L.inter);
+    const Plan p = plan_ring<FMT>(L.x_terms, L.group, L.hidden, L.inter);
     if (p.stages == 0) return cudaErrorInvalidConfiguration;
     L.n_stages = p.stages, L.finish = p.finish, L.scale_slots[0] = p.slots[0], L.scale_slots[1] = p.slots[1];
     L.stage_bytes = stage_size<FMT>(L.hidden, L.inter);
@@ -970,7 +950,7 @@ cudaError_t launch_layer(MoeLayer L, int sm_count, cudaStream_t st) {
         L.chunk[i] = chunk_cols<FMT>(k);
         L.n_chunks[i] = (k + L.chunk[i] - 1) / L.chunk[i];
     }
-    const void* fn = (const void*)moe_layer_kernel<FMT, NT, SETS>;
+    const void* fn = (const void*)moe_layer_kernel<FMT, SETS>;
     cudaError_t e = set_max_dyn_smem(fn, 227 * 1024);
     if (e != cudaSuccess) return e;
     void* args[] = {&L};
@@ -980,28 +960,24 @@ cudaError_t launch_layer(MoeLayer L, int sm_count, cudaStream_t st) {
 template <int FMT>
 cudaError_t launch_fmt(MoeLayer L, int sm_count, cudaStream_t st) {
     L.x_terms = L.type == LQ_T_BF16 ? 1 : 2;
-    // a ring that covers the memory's latency beside the columns of a group
-    auto room = [&](int nt, int group) {
-        return (size_t)plan_ring<FMT>(nt, L.x_terms, group, L.hidden, L.inter).stages * stage_size<FMT>(L.hidden, L.inter) >= 48 * 1024;
-    };
-    // An expert with more tokens than a group holds is read once per group.  Groups of 8 instead of 4 tokens when an expert's
-    // tokens are likely to be more than 4 and shared memory takes them: by a second tile of columns, or for bf16 layers by a
-    // second set of them between the products.  Measured with 4 | 8, bf16 tokens on 32 MXFP4 experts of 2880 x 2880, 4 a
-    // token: 16 tokens 112 | 119 us, 24 141 | 138, 64 248 | 190.  (Groups of 16, with both, gain here and lose there:
-    // 8 NVFP4 experts of 2048 x 1024, 4 a token, 64 tokens 76 against 82 us, 16 tokens 49 against 45.)
-    const bool eight = 2 * L.tokens * L.top_e > 5 * L.experts && L.tokens > 4;
+    // An expert with more tokens than a group holds is read once per group; a second set of columns doubles a group's products,
+    // a bf16 layer's behind gate/up only.  Groups of 8 instead of 4 tokens by the tokens an expert is likely to have, where
+    // shared memory takes the second set.  Measured with 4 | 8, 32 MXFP4 experts of 2880 x 2880, 4 a token: bf16, 16 tokens
+    // 107 | 114 us, 24 135 | 132, 32 150 | 138; f32, 24 tokens 136 | 144, 32 151 | 151, 64 241 | 204; 64 FP8 experts of
+    // 3840 x 800, 6 a token, 37 tokens: bf16 186 | 173, f32 189 | 195.
+    const bool many = 2 * L.tokens * L.top_e > (L.x_terms == 1 ? 5 : 7) * L.experts && L.tokens > 4;
     L.group = 8;
-    if (L.x_terms == 2 && eight && room(2, 8)) return launch_layer<FMT, 2, false>(L, sm_count, st);
-    if (L.x_terms == 1 && eight && room(1, 8)) return launch_layer<FMT, 1, true>(L, sm_count, st);
+    if (many && plan_ring<FMT>(L.x_terms, L.group, L.hidden, L.inter).stages > 0)
+        return launch_layer<FMT, true>(L, sm_count, st);
     L.group = 4;
-    return launch_layer<FMT, 1, false>(L, sm_count, st);
+    return launch_layer<FMT, false>(L, sm_count, st);
 }
 
 }  // namespace
 
 template <int FMT>
 static bool fits(int hidden, int inter) {
-    return plan_ring<FMT>(1, 2, 4, hidden, inter).stages > 0;
+    return plan_ring<FMT>(2, 4, hidden, inter).stages > 0;
 }
 bool moe_layer_supported(int fmt, int hidden, int inter) {
     if (hidden <= 0 || inter <= 0 || hidden % 32 || inter % 32 || hidden > 8192 || inter > 8192) return false;
