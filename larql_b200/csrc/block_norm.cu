@@ -301,7 +301,7 @@ __device__ __forceinline__ float inverse_rms_pairs(F2 (&v)[N], float inv_cols, f
 }
 
 // Many long rows: a block walks its rows with the next one's operands on their way into shared memory (bulk copies), so
-// that the memory is never idle during a row's two reductions.  4096 x 8192 bf16 with a full gate: 64 us (5.2 TB/s) against 98
+// that the memory is never idle during a row's two reductions.  4096 x 8192 bf16 with a full gate: 60 us (5.6 TB/s) against 98
 // with loads into registers.
 template <class T, int VEC, int NV, bool SAME, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) block_norm_stream_kernel(const BlockNorm a, int gate_rows) {

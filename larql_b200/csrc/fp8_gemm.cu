@@ -7,7 +7,8 @@
 // scales change along the contraction, so a block's 128-long partial product (four K = 32 steps of tcgen05.mma
 // kind::f8f6f4, f32 accumulators in tensor memory) is read back, multiplied by its scale and added to an f32
 // accumulator in registers, while the tensor core works on the next block in another accumulator buffer.  The
-// partial products are exact sums of 8-bit products in f32; every other operation is one f32 fused multiply-add.
+// products are exact, their sum over a block is held in f32 with the tensor core's rounding (they span 2^-18 to 2^18); the
+// two scales' product is rounded to f32, and a block's sum enters by one f32 fused multiply-add.
 //
 // Two kernels, chosen by estimates of their time (way_of has the rule and what both measured):
 //   fp8_few_kernel    rows of the weight are the 128 lanes of an accumulator, tokens its 16, 32 or 64 columns.  What
@@ -488,9 +489,11 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 }
 
 // ----------------------------------------------------------- many tokens ----
-// What bounds it is tensor memory, which the product's accumulation and the promotion's reads share: a block (128 x 256 x
-// 128) takes 0.31 us of multiplication alone, 0.60 with its 128 KB read back.  4096 x 8192 -> 28672 in 1.02 ms, 1.9 PFLOP/s,
-// in a burst, 1.2 ms at the power limit.  Measured and not kept: pairs of CTAs on one tile (a third less to load: 1.06 ms),
+// What bounds it is the promotion: a block (128 x 256 x 128) takes 0.60 us, 0.59 with a quarter of its multiplications, and
+// 0.43 without the promotion.  What of the promotion costs that is not known: it reads the block's 128 KB from tensor
+// memory, from the barrier on and to the end before the next block's barrier, and its threads (96 registers at 640
+// threads) spill 400 to 976 bytes.  4096 x 8192 -> 28672 in 1.02 ms, 1.9 PFLOP/s, in a burst, 1.2 ms at the power limit.
+// Measured and not kept: pairs of CTAs on one tile (a third less to load: 1.06 ms),
 // accumulators handed over by halves (1.05), two multiply-adds an instruction (1.09), one arrival a warp (1.05).
 constexpr int MANY_M = 128, MANY_N = 256, MANY_STAGES = 4;
 constexpr int MANY_STAGE = (MANY_M + MANY_N) * 128;

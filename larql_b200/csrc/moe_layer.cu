@@ -28,8 +28,8 @@
 // f32 sums of 32 products, e4m3 (per row and 16) the f16 codes, which is exact (2 + 4 bits).  (One term between the products of a bf16 layer saves about 5 us in the two cases of several tokens below and keeps
 // 11 bits of an activation.)
 // Measured: 32 MXFP4 experts of 2880 x 2880, 4 a token: 16 bf16 tokens 107 us for 373 MB, 3.5 TB/s; one f32 token 33 us for
-// 53 MB.  64 FP8 experts of 3840 x 800, 6 a token: 37 bf16 tokens 173 us for 576 MB, 3.3 TB/s.  The copies alone take 55, 9
-// and 93 us: the compute warps' conversions and latencies bound it (integer pipe 51 %, an instruction in 58 % of the
+// 53 MB.  64 FP8 experts of 3840 x 800, 6 a token: 37 bf16 tokens 168 us for 576 MB, 3.4 TB/s.  The copies alone take 55, 9
+// and 93 us: the compute warps' conversions and latencies bound it (integer pipe 47 %, an instruction in 56 % of the
 // cycles, tensor pipe 19 %), and for one token the routing's exchange between the CTAs and the two phases' starts.
 // (Tried: e4m3 terms and m16n8k32 e4m3 products, which need no conversion of FP8 codes: that form is converted to f16
 // behind the instruction, 32 cycles of a scheduler against 2 x 8.)
@@ -145,9 +145,6 @@ __device__ __forceinline__ unsigned add_release(unsigned* word, unsigned n) {
     unsigned before;
     asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], %2;" : "=r"(before) : "l"(word), "r"(n) : "memory");
     return before;
-}
-__device__ __forceinline__ void ml_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -676,7 +673,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                         __stcg(reinterpret_cast<float4*>(o + 16), a1);
                     }
                     __syncwarp();
-                    if (lane == 0) ml_arrive(&sh.rempty[buf]);
+                    if (lane == 0) mbar_arrive_one(&sh.rempty[buf]);
                 }
                 publish();
                 continue;
@@ -852,7 +849,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     if (SETS && rest) steps(std::integral_constant<bool, SETS>{});
                     else steps(std::false_type{});
                     __syncwarp();
-                    if (lane == 0) ml_arrive(&sh.empty[st]);
+                    if (lane == 0) mbar_arrive_one(&sh.empty[st]);
                     if (++st == L.n_stages) st = 0, lap ^= 1u;
                 }
                 if (ok) ok = __all_sync(0xffffffffu, ml_wait<false>(&sh.rempty[rb], rlap ^ 1u));
@@ -864,7 +861,7 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                     mine[RED + at[q]] = acc2[q];
                 }
                 __syncwarp();
-                if (lane == 0) ml_arrive(&sh.rfull[rb]);
+                if (lane == 0) mbar_arrive_one(&sh.rfull[rb]);
                 if (++rb == L.finish) rb = 0, rlap ^= 1u;
             }
         }
