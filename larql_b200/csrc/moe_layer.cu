@@ -559,6 +559,8 @@ __global__ void __launch_bounds__(ML_THREADS, 1) moe_layer_kernel(const __grid_c
                         a = expert_of(sh, gi, max(a, 0));
                         const MoeExpert& ex = L.table[sh.active[a]];
                         m0 = &ex.map[w.is_down ? 2 : 0], m1 = &ex.map[w.is_down ? 2 : 1];
+                        tma_acquire_map(m0);
+                        if (!w.is_down) tma_acquire_map(m1);
                         sc0 = ex.scales[w.is_down ? 2 : 0], sc1 = ex.scales[w.is_down ? 2 : 1];
                     }
                     const int row0 = tile * (w.is_down ? 32 : 16), row1 = w.is_down ? row0 + 16 : row0;

@@ -187,6 +187,19 @@ def test_moe_layer_scales_at_the_ends(be, shift, down_shift, x_shift):
     check(layer, x, layer.run(be, x))
 
 
+@gpu
+@pytest.mark.parametrize("fmt", ["mxfp4", "fp8"])
+def test_layers_made_one_after_another_in_the_same_memory(be, fmt):
+    """Layers made, run and destroyed in turn: the table and the tensor maps of each mostly lie where the last one's did, and
+    describe other matrices of other sizes."""
+    for i in range(12):
+        hidden, inter = (256, 96) if i % 3 else (96, 256)
+        layer = Layer(be, fmt, hidden, inter, 6, 2, "bf16", False, True, 40 + i)
+        x = tokens(gen(i), 1 + 3 * (i % 4), hidden, "bf16")
+        check(layer, x, layer.run(be, x))
+        layer.layer.close()
+
+
 # ----------------------------------------------------------- block norm ----
 BIG = torch.finfo(torch.float32).max
 
